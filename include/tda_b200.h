@@ -243,6 +243,114 @@ int tda_debug_set(int inject, uint64_t wait_timeout_ns);
  * in neither).  NULL turns it off (the default).  Process-wide setting. */
 int tda_debug_stats(void* counters);
 
+/* ------------------------------------------------------------------------
+ * Softmax differential attention: out = (P1 - lambda P2) v with
+ * P_m = softmax(scale q_m k_m^T) over the keys a query row sees: j <
+ * key_lengths[b] (all when NULL) and, when causal, j <= i + k_len - q_len.  A
+ * row that sees no key gives zeros (and no gradient).
+ *
+ * q1, q2: (batch, heads, q_len, head_dim); k1, k2, v: (batch, kv_heads, k_len,
+ * head_dim), query head h reads kv head h / (heads / kv_heads).  strides:
+ * element strides of the batch, head and sequence dimensions of q1, q2, k1,
+ * k2, v (15 values, positive multiples of 8) or NULL for contiguous arrays.
+ * out: contiguous, of the inputs' type.  For a later backward also o12 (fp32
+ * [2][batch][heads][q_len][head_dim]: P1 v and P2 v) and lse (fp32
+ * [2][batch][heads][q_len]: log2 of each map's row sum of 2^(log2(e) scale s),
+ * +infinity for a row without keys); both NULL when no gradient is wanted.
+ * lambda: device values of lambda_dtype at b * lambda_stride_b + h *
+ * lambda_stride_h (used as they are, not clamped), or NULL for lambda_value.
+ * bf16 and fp16 with head_dim 64 or 128 run on the tcgen05 tensor cores, fp32
+ * and other head dims (a power of two in [16, 256]) on the CUDA cores in fp32.
+ * ------------------------------------------------------------------------ */
+int tda_sdiff_fwd(const void* q1, const void* q2, const void* k1, const void* k2, const void* v,
+                  const int64_t* strides, void* out, float* o12, float* lse, int dtype, int64_t batch, int64_t heads,
+                  int64_t kv_heads, int64_t q_len, int64_t k_len, int64_t head_dim, float scale, int causal,
+                  const int32_t* key_lengths, const void* lambda, int lambda_dtype, int64_t lambda_stride_b,
+                  int64_t lambda_stride_h, float lambda_value, int* status, void* stream);
+
+/* Bytes of device scratch tda_sdiff_bwd needs. */
+size_t tda_sdiff_bwd_workspace_size(int64_t batch, int64_t heads, int64_t q_len);
+
+/* Gradients of tda_sdiff_fwd, of the inputs' type and contiguous: dq1, dq2
+ * like q1, dk1, dk2, dv like v (summed over the heads that share them), and
+ * dlam (fp32 (batch, heads), or NULL).  o12 and lse are the forward's;
+ * dout_strides: 3 values or NULL.  Deterministic: no atomic sums. */
+int tda_sdiff_bwd(const void* q1, const void* q2, const void* k1, const void* k2, const void* v,
+                  const int64_t* strides, const void* dout, const int64_t* dout_strides,
+                  const float* o12, const float* lse, void* dq1, void* dq2, void* dk1, void* dk2, void* dv, float* dlam,
+                  int dtype, int64_t batch, int64_t heads, int64_t kv_heads, int64_t q_len, int64_t k_len,
+                  int64_t head_dim, float scale, int causal, const int32_t* key_lengths, const void* lambda,
+                  int lambda_dtype, int64_t lambda_stride_b, int64_t lambda_stride_h, float lambda_value,
+                  void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The 4-bit paged cache and attention over it (one new token a request).
+ *
+ * cache: device array of num_pages x kv_heads blocks of
+ * tda_cache4_block_bytes(page_size, head_dim) bytes, zeroed once by the
+ * caller; page_size 16, 32, 64 or 128, head_dim 64 or 128, num_pages *
+ * page_size below 2^31.  Slot s is row s % page_size of page s / page_size.
+ * Elements are held in groups of 32 along the head dimension as codes
+ * round(7 x / amax) (half to even) and a bf16 scale amax / 7; a group that
+ * holds an infinity or a NaN reads back as NaN.  With normalize_keys the
+ * scales of k1 and k2 are multiplied by 1 / max(||k||_2, 1e-12).
+ * ------------------------------------------------------------------------ */
+
+/* Bytes of one (page, kv head) block; 0 for an unsupported size. */
+size_t tda_cache4_block_bytes(int64_t page_size, int64_t head_dim);
+
+/* Page plan of one step, built on the device.  Request r holds lengths[r]
+ * tokens in its first ceil(lengths[r] / page_size) entries of block_table
+ * ((requests, table_width) int32, rows table_stride apart) and receives
+ * new_tokens[r] more.  Fresh pages are taken from free_pages[*free_head ...
+ * num_free) in request order and written into the table.  Row i of the packed
+ * new tokens gets its slot, position and request; slots is -1 for a token that
+ * found no page (list or table exhausted), all three are -1 for rows past the
+ * last token.  starts ((requests + 1) prefix sums of new_tokens), lengths_out
+ * (tokens held afterwards), *free_head_out and *dropped (tokens that found no
+ * page) describe the step; outputs must not overlap inputs. */
+int tda_plan_pages(const int32_t* lengths, const int32_t* new_tokens, int64_t requests, int32_t* block_table,
+                   int64_t table_stride, int64_t table_width, const int32_t* free_pages, int64_t num_free,
+                   const int32_t* free_head, int64_t page_size, int64_t rows, int32_t* slots, int32_t* positions,
+                   int32_t* request_ids, int32_t* starts, int32_t* lengths_out, int32_t* free_head_out,
+                   int32_t* dropped, void* stream);
+
+/* Quantise (tokens, kv_heads, head_dim) rows into their slots; a slot outside
+ * the cache (-1) is skipped, slots of one call are distinct.  strides: token
+ * and head element strides of k1, k2, v (6 values, multiples of 8) or NULL for
+ * contiguous rows. */
+int tda_cache4_append(const void* k1, const void* k2, const void* v, int dtype, const int64_t* strides,
+                      const int32_t* slots, int64_t tokens, void* cache, int64_t num_pages, int64_t kv_heads,
+                      int64_t head_dim, int64_t page_size, int normalize_keys, void* stream);
+
+/* The values slots hold, as contiguous (tokens, kv_heads, head_dim) rows of
+ * dtype; zeros for a slot outside the cache. */
+int tda_cache4_read(const void* cache, int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                    const int32_t* slots, int64_t tokens, void* k1, void* k2, void* v, int dtype, void* stream);
+
+#define TDA_MAP_SOFTMAX 0
+#define TDA_MAP_THRESHOLD 1
+
+/* Device scratch of tda_cache4_attention (may be 0). */
+size_t tda_cache4_workspace_size(int map, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                 int64_t page_size, int64_t table_width);
+
+/* One query token a request over its lengths[b] cached tokens:
+ *   TDA_MAP_SOFTMAX:   (softmax(scale q1.k1) - lambda softmax(scale q2.k2)) v
+ *   TDA_MAP_THRESHOLD: (P1 - clamp(lambda, 0, 1) P2) v, P = relu(q.k - tau)^relu_power,
+ *                      tau = beta sqrt(2 ln(lengths[b]) / head_dim); normalize divides q by its norm
+ * q1, q2: (batch, heads, head_dim) bf16 / fp16, q_strides = batch and head
+ * strides of q1 and of q2 (4 values) or NULL; out contiguous, of q's type.
+ * lambda: device values of lambda_dtype at b * lambda_stride_b + h *
+ * lambda_stride_h, or NULL for lambda_value.  A request of length 0 gives
+ * zeros; table entries outside the cache are skipped. */
+int tda_cache4_attention(int map, const void* q1, const void* q2, int dtype, const int64_t* q_strides, void* out,
+                         int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, const void* cache,
+                         int64_t num_pages, int64_t page_size, const int32_t* block_table, int64_t table_stride,
+                         int64_t table_width, const int32_t* lengths, const void* lambda, int lambda_dtype,
+                         int64_t lambda_stride_b, int64_t lambda_stride_h, float lambda_value, float scale, float beta,
+                         float relu_power, int normalize, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,21 @@ from .ops import (  # noqa: F401
     rect_forward,
     threshold_rela_triton,
 )
+from .cache4 import (  # noqa: F401
+    Cache4,
+    PagePlan,
+    cache4_append,
+    cache4_read,
+    cache4_softmax_attention,
+    cache4_threshold_attention,
+    plan_pages,
+)
+from .sdiff import (  # noqa: F401
+    DifferentialSoftmaxFunction,
+    differential_softmax_attention,
+    sdiff_backward,
+    sdiff_forward,
+)
 
 __all__ = [
     "threshold_rela_triton",
@@ -24,4 +39,15 @@ __all__ = [
     "rect_backward",
     "diff_forward",
     "check_status",
+    "differential_softmax_attention",
+    "DifferentialSoftmaxFunction",
+    "sdiff_forward",
+    "sdiff_backward",
+    "Cache4",
+    "PagePlan",
+    "plan_pages",
+    "cache4_append",
+    "cache4_read",
+    "cache4_softmax_attention",
+    "cache4_threshold_attention",
 ]

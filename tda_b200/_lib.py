@@ -15,6 +15,9 @@ TDA_F32 = 0
 TDA_BF16 = 1
 TDA_F16 = 2
 
+TDA_MAP_SOFTMAX = 0
+TDA_MAP_THRESHOLD = 1
+
 TDA_OK = 0
 TDA_ERR_INVALID = -1
 TDA_ERR_UNSUPPORTED = -2
@@ -47,6 +50,16 @@ SIGNATURES = {
                                  _I, _P, _SZ, _P, _P]),
     "tda_bwd_workspace_size": (_SZ, [_I, _I64, _I64, _I64, _I]),
     "tda_rect_bwd": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _F, _F, _I, _F, _I, _P, _SZ, _P, _P]),
+    "tda_sdiff_fwd": (_I, [_P] * 9 + [_I] + [_I64] * 6 + [_F, _I, _P, _P, _I, _I64, _I64, _F, _P, _P]),
+    "tda_sdiff_bwd_workspace_size": (_SZ, [_I64, _I64, _I64]),
+    "tda_sdiff_bwd": (_I, [_P] * 16 + [_I] + [_I64] * 6 + [_F, _I, _P, _P, _I, _I64, _I64, _F, _P, _SZ, _P, _P]),
+    "tda_cache4_block_bytes": (_SZ, [_I64, _I64]),
+    "tda_plan_pages": (_I, [_P, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64] + [_P] * 8),
+    "tda_cache4_append": (_I, [_P, _P, _P, _I, _P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I, _P]),
+    "tda_cache4_read": (_I, [_P, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I, _P]),
+    "tda_cache4_workspace_size": (_SZ, [_I, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "tda_cache4_attention": (_I, [_I, _P, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
+                                  _I, _I64, _I64, _F, _F, _F, _F, _I, _P, _SZ, _P]),
 }
 
 _lib = None

@@ -1,0 +1,531 @@
+// The 4-bit paged cache: page plan of a serving step, append (quantise and
+// scatter) and read (gather and widen), with their C entry points.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tda_cache4.cuh"
+#include "tda_host.h"
+
+namespace tda {
+namespace {
+
+// ================================================================== page plan
+// Request r holds len[r] tokens in ceil(len / page) pages and gets new[r] more.
+// Pages wanted are handed out in request order from free[head..]; a request
+// that the list cannot serve keeps what it got and drops its last tokens.
+struct PlanParams {
+  const int* lengths;
+  const int* added;
+  int* table;
+  const int* free_pages;
+  const int* free_head;
+  int* slots;
+  int* positions;
+  int* requests;
+  int* starts;
+  int* lengths_out;
+  int* free_head_out;
+  int* dropped;
+  long long table_stride;
+  int B;
+  int width;
+  int n_free;
+  int page;
+  int rows;
+};
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanRound = 2048;  // requests scanned at a time
+constexpr int kPlanRows = 2048;   // token rows of one block
+
+// Exclusive prefix sums of (a, b) over the block and their totals.
+__device__ void block_scan2(int& a, int& b, int& ta, int& tb, int2* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int a0 = a, b0 = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) {
+      a += x;
+      b += y;
+    }
+  }
+  if (lane == 31) warp_sums[warp] = make_int2(a, b);
+  __syncthreads();
+  int pa = 0, pb = 0;
+  ta = tb = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    const int2 s = warp_sums[w];
+    if (w < warp) {
+      pa += s.x;
+      pb += s.y;
+    }
+    ta += s.x;
+    tb += s.y;
+  }
+  a += pa - a0;
+  b += pb - b0;
+  __syncthreads();
+}
+
+// Every block scans all requests (a few KB from L2) and then writes its own
+// rows, so the plan is one launch.  The table entries of request r are written
+// by block r % gridDim.x; rows take fresh pages from the free list itself, so
+// no block reads an entry that another one writes.
+__global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanParams p) {
+  __shared__ int s_start[kPlanRound + 1], s_first[kPlanRound], s_len[kPlanRound], s_after[kPlanRound],
+      s_got[kPlanRound];
+  __shared__ int2 warp_sums[kPlanThreads / 32];
+  const int tid = threadIdx.x;
+  const int head = max(0, *p.free_head);
+  const int left = max(0, p.n_free - head);
+  const long long row0 = static_cast<long long>(blockIdx.x) * kPlanRows;
+  const int row_end = static_cast<int>(min(static_cast<long long>(p.rows), row0 + kPlanRows));
+  int base_tok = 0, base_page = 0, kept = 0, taken = 0;
+  constexpr int kPer = kPlanRound / kPlanThreads;
+  for (int r0 = 0; r0 < p.B; r0 += kPlanRound) {
+    const int n = min(kPlanRound, p.B - r0);
+    int add[kPer], want[kPer], held[kPer], sa = 0, sw = 0, ta, tw;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = tid * kPer + i;
+      add[i] = want[i] = held[i] = 0;
+      if (r < n) {
+        const int len = max(0, min(p.lengths[r0 + r], p.width * p.page));  // a table holds no more
+        add[i] = max(0, p.added[r0 + r]);
+        held[i] = (len + p.page - 1) / p.page;
+        const long long last = (static_cast<long long>(len) + add[i] + p.page - 1) / p.page;
+        want[i] = static_cast<int>(min(last, static_cast<long long>(p.width))) - held[i];
+        s_len[r] = len;
+      }
+      sa += add[i];
+      sw += want[i];
+    }
+    block_scan2(sa, sw, ta, tw, warp_sums);
+    sa += base_tok;
+    sw += base_page;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = tid * kPer + i;
+      if (r < n) {
+        const int got = min(want[i], max(0, left - sw));
+        const int len = s_len[r];
+        const int after = static_cast<int>(min(static_cast<long long>(len) + add[i],
+                                               static_cast<long long>(held[i] + got) * p.page));
+        s_start[r] = sa;
+        s_first[r] = sw;
+        s_after[r] = after;
+        s_got[r] = got;
+        kept += after - len;
+        taken += got;
+        if (blockIdx.x == 0) {
+          p.starts[r0 + r] = sa;
+          p.lengths_out[r0 + r] = after;
+        }
+      }
+      sa += add[i];
+      sw += want[i];
+    }
+    base_tok += ta;
+    base_page += tw;
+    if (tid == 0) s_start[n] = base_tok;
+    __syncthreads();
+    // fresh table entries: a warp a request
+    for (int r = blockIdx.x + (tid >> 5) * gridDim.x; r < n; r += gridDim.x * (kPlanThreads / 32)) {
+      const int held0 = (s_len[r] + p.page - 1) / p.page;
+      for (int c = tid & 31; c < s_got[r]; c += 32)
+        p.table[(r0 + r) * p.table_stride + held0 + c] = p.free_pages[head + s_first[r] + c];
+    }
+    // rows of this round that belong to this block
+    const int lo = max(static_cast<int>(row0), s_start[0]), hi = min(row_end, s_start[n]);
+    for (int i = lo + tid; i < hi; i += kPlanThreads) {
+      int a = 0, b = n - 1;  // last request whose start is <= i
+      while (a < b) {
+        const int m = (a + b + 1) >> 1;
+        if (s_start[m] <= i)
+          a = m;
+        else
+          b = m - 1;
+      }
+      const int len = s_len[a], pos = len + (i - s_start[a]);
+      int slot = -1;
+      if (pos < s_after[a]) {
+        const int held0 = (len + p.page - 1) / p.page, c = pos / p.page;
+        const int pg = c < held0 ? p.table[(r0 + a) * p.table_stride + c] : p.free_pages[head + s_first[a] + c - held0];
+        slot = pg * p.page + pos % p.page;
+      }
+      p.slots[i] = slot;
+      p.positions[i] = pos;
+      p.requests[i] = r0 + a;
+    }
+    __syncthreads();
+  }
+  for (int i = max(static_cast<int>(row0), base_tok) + tid; i < row_end; i += kPlanThreads)
+    p.slots[i] = p.positions[i] = p.requests[i] = -1;
+  if (blockIdx.x == 0) {
+    int tk, tt;
+    block_scan2(kept, taken, tk, tt, warp_sums);
+    if (tid == 0) {
+      p.starts[p.B] = base_tok;
+      *p.free_head_out = head + tt;
+      *p.dropped = base_tok - tk;
+    }
+  }
+}
+
+// ================================================================== append
+struct AppendParams {
+  const void* x[3];  // k1, k2, v: (tokens, heads, D)
+  long long st[3], sh[3];
+  const int* slots;
+  uint8_t* cache;
+  long long num_slots;
+  long long tokens;
+  int heads;
+  int page;
+  int normalize;
+};
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static __device__ __forceinline__ void load4(const float* p, float (&x)[8], int at) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[at] = v.x, x[at + 1] = v.y, x[at + 2] = v.z, x[at + 3] = v.w;
+  }
+  static __device__ __forceinline__ void store4(float* p, const float* x) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  }
+};
+template <>
+struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[8], int at) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[at] = __uint_as_float(v.x << 16), x[at + 1] = __uint_as_float(v.x & 0xffff0000u);
+    x[at + 2] = __uint_as_float(v.y << 16), x[at + 3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void store4(__nv_bfloat16* p, const float* x) {
+    __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+  }
+};
+template <>
+struct Elem<__half> {
+  static __device__ __forceinline__ void load4(const __half* p, float (&x)[8], int at) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+    x[at] = a.x, x[at + 1] = a.y, x[at + 2] = b.x, x[at + 3] = b.y;
+  }
+  static __device__ __forceinline__ void store4(__half* p, const float* x) {
+    __half2 a = __floats2half2_rn(x[0], x[1]), b = __floats2half2_rn(x[2], x[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+  }
+};
+
+// round-half-even of 7 |x| / amax without a division: t is within 2^-20 of the
+// quotient, and the choice between its floor f and f + 1 compares 14 |x| with
+// (2 f + 1) amax, both exact in fp32 for bf16 and fp16 inputs.  A floor that t
+// got wrong by one (a quotient at a whole number) ends at the same code.
+__device__ __forceinline__ int code_of(float x, float amax, float inv7) {
+  const float ax = fabsf(x);
+  const int f = min(7, static_cast<int>(ax * inv7));
+  const float d = fmaf(-static_cast<float>(2 * f + 1), amax, 14.0f * ax);
+  const int c = f + ((d > 0.0f || (d == 0.0f && (f & 1))) ? 1 : 0);
+  return x < 0.0f ? 8 - c : 8 + c;
+}
+
+__device__ __forceinline__ uint32_t max_bits(uint32_t a, float x) { return max(a, __float_as_uint(x) & 0x7fffffffu); }
+
+// A thread makes one 32-bit word of codes from 8 elements (two runs of 4), so
+// D / 8 neighbouring threads make a row; bound by the 2 bytes an element read.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) cache4_append_kernel(const AppendParams p) {
+  constexpr int kPer = D / 8;
+  const long long rows = p.tokens * p.heads;
+  const int xi = blockIdx.y;  // tensor
+  const long long idx = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const long long row = idx / kPer;
+  const int e = static_cast<int>(idx % kPer);
+  const bool in = row < rows;
+  const long long tok = in ? row / p.heads : 0;
+  const int h = in ? static_cast<int>(row % p.heads) : 0;
+  const int slot = in ? p.slots[tok] : -1;
+  const bool live = slot >= 0 && slot < p.num_slots;
+  const bool is_v = xi == 2;
+  // K: word w of lane t; V: word u of lane g
+  const int w = is_v ? e / 8 : e / 4, l = is_v ? e % 8 : e % 4;
+  const int d0 = is_v ? 64 * w + 4 * l : 32 * w + 4 * l;
+  const int d1 = is_v ? d0 + 32 : d0 + 16;
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (live) {
+    const T* src = static_cast<const T*>(p.x[xi]) + tok * p.st[xi] + h * p.sh[xi];
+    Elem<T>::load4(src + d0, x, 0);
+    Elem<T>::load4(src + d1, x, 4);
+  }
+  // largest magnitude of each run's group, as bits so that a NaN wins
+  uint32_t m0 = 0, m1 = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m0 = max_bits(m0, x[i]);
+    m1 = max_bits(m1, x[4 + i]);
+  }
+  if (!is_v) m0 = m1 = max(m0, m1);
+  for (int o = 1; o < (is_v ? 8 : 4); o <<= 1) {
+    m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+    m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+  }
+  float inv_norm = 1.0f;
+  if (p.normalize && !is_v) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+    for (int o = 1; o < kPer; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    inv_norm = 1.0f / fmaxf(sqrtf(ss), 1e-12f);
+  }
+  if (!live) return;
+  uint32_t word = 0;
+  float sc[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float amax = __uint_as_float(r ? m1 : m0);
+    const bool finite = (r ? m1 : m0) < 0x7f800000u;
+    sc[r] = finite ? amax / 7.0f * inv_norm : __uint_as_float(0x7fc00000u);
+    // far from the ends of the exponent's range, so that neither 7 / amax nor 14 x leaves it
+    const float lift = amax < 1e-18f ? 0x1p80f : (amax > 1e18f ? 0x1p-80f : 1.0f);
+    amax *= lift;
+    const float inv7 = amax > 0.0f ? __fdividef(7.0f, amax) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = (finite && amax > 0.0f) ? code_of(x[4 * r + j] * lift, amax, inv7) : 8;
+      // K: half r, register 2 r + j / 2, low or high half j % 2; V: run r, element j
+      const int nib = is_v ? 4 * r + j : (2 * r + (j >> 1)) + 4 * (j & 1);
+      word |= static_cast<uint32_t>(c) << (4 * nib);
+    }
+  }
+  uint8_t* blk = p.cache + (static_cast<size_t>(slot / p.page) * p.heads + h) * cache4_block_bytes(p.page, D);
+  const int at = slot % p.page;
+  uint8_t* codes = blk + cache4_codes_at(xi, p.page, D) + at * cache4_row_bytes(D);
+  *reinterpret_cast<uint32_t*>(codes + l * (is_v ? D / 16 : D / 8) + 4 * w) = word;
+  if (l == 0) {
+    __nv_bfloat16* s = reinterpret_cast<__nv_bfloat16*>(blk + cache4_scales_at(xi, p.page, D) + at * cache4_scale_bytes(D));
+    if (is_v) {
+      s[2 * w] = __float2bfloat16_rn(sc[0]);
+      s[2 * w + 1] = __float2bfloat16_rn(sc[1]);
+    } else {
+      s[w] = __float2bfloat16_rn(sc[0]);
+    }
+  }
+}
+
+// ================================================================== read
+struct ReadParams {
+  const uint8_t* cache;
+  const int* slots;
+  void* y[3];
+  long long num_slots;
+  long long tokens;
+  int heads;
+  int page;
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(256) cache4_read_kernel(const ReadParams p) {
+  constexpr int kPer = D / 8;
+  const int xi = blockIdx.y;
+  const long long idx = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const long long row = idx / kPer;
+  if (row >= p.tokens * p.heads) return;
+  const int e = static_cast<int>(idx % kPer);
+  const long long tok = row / p.heads;
+  const int h = static_cast<int>(row % p.heads);
+  const int slot = p.slots[tok];
+  const bool is_v = xi == 2;
+  const int w = is_v ? e / 8 : e / 4, l = is_v ? e % 8 : e % 4;
+  const int d0 = is_v ? 64 * w + 4 * l : 32 * w + 4 * l;
+  const int d1 = is_v ? d0 + 32 : d0 + 16;
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (slot >= 0 && slot < p.num_slots) {
+    const uint8_t* blk = p.cache + (static_cast<size_t>(slot / p.page) * p.heads + h) * cache4_block_bytes(p.page, D);
+    const int at = slot % p.page;
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(blk + cache4_codes_at(xi, p.page, D) +
+                                                             at * cache4_row_bytes(D) + l * (is_v ? D / 16 : D / 8) + 4 * w);
+    const __nv_bfloat16* s =
+        reinterpret_cast<const __nv_bfloat16*>(blk + cache4_scales_at(xi, p.page, D) + at * cache4_scale_bytes(D));
+    const float s0 = __bfloat162float(s[is_v ? 2 * w : w]), s1 = __bfloat162float(s[is_v ? 2 * w + 1 : w]);
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int nib = is_v ? 4 * r + j : (2 * r + (j >> 1)) + 4 * (j & 1);
+        x[4 * r + j] = static_cast<float>(static_cast<int>((word >> (4 * nib)) & 15u) - 8) * (r ? s1 : s0);
+      }
+  }
+  T* y = static_cast<T*>(p.y[xi]) + row * D;
+  Elem<T>::store4(y + d0, x);
+  Elem<T>::store4(y + d1, x + 4);
+}
+
+template <typename P, typename K>
+cudaError_t launch_rows(K kernel, const P& p, long long tokens, int heads, int D, cudaStream_t s) {
+  const long long blocks = ceil_div(tokens * heads * (D / 8), 256);
+  kernel<<<dim3(static_cast<unsigned>(blocks), 3), 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+int check_cache(const void* cache, int64_t num_pages, int64_t heads, int64_t D, int64_t page) {
+  if (D != 64 && D != 128) return fail(TDA_ERR_UNSUPPORTED, "the 4-bit cache needs head_dim 64 or 128 (got %lld)", static_cast<long long>(D));
+  if (page != 16 && page != 32 && page != 64 && page != 128)
+    return fail(TDA_ERR_INVALID, "page_size must be 16, 32, 64 or 128 (got %lld)", static_cast<long long>(page));
+  if (heads < 1 || num_pages < 1) return fail(TDA_ERR_INVALID, "num_pages and kv heads must be >= 1");
+  if (num_pages > 0x7fffffffll / page) return fail(TDA_ERR_INVALID, "num_pages * page_size must fit 31 bits");
+  if (!cache || !aligned(cache, 16)) return fail(TDA_ERR_INVALID, "cache must be non-NULL and 16-byte aligned");
+  return TDA_OK;
+}
+
+int check_rows(int64_t tokens, int64_t heads, int64_t D) {
+  if (tokens < 1) return fail(TDA_ERR_INVALID, "tokens must be >= 1");
+  if (tokens > 0x7fffffffll * 256 / (heads * (D / 8))) return fail(TDA_ERR_INVALID, "tokens * heads exceed the grid limit");
+  return TDA_OK;
+}
+
+}  // namespace
+
+int cache4_check(const void* cache, int64_t num_pages, int64_t heads, int64_t D, int64_t page) {
+  return check_cache(cache, num_pages, heads, D, page);
+}
+
+}  // namespace tda
+
+using namespace tda;
+
+extern "C" {
+
+size_t tda_cache4_block_bytes(int64_t page_size, int64_t head_dim) {
+  if ((head_dim != 64 && head_dim != 128) || page_size < 16 || page_size > 128 || (page_size & (page_size - 1)) != 0) return 0;
+  return cache4_block_bytes(static_cast<int>(page_size), static_cast<int>(head_dim));
+}
+
+int tda_plan_pages(const int32_t* lengths, const int32_t* new_tokens, int64_t requests, int32_t* block_table,
+                   int64_t table_stride, int64_t table_width, const int32_t* free_pages, int64_t num_free,
+                   const int32_t* free_head, int64_t page_size, int64_t rows, int32_t* slots, int32_t* positions,
+                   int32_t* request_ids, int32_t* starts, int32_t* lengths_out, int32_t* free_head_out,
+                   int32_t* dropped, void* stream) {
+  if (requests < 1 || requests > (1 << 24)) return fail(TDA_ERR_INVALID, "requests must be in [1, 2^24]");
+  if (table_width < 1 || table_stride < table_width) return fail(TDA_ERR_INVALID, "block table needs a width >= 1 and a stride >= the width");
+  if (page_size < 1 || page_size > (1 << 16)) return fail(TDA_ERR_INVALID, "page_size must be in [1, 65536]");
+  if (table_width > (1ll << 30) / page_size) return fail(TDA_ERR_INVALID, "table width * page_size must fit 30 bits");
+  if (num_free < 0 || num_free > 0x7fffffffll / page_size) return fail(TDA_ERR_INVALID, "free list too long");
+  if (rows < 0 || rows > (1ll << 30)) return fail(TDA_ERR_INVALID, "rows must be in [0, 2^30]");
+  const void* need[] = {lengths, new_tokens, block_table, free_head, starts, lengths_out, free_head_out, dropped};
+  for (const void* x : need)
+    if (!x || !aligned(x, 4)) return fail(TDA_ERR_INVALID, "plan arrays must be non-NULL int32");
+  if (num_free > 0 && !free_pages) return fail(TDA_ERR_INVALID, "free_pages is NULL");
+  if (rows > 0 && (!slots || !positions || !request_ids)) return fail(TDA_ERR_INVALID, "row outputs are NULL");
+  PlanParams p;
+  p.lengths = lengths;
+  p.added = new_tokens;
+  p.table = block_table;
+  p.free_pages = free_pages;
+  p.free_head = free_head;
+  p.slots = slots;
+  p.positions = positions;
+  p.requests = request_ids;
+  p.starts = starts;
+  p.lengths_out = lengths_out;
+  p.free_head_out = free_head_out;
+  p.dropped = dropped;
+  p.table_stride = table_stride;
+  p.B = static_cast<int>(requests);
+  p.width = static_cast<int>(table_width);
+  p.n_free = static_cast<int>(num_free);
+  p.page = static_cast<int>(page_size);
+  p.rows = static_cast<int>(rows);
+  const int64_t blocks = rows > 0 ? ceil_div(rows, kPlanRows) : 1;
+  plan_pages_kernel<<<static_cast<unsigned>(blocks), kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TDA_OK : cuda_fail(e, "page plan launch");
+}
+
+int tda_cache4_append(const void* k1, const void* k2, const void* v, int dtype, const int64_t* strides,
+                      const int32_t* slots, int64_t tokens, void* cache, int64_t num_pages, int64_t kv_heads,
+                      int64_t head_dim, int64_t page_size, int normalize_keys, void* stream) {
+  if (int e = check_cache(cache, num_pages, kv_heads, head_dim, page_size)) return e;
+  if (int e = check_rows(tokens, kv_heads, head_dim)) return e;
+  if (!slots || !aligned(slots, 4)) return fail(TDA_ERR_INVALID, "slots must be non-NULL int32");
+  AppendParams p;
+  const void* xs[3] = {k1, k2, v};
+  for (int i = 0; i < 3; ++i) {
+    if (!xs[i] || !aligned(xs[i], 16)) return fail(TDA_ERR_INVALID, "k1, k2 and v must be non-NULL and 16-byte aligned");
+    p.x[i] = xs[i];
+    p.st[i] = strides ? strides[2 * i] : kv_heads * head_dim;
+    p.sh[i] = strides ? strides[2 * i + 1] : head_dim;
+    if (p.st[i] <= 0 || p.sh[i] <= 0 || (p.st[i] | p.sh[i]) % 8 != 0)
+      return fail(TDA_ERR_INVALID, "input strides must be positive multiples of 8 elements");
+  }
+  p.slots = slots;
+  p.cache = static_cast<uint8_t*>(cache);
+  p.num_slots = num_pages * page_size;
+  p.tokens = tokens;
+  p.heads = static_cast<int>(kv_heads);
+  p.page = static_cast<int>(page_size);
+  p.normalize = normalize_keys != 0;
+  const int D = static_cast<int>(head_dim);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+#define TDA_APPEND(T) (D == 64 ? launch_rows(cache4_append_kernel<64, T>, p, tokens, p.heads, D, s) \
+                               : launch_rows(cache4_append_kernel<128, T>, p, tokens, p.heads, D, s))
+  if (dtype == TDA_BF16)
+    e = TDA_APPEND(__nv_bfloat16);
+  else if (dtype == TDA_F16)
+    e = TDA_APPEND(__half);
+  else if (dtype == TDA_F32)
+    e = TDA_APPEND(float);
+  else
+    return fail(TDA_ERR_INVALID, "dtype must be TDA_F32, TDA_BF16 or TDA_F16");
+#undef TDA_APPEND
+  return e == cudaSuccess ? TDA_OK : cuda_fail(e, "cache append launch");
+}
+
+int tda_cache4_read(const void* cache, int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                    const int32_t* slots, int64_t tokens, void* k1, void* k2, void* v, int dtype, void* stream) {
+  if (int e = check_cache(cache, num_pages, kv_heads, head_dim, page_size)) return e;
+  if (int e = check_rows(tokens, kv_heads, head_dim)) return e;
+  if (!slots || !aligned(slots, 4)) return fail(TDA_ERR_INVALID, "slots must be non-NULL int32");
+  ReadParams p;
+  void* ys[3] = {k1, k2, v};
+  for (int i = 0; i < 3; ++i) {
+    if (!ys[i] || !aligned(ys[i], 16)) return fail(TDA_ERR_INVALID, "k1, k2 and v must be non-NULL and 16-byte aligned");
+    p.y[i] = ys[i];
+  }
+  p.cache = static_cast<const uint8_t*>(cache);
+  p.slots = slots;
+  p.num_slots = num_pages * page_size;
+  p.tokens = tokens;
+  p.heads = static_cast<int>(kv_heads);
+  p.page = static_cast<int>(page_size);
+  const int D = static_cast<int>(head_dim);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+#define TDA_READ(T) (D == 64 ? launch_rows(cache4_read_kernel<64, T>, p, tokens, p.heads, D, s) \
+                             : launch_rows(cache4_read_kernel<128, T>, p, tokens, p.heads, D, s))
+  if (dtype == TDA_BF16)
+    e = TDA_READ(__nv_bfloat16);
+  else if (dtype == TDA_F16)
+    e = TDA_READ(__half);
+  else if (dtype == TDA_F32)
+    e = TDA_READ(float);
+  else
+    return fail(TDA_ERR_INVALID, "dtype must be TDA_F32, TDA_BF16 or TDA_F16");
+#undef TDA_READ
+  return e == cudaSuccess ? TDA_OK : cuda_fail(e, "cache read launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,264 @@
+"""Softmax differential attention on the tda_b200 C ABI.
+
+``differential_softmax_attention(q1, q2, k1, k2, v, lambda_param, scale=None,
+causal=True, key_lengths=None)``:
+
+    out = (softmax(scale q1 k1^T) - lambda softmax(scale q2 k2^T)) v
+
+the form that threshold differential attention replaces, with its gradients
+(q1, q2, k1, k2, v and lambda).  q1, q2: (B, H, Sq, D); k1, k2, v: (B, Hkv, Sk,
+D), Hkv dividing H (query head h reads kv head h // (H / Hkv); gradients of
+shared heads are summed).  Row i sees key j when j < key_lengths[b] and, when
+causal, j <= i + Sk - Sq; a row that sees no key gives zeros.  lambda is used
+as it is (no clamp): a float, or a tensor that broadcasts over (batch, head).
+
+bf16 and fp16 with head_dim 64 / 128 run on the tcgen05 tensor cores; fp32 and
+other head dims (powers of two in [16, 256]) run in fp32 on the CUDA cores;
+other float types are widened to fp32.  There is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from . import ops as _ops
+
+_CODE = {torch.float32: _lib.TDA_F32, torch.bfloat16: _lib.TDA_BF16, torch.float16: _lib.TDA_F16}
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _on:
+    """Makes ``device`` current around a launch, at no cost where it already is."""
+
+    def __init__(self, device):
+        self.ctx = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def lambda_ref(lam, B: int, H: int, device: torch.device, what: str):
+    """(pointer, dtype code, batch stride, head stride, value, keep-alive) of a
+    lambda: a float or one-element CPU tensor is read on the host, a tensor that
+    broadcasts over (batch, head) stays on the device in its own type."""
+    if not isinstance(lam, torch.Tensor):
+        return None, 0, 0, 0, float(lam), None
+    if not lam.dtype.is_floating_point:
+        raise TypeError(f"{what}: lambda must be floating point, got {lam.dtype}")
+    if not lam.is_cuda and lam.numel() == 1:
+        return None, 0, 0, 0, float(lam.item()), None
+    l4 = lam.detach()
+    if lam.dim() > 4:
+        raise ValueError(f"{what}: lambda may have at most 4 dimensions, got {lam.dim()}")
+    l4 = l4[(None,) * (4 - lam.dim())]
+    if l4.shape[2] != 1 or l4.shape[3] != 1 or l4.shape[0] not in (1, B) or l4.shape[1] not in (1, H):
+        raise ValueError(f"{what}: lambda must broadcast over (batch, head) alone, i.e. to ({B}, {H}, 1, 1); "
+                         f"got {tuple(lam.shape)}")
+    if l4.device != device:
+        l4 = l4.to(device)
+    if l4.dtype not in _CODE:
+        l4 = l4.float()
+    return (l4.data_ptr(), _CODE[l4.dtype], l4.stride(0) if l4.shape[0] != 1 else 0,
+            l4.stride(1) if l4.shape[1] != 1 else 0, 0.0, l4)
+
+
+def _check(q1, q2, k1, k2, v, key_lengths, what="differential_softmax_attention"):
+    ts = (q1, q2, k1, k2, v)
+    for t in ts:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: expected torch.Tensor inputs")
+    if q1.dim() != 4 or k1.dim() != 4:
+        raise ValueError(f"{what}: expected (batch, heads, seq_len, head_dim) tensors, got {tuple(q1.shape)} and "
+                         f"{tuple(k1.shape)}")
+    if q1.shape != q2.shape:
+        raise ValueError(f"{what}: q1 and q2 must have one shape, got {tuple(q1.shape)} and {tuple(q2.shape)}")
+    if not (k1.shape == k2.shape == v.shape):
+        raise ValueError(f"{what}: k1, k2 and v must have one shape")
+    if q1.shape[0] != k1.shape[0] or q1.shape[3] != k1.shape[3]:
+        raise ValueError(f"{what}: batch and head_dim of queries {tuple(q1.shape)} and keys {tuple(k1.shape)} differ")
+    if k1.shape[1] == 0 or q1.shape[1] % k1.shape[1] != 0:
+        raise ValueError(f"{what}: the kv heads ({k1.shape[1]}) must divide the query heads ({q1.shape[1]})")
+    D = q1.shape[3]
+    if D < 16 or D > 256 or (D & (D - 1)) != 0:
+        raise ValueError(f"{what}: head_dim must be a power of two in [16, 256], got {D}")
+    if not q1.is_cuda:
+        raise RuntimeError(f"{what}: tda_b200 runs on CUDA tensors only (got device {q1.device}); "
+                           "there is no CPU fallback")
+    for t in ts:
+        if t.device != q1.device:
+            raise RuntimeError(f"{what}: all inputs must be on one device")
+        if not t.dtype.is_floating_point:
+            raise TypeError(f"{what}: floating point inputs required, got {t.dtype}")
+    if key_lengths is not None:
+        if not isinstance(key_lengths, torch.Tensor) or key_lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{what}: key_lengths must be an int32 or int64 tensor")
+        if key_lengths.shape != (q1.shape[0],):
+            raise ValueError(f"{what}: key_lengths must have shape ({q1.shape[0]},), got {tuple(key_lengths.shape)}")
+        if key_lengths.device != q1.device:
+            raise RuntimeError(f"{what}: key_lengths must be on the inputs' device")
+
+
+def _compute_dtype(ts) -> torch.dtype:
+    common = ts[0].dtype
+    for t in ts[1:]:
+        if t.dtype != common:
+            common = torch.promote_types(common, t.dtype)
+    return common if common in _CODE else torch.float32
+
+
+def view_of(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """``t`` in ``dtype`` as the kernels read it in place: contiguous last
+    dimension, other strides positive multiples of 8 elements (any stride of a
+    dimension of size 1 counts as fitting), 16-byte aligned; else a copy."""
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+    if ok:
+        for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+            if n != 1 and (s <= 0 or s % 8):
+                ok = False
+                break
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def strides_of(ts):
+    """Element strides of all but the last dimension, a stride that is never
+    used (size 1) given as the row's length."""
+    out = []
+    for t in ts:
+        d = t.shape[-1]
+        out += [s if n != 1 else d for n, s in zip(t.shape[:-1], t.stride()[:-1])]
+    return (ctypes.c_int64 * len(out))(*out)
+
+
+def _lengths32(key_lengths):
+    if key_lengths is None:
+        return None
+    return key_lengths.to(torch.int32).contiguous()
+
+
+def sdiff_forward(q1, q2, k1, k2, v, lambda_param, scale=None, causal=True, key_lengths=None, save=True):
+    """(out, o12, lse): the attention and, where ``save``, what its backward
+    needs: each map's product with v (fp32 (2, B, H, Sq, D)) and the row sums
+    (fp32 (2, B, H, Sq), log2; +inf where a row sees no key); None otherwise.
+    No autograd."""
+    _check(q1, q2, k1, k2, v, key_lengths)
+    B, H, Sq, D = q1.shape
+    Hkv, Sk = k1.shape[1], k1.shape[2]
+    dt = _compute_dtype((q1, q2, k1, k2, v))
+    out = torch.empty((B, H, Sq, D), dtype=dt, device=q1.device)
+    o12 = torch.empty((2, B, H, Sq, D), dtype=torch.float32, device=q1.device) if save else None
+    lse = torch.empty((2, B, H, Sq), dtype=torch.float32, device=q1.device) if save else None
+    if out.numel() == 0 or Sk == 0:
+        return out.zero_(), o12.zero_() if save else None, lse.fill_(math.inf) if save else None
+    ts = [view_of(t, dt) for t in (q1, q2, k1, k2, v)]
+    kl = _lengths32(key_lengths)
+    lp, lc, lsb, lsh, lv, keep = lambda_ref(lambda_param, B, H, q1.device, "differential_softmax_attention")
+    lib = _lib.load()
+    with _on(q1.device):
+        rc = lib.tda_sdiff_fwd(*[t.data_ptr() for t in ts], strides_of(ts), out.data_ptr(),
+                               o12.data_ptr() if save else None, lse.data_ptr() if save else None, _CODE[dt], B, H, Hkv, Sq, Sk, D,
+                               1.0 / math.sqrt(D) if scale is None else float(scale), int(causal),
+                               None if kl is None else kl.data_ptr(), lp, lc, lsb, lsh, lv,
+                               _ops._status_word(q1.device).data_ptr(), _stream(q1.device))
+    _lib.check(rc)
+    if _ops._SYNC_CHECK:
+        _ops.check_status(q1.device)
+    return out, o12, lse
+
+
+def sdiff_backward(q1, q2, k1, k2, v, dout, o12, lse, lambda_param, scale=None, causal=True, key_lengths=None,
+                   need_dlam=True):
+    """(dq1, dq2, dk1, dk2, dv, dlam) for the upstream gradient ``dout`` from
+    the forward's (o12, lse); gradients in the compute type, ``dlam`` fp32 (B,
+    H), None when not asked for."""
+    _check(q1, q2, k1, k2, v, key_lengths)
+    if dout.shape != q1.shape:
+        raise ValueError(f"differential_softmax_attention: dout must have shape {tuple(q1.shape)}, got "
+                         f"{tuple(dout.shape)}")
+    B, H, Sq, D = q1.shape
+    Hkv, Sk = k1.shape[1], k1.shape[2]
+    dt = _compute_dtype((q1, q2, k1, k2, v))
+    dev = q1.device
+    dq = [torch.empty((B, H, Sq, D), dtype=dt, device=dev) for _ in range(2)]
+    dkv = [torch.empty((B, Hkv, Sk, D), dtype=dt, device=dev) for _ in range(3)]
+    dlam = torch.empty((B, H), dtype=torch.float32, device=dev) if need_dlam else None
+    if q1.numel() == 0 or Sk == 0:
+        return (*[t.zero_() for t in dq + dkv], dlam.zero_() if need_dlam else None)
+    ts = [view_of(t, dt) for t in (q1, q2, k1, k2, v)]
+    g = view_of(dout, dt)
+    kl = _lengths32(key_lengths)
+    lp, lc, lsb, lsh, lv, keep = lambda_ref(lambda_param, B, H, dev, "differential_softmax_attention")
+    lib = _lib.load()
+    ws_n = lib.tda_sdiff_bwd_workspace_size(B, H, Sq)
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = lib.tda_sdiff_bwd(*[t.data_ptr() for t in ts], strides_of(ts), g.data_ptr(), strides_of([g]),
+                               o12.data_ptr(), lse.data_ptr(), *[t.data_ptr() for t in dq + dkv],
+                               dlam.data_ptr() if need_dlam else None, _CODE[dt], B, H, Hkv, Sq, Sk, D,
+                               1.0 / math.sqrt(D) if scale is None else float(scale), int(causal),
+                               None if kl is None else kl.data_ptr(), lp, lc, lsb, lsh, lv, ws.data_ptr(), ws_n,
+                               _ops._status_word(dev).data_ptr(), _stream(dev))
+    _lib.check(rc)
+    if _ops._SYNC_CHECK:
+        _ops.check_status(dev)
+    return (*dq, *dkv, dlam)
+
+
+def dlam_like(dlam: torch.Tensor, lam: torch.Tensor) -> torch.Tensor:
+    """(B, H) gradients summed to lambda's shape, in its type and on its device."""
+    g = dlam[:, :, None, None]
+    if lam.numel() == 1:
+        g = g.sum()
+    else:
+        g = g.sum_to_size((1,) * (4 - lam.dim()) + tuple(lam.shape))
+    return g.reshape(lam.shape).to(device=lam.device, dtype=lam.dtype)
+
+
+class DifferentialSoftmaxFunction(torch.autograd.Function):
+    """forward(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths)."""
+
+    @staticmethod
+    def forward(ctx, q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths):
+        out, o12, lse = sdiff_forward(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths)
+        lam_t = lambda_param if isinstance(lambda_param, torch.Tensor) else None
+        ctx.save_for_backward(q1, q2, k1, k2, v, lam_t, key_lengths, o12, lse)
+        ctx.lam = None if lam_t is not None else float(lambda_param)
+        ctx.scale, ctx.causal = scale, causal
+        return out if out.dtype == q1.dtype else out.to(q1.dtype)
+
+    @staticmethod
+    def backward(ctx, dout):
+        q1, q2, k1, k2, v, lam_t, kl, o12, lse = ctx.saved_tensors
+        lam = ctx.lam if lam_t is None else lam_t
+        need = lam_t is not None and ctx.needs_input_grad[5]
+        g = sdiff_backward(q1, q2, k1, k2, v, dout, o12, lse, lam, ctx.scale, ctx.causal, kl, need)
+        cast = [x if x.dtype == t.dtype else x.to(t.dtype) for x, t in zip(g[:5], (q1, q2, k1, k2, v))]
+        return (*cast, dlam_like(g[5], lam_t) if need else None, None, None, None)
+
+
+def differential_softmax_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=True, key_lengths=None):
+    """out = (softmax(scale q1 k1^T) - lambda softmax(scale q2 k2^T)) v, q1's
+    shape and dtype; differentiable in q1, q2, k1, k2, v and lambda.  ``scale``
+    defaults to head_dim ** -0.5.  See the module's docstring.  Under
+    torch.compile it runs as the operator ``tda::sdiff_fwd``."""
+    if torch.compiler.is_compiling():
+        lam = lambda_param if isinstance(lambda_param, torch.Tensor) else torch.tensor(float(lambda_param))
+        sc = 1.0 / math.sqrt(q1.shape[-1]) if scale is None else float(scale)
+        return torch.ops.tda.sdiff_fwd(q1, q2, k1, k2, v, lam, sc, bool(causal), key_lengths)[0]
+    if not (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                            for t in (q1, q2, k1, k2, v, lambda_param))):
+        out = sdiff_forward(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths, save=False)[0]
+        return out if out.dtype == q1.dtype else out.to(q1.dtype)
+    return DifferentialSoftmaxFunction.apply(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths)

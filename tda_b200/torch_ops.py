@@ -5,6 +5,9 @@
     torch.ops.tda.rect_bwd(q, k, v, dout, beta, relu_power, normalize) -> (dq, dk, dv)
     torch.ops.tda.diff_bwd(q1, q2, k1, k2, v, dout, beta, lambda_param, relu_power, normalize,
                            need_dlam) -> (dq1, dq2, dk1, dk2, dv, dlambda)
+    torch.ops.tda.sdiff_fwd(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths) -> (out, o12, lse)
+    torch.ops.tda.sdiff_bwd(q1, q2, k1, k2, v, dout, o12, lse, lambda_param, scale, causal, key_lengths,
+                            need_dlam) -> (dq1, dq2, dk1, dk2, dv, dlambda)
 
 The reference's entry points are a ``torch.autograd.Function``
 (triton_threshold_attention.py:327) that torch can trace.  The CUDA library
@@ -25,7 +28,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import ops
+from . import ops, sdiff
 
 
 def _same_shapes(*ts):
@@ -120,3 +123,58 @@ def _diff_backward(ctx, dout):
 
 
 diff_fwd.register_autograd(_diff_backward, setup_context=_diff_setup)
+
+
+# ------------------------------------------------- softmax differential attention
+@torch.library.custom_op("tda::sdiff_fwd", mutates_args=())
+def sdiff_fwd(q1: Tensor, q2: Tensor, k1: Tensor, k2: Tensor, v: Tensor, lambda_param: Tensor, scale: float,
+              causal: bool, key_lengths: Tensor | None) -> tuple[Tensor, Tensor, Tensor]:
+    """Softmax differential attention: (out, o12, lse), the last two for the backward."""
+    out, o12, lse = sdiff.sdiff_forward(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths)
+    return out.to(q1.dtype), o12, lse
+
+
+@sdiff_fwd.register_fake
+def _sdiff_fwd_fake(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths):
+    shape = q1.shape
+    return (q1.new_empty(shape), q1.new_empty((2, *shape), dtype=torch.float32),
+            q1.new_empty((2, shape[0], shape[1], shape[2]), dtype=torch.float32))
+
+
+@torch.library.custom_op("tda::sdiff_bwd", mutates_args=())
+def sdiff_bwd(q1: Tensor, q2: Tensor, k1: Tensor, k2: Tensor, v: Tensor, dout: Tensor, o12: Tensor,
+              lse: Tensor, lambda_param: Tensor, scale: float, causal: bool, key_lengths: Tensor | None,
+              need_dlam: bool) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(dq1, dq2, dk1, dk2, dv, dlambda) of sdiff_fwd; dlambda is zeros of
+    lambda's shape when ``need_dlam`` is False."""
+    g = sdiff.sdiff_backward(q1, q2, k1, k2, v, dout, o12, lse, lambda_param, scale, causal, key_lengths, need_dlam)
+    grads = [x.to(t.dtype) for x, t in zip(g[:5], (q1, q2, k1, k2, v))]
+    dlam = sdiff.dlam_like(g[5], lambda_param) if need_dlam else torch.zeros_like(lambda_param)
+    return grads[0], grads[1], grads[2], grads[3], grads[4], dlam
+
+
+@sdiff_bwd.register_fake
+def _sdiff_bwd_fake(q1, q2, k1, k2, v, dout, o12, lse, lambda_param, scale, causal, key_lengths, need_dlam):
+    return (q1.new_empty(q1.shape), q2.new_empty(q2.shape), k1.new_empty(k1.shape), k2.new_empty(k2.shape),
+            v.new_empty(v.shape), lambda_param.new_empty(lambda_param.shape))
+
+
+def _sdiff_setup(ctx, inputs, output):
+    q1, q2, k1, k2, v, lam, scale, causal, key_lengths = inputs
+    _out, o12, lse = output
+    ctx.save_for_backward(q1, q2, k1, k2, v, lam, key_lengths, o12, lse)
+    ctx.args = (scale, causal)
+    ctx.set_materialize_grads(False)
+
+
+def _sdiff_backward(ctx, dout, _do12, _dlse):
+    q1, q2, k1, k2, v, lam, key_lengths, o12, lse = ctx.saved_tensors
+    if dout is None:
+        return (None,) * 9
+    scale, causal = ctx.args
+    need = bool(ctx.needs_input_grad[5])
+    g = torch.ops.tda.sdiff_bwd(q1, q2, k1, k2, v, dout, o12, lse, lam, scale, causal, key_lengths, need)
+    return g[0], g[1], g[2], g[3], g[4], (g[5] if need else None), None, None, None
+
+
+sdiff_fwd.register_autograd(_sdiff_backward, setup_context=_sdiff_setup)
