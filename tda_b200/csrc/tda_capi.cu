@@ -338,6 +338,7 @@ size_t rk_bytes(int64_t BH, int64_t S) { return tda::key_table_floats(BH, S) * s
 }  // namespace
 
 void tda::set_last_error(const char* msg) { g_last_error = msg ? msg : ""; }
+unsigned long long tda::wait_timeout_ns() { return g_timeout_ns.load(); }
 
 extern "C" {
 

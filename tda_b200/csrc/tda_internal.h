@@ -273,6 +273,9 @@ cudaError_t launch_key_norms_strided(int n, const void* const x[2], float* const
                                      int S, int S_pad, int D, const int64_t stride_b[2], const int64_t stride_h[2],
                                      const int64_t stride_s[2], cudaStream_t stream);
 
+// Limit of a kernel's bounded waits (tda_debug_set).
+unsigned long long wait_timeout_ns();
+
 // Sets the thread-local message returned by tda_last_error().
 void set_last_error(const char* msg);
 

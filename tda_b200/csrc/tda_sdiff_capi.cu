@@ -3,9 +3,17 @@
 #include <cmath>
 #include <cstring>
 
-#include "tda_sdiff.h"
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "tda_sdiff_tc.cuh"
 
 using namespace tda;
+
+namespace tda {
+cudaError_t launch_sdiff_tc_fwd(const SdTcParams& tp, int dtype, int D, cudaStream_t s);
+}
 
 namespace {
 
@@ -50,6 +58,72 @@ int fill(SdParams& p, const void* q1, const void* q2, const void* k1, const void
   return TDA_OK;
 }
 
+// bf16 and fp16 at these head dims fit the tensor-core kernels' tiles; fp32 needs
+// its own arithmetic and other head dims do not fill a 128-byte box
+bool on_tensor_cores(int dtype, int64_t D) { return dtype != TDA_F32 && (D == 64 || D == 128); }
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+// {D, S, heads, batches} with boxes of 128 bytes x 128 rows, 128-byte swizzle, zeros out of bounds
+int map4(CUtensorMap* m, int dtype, const SdView& x, int64_t B, int64_t H, int64_t S, int64_t D) {
+  auto enc = encoder();
+  if (!enc) return fail(TDA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const int es = dtype == TDA_F32 ? 4 : 2;
+  const CUtensorMapDataType dt = dtype == TDA_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : dtype == TDA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(H), static_cast<cuuint64_t>(B)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(x.ss) * es, static_cast<cuuint64_t>(x.sh) * es, static_cast<cuuint64_t>(x.sb) * es};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(kTile), 1, 1};
+  cuuint32_t one[4] = {1, 1, 1, 1};
+  CUresult r = enc(m, dt, 4, const_cast<void*>(x.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TDA_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", static_cast<int>(r));
+  return TDA_OK;
+}
+
+// a contiguous (n, S, D) output as {D, S, n}, same boxes
+int map3(CUtensorMap* m, int dtype, const void* x, int64_t n, int64_t S, int64_t D) {
+  auto enc = encoder();
+  if (!enc) return fail(TDA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const int es = dtype == TDA_F32 ? 4 : 2;
+  const CUtensorMapDataType dt = dtype == TDA_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : dtype == TDA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(n)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(D * es), static_cast<cuuint64_t>(S * D * es)};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(kTile), 1};
+  cuuint32_t one[3] = {1, 1, 1};
+  CUresult r = enc(m, dt, 3, const_cast<void*>(x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TDA_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", static_cast<int>(r));
+  return TDA_OK;
+}
+
+int input_maps(SdTcParams& tp, int dtype, int64_t D) {
+  const SdParams& p = tp.p;
+  for (int i = 0; i < 2; ++i) {
+    if (int e = map4(&tp.m.q[i], dtype, p.q[i], p.B, p.H, p.Sq, D)) return e;
+    if (int e = map4(&tp.m.k[i], dtype, p.k[i], p.B, p.Hkv, p.Sk, D)) return e;
+  }
+  if (int e = map4(&tp.m.v, dtype, p.v, p.B, p.Hkv, p.Sk, D)) return e;
+  tp.n_qt = static_cast<int>(ceil_div(p.Sq, kTile));
+  tp.n_kt = static_cast<int>(ceil_div(p.Sk, kTile));
+  tp.timeout_ns = wait_timeout_ns();
+  return TDA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -71,7 +145,21 @@ int tda_sdiff_fwd(const void* q1, const void* q2, const void* k1, const void* k2
   p.out = out;
   p.o12 = o12;
   p.lse = lse;
-  cudaError_t e = launch_sdiff_simt_fwd(p, dtype, static_cast<int>(head_dim), static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (on_tensor_cores(dtype, head_dim)) {
+    SdTcParams tp;
+    std::memset(&tp, 0, sizeof(tp));
+    tp.p = p;
+    tp.status = status;
+    if (int r = input_maps(tp, dtype, head_dim)) return r;
+    if (int r = map3(&tp.m.out, dtype, out, batch * heads, q_len, head_dim)) return r;
+    if (o12)
+      if (int r = map3(&tp.m.o12, TDA_F32, o12, 2 * batch * heads, q_len, head_dim)) return r;
+    e = launch_sdiff_tc_fwd(tp, dtype, static_cast<int>(head_dim), s);
+  } else {
+    e = launch_sdiff_simt_fwd(p, dtype, static_cast<int>(head_dim), s);
+  }
   return e == cudaSuccess ? TDA_OK : cuda_fail(e, "softmax differential forward launch");
 }
 
