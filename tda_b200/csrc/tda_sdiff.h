@@ -38,7 +38,8 @@ struct SdParams {
   float c;         // scale log2(e)
   // backward
   SdView dout;
-  float* delta;    // [2][B][H][Sq]: D_1, D_2
+  float2* table;   // [2][B][H][pad]: {L_m, D_m} of each row, {+inf, 0} past Sq
+  int pad;         // Sq rounded up to a tile of 128
   void* dq[2];     // contiguous, of the inputs' type
   void* dk[2];
   void* dv;

@@ -13,6 +13,7 @@ using namespace tda;
 
 namespace tda {
 cudaError_t launch_sdiff_tc_fwd(const SdTcParams& tp, int dtype, int D, cudaStream_t s);
+cudaError_t launch_sdiff_tc_bwd(const SdTcParams& tp, int dtype, int D, cudaStream_t s);
 }
 
 namespace {
@@ -165,7 +166,7 @@ int tda_sdiff_fwd(const void* q1, const void* q2, const void* k1, const void* k2
 
 size_t tda_sdiff_bwd_workspace_size(int64_t batch, int64_t heads, int64_t q_len) {
   if (batch < 1 || heads < 1 || q_len < 1) return 0;
-  return 2 * static_cast<size_t>(batch) * heads * q_len * sizeof(float);
+  return 2 * static_cast<size_t>(batch) * heads * padded_seq(q_len) * sizeof(float2);
 }
 
 int tda_sdiff_bwd(const void* q1, const void* q2, const void* k1, const void* k2, const void* v,
@@ -194,7 +195,8 @@ int tda_sdiff_bwd(const void* q1, const void* q2, const void* k1, const void* k2
     return fail(TDA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed", bytes);
   p.o12 = const_cast<float*>(o12);
   p.lse = const_cast<float*>(lse);
-  p.delta = static_cast<float*>(workspace);
+  p.table = static_cast<float2*>(workspace);
+  p.pad = static_cast<int>(padded_seq(q_len));
   p.dq[0] = dq1;
   p.dq[1] = dq2;
   p.dk[0] = dk1;
@@ -204,7 +206,22 @@ int tda_sdiff_bwd(const void* q1, const void* q2, const void* k1, const void* k2
   const int D = static_cast<int>(head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = launch_sdiff_delta(p, dtype, D, s);
-  if (e == cudaSuccess) e = launch_sdiff_simt_bwd(p, dtype, D, s);
+  if (e == cudaSuccess && on_tensor_cores(dtype, head_dim)) {
+    SdTcParams tp;
+    std::memset(&tp, 0, sizeof(tp));
+    tp.p = p;
+    tp.status = status;
+    if (int r = input_maps(tp, dtype, head_dim)) return r;
+    if (int r = map4(&tp.m.dout, dtype, p.dout, batch, heads, q_len, head_dim)) return r;
+    for (int i = 0; i < 2; ++i) {
+      if (int r = map3(&tp.m.dq[i], dtype, p.dq[i], batch * heads, q_len, head_dim)) return r;
+      if (int r = map3(&tp.m.dk[i], dtype, p.dk[i], batch * kv_heads, k_len, head_dim)) return r;
+    }
+    if (int r = map3(&tp.m.dv, dtype, dv, batch * kv_heads, k_len, head_dim)) return r;
+    e = launch_sdiff_tc_bwd(tp, dtype, D, s);
+  } else if (e == cudaSuccess) {
+    e = launch_sdiff_simt_bwd(p, dtype, D, s);
+  }
   return e == cudaSuccess ? TDA_OK : cuda_fail(e, "softmax differential backward launch");
 }
 

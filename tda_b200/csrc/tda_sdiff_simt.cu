@@ -140,6 +140,10 @@ __device__ __forceinline__ long long row_at(const SdParams& p, int m, int b, int
   return ((static_cast<long long>(m) * p.B + b) * p.H + h) * p.Sq + i;
 }
 
+__device__ __forceinline__ long long table_at(const SdParams& p, int m, int b, int h, int i) {
+  return ((static_cast<long long>(m) * p.B + b) * p.H + h) * p.pad + i;
+}
+
 // ================================================================== forward
 template <typename T, int D>
 __global__ void __launch_bounds__(256) sdiff_simt_fwd_kernel(const SdParams p) {
@@ -230,7 +234,7 @@ __global__ void __launch_bounds__(256) sdiff_simt_fwd_kernel(const SdParams p) {
 // D_1 = dout . O_1 and D_2 = dout . O_2, a warp a row.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) sdiff_delta_kernel(const SdParams p) {
-  const long long rows = static_cast<long long>(p.B) * p.H * p.Sq;
+  const long long rows = static_cast<long long>(p.B) * p.H * p.pad, all = static_cast<long long>(p.B) * p.H * p.Sq;
   const int lane = threadIdx.x & 31;
   constexpr int kLanes = D / 4 < 32 ? D / 4 : 32;
   constexpr int kPerWarp = 32 / kLanes;
@@ -238,13 +242,15 @@ __global__ void __launch_bounds__(256) sdiff_delta_kernel(const SdParams p) {
   const long long row = warp * kPerWarp + lane / kLanes;
   const int l = lane % kLanes;
   float a = 0.f, c = 0.f;
-  if (row < rows) {
-    const int i = static_cast<int>(row % p.Sq);
-    const int h = static_cast<int>(row / p.Sq % p.H), b = static_cast<int>(row / p.Sq / p.H);
+  const long long bh = row / p.pad;
+  const int i = static_cast<int>(row % p.pad);
+  const long long at = bh * p.Sq + i;
+  if (row < rows && i < p.Sq) {
+    const int h = static_cast<int>(bh % p.H), b = static_cast<int>(bh / p.H);
     const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.sb + h * p.dout.sh + i * p.dout.ss;
 #pragma unroll
     for (int d = 4 * l; d < D; d += 4 * kLanes) {
-      const float4 x = load4(g + d), y = load4(p.o12 + row * D + d), z = load4(p.o12 + (rows + row) * D + d);
+      const float4 x = load4(g + d), y = load4(p.o12 + at * D + d), z = load4(p.o12 + (all + at) * D + d);
       a += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
       c += x.x * z.x + x.y * z.y + x.z * z.z + x.w * z.w;
     }
@@ -255,8 +261,8 @@ __global__ void __launch_bounds__(256) sdiff_delta_kernel(const SdParams p) {
     c += __shfl_xor_sync(0xffffffffu, c, o);
   }
   if (row < rows && l == 0) {
-    p.delta[row] = a;
-    p.delta[rows + row] = c;
+    p.table[row] = make_float2(i < p.Sq ? p.lse[at] : kInf, a);
+    p.table[rows + row] = make_float2(i < p.Sq ? p.lse[all + at] : kInf, c);
   }
 }
 
@@ -264,9 +270,9 @@ __global__ void __launch_bounds__(256) sdiff_delta_kernel(const SdParams p) {
 __global__ void __launch_bounds__(256) sdiff_dlam_kernel(const SdParams p) {
   __shared__ float part[256];
   const long long bh = blockIdx.x;
-  const float* d = p.delta + static_cast<long long>(p.B) * p.H * p.Sq + bh * p.Sq;
+  const float2* d = p.table + (static_cast<long long>(p.B) * p.H + bh) * p.pad;
   float s = 0.f;
-  for (int i = threadIdx.x; i < p.Sq; i += 256) s += d[i];
+  for (int i = threadIdx.x; i < p.Sq; i += 256) s += d[i].y;
   part[threadIdx.x] = s;
   __syncthreads();
   for (int o = 128; o > 0; o >>= 1) {
@@ -296,8 +302,9 @@ __global__ void __launch_bounds__(256) sdiff_simt_dq_kernel(const SdParams p) {
 #pragma unroll
   for (int r = 0; r < C::R; ++r) {
     const int i = i0 + ty * C::R + r;
-    lse[r] = i < p.Sq ? p.lse[row_at(p, m, b, h, i)] : kInf;
-    del[r] = i < p.Sq ? p.delta[row_at(p, m, b, h, i)] : 0.f;
+    const float2 t = i < p.Sq ? p.table[table_at(p, m, b, h, i)] : make_float2(kInf, 0.f);
+    lse[r] = t.x;
+    del[r] = t.y;
 #pragma unroll
     for (int c = 0; c < C::C; ++c) o[r][c] = 0.f;
   }
@@ -365,8 +372,9 @@ __global__ void __launch_bounds__(256) sdiff_simt_dkv_kernel(const SdParams p) {
         load_tile<T, D>(gs, p.dout, b, h, i0, p.Sq);
         if (threadIdx.x < C::BT) {
           const int i = i0 + threadIdx.x;
-          ls[threadIdx.x] = i < p.Sq ? p.lse[row_at(p, m, b, h, i)] : kInf;
-          es[threadIdx.x] = i < p.Sq ? p.delta[row_at(p, m, b, h, i)] : 0.f;
+          const float2 t = i < p.Sq ? p.table[table_at(p, m, b, h, i)] : make_float2(kInf, 0.f);
+          ls[threadIdx.x] = t.x;
+          es[threadIdx.x] = t.y;
         }
         __syncthreads();
         float s[C::R][C::R], dp[C::R][C::R];
@@ -422,7 +430,7 @@ cudaError_t fwd(const SdParams& p, cudaStream_t s) {
 
 template <typename T, int D>
 cudaError_t delta(const SdParams& p, cudaStream_t s) {
-  const long long rows = static_cast<long long>(p.B) * p.H * p.Sq;
+  const long long rows = static_cast<long long>(p.B) * p.H * p.pad;
   constexpr int kPerBlock = 8 * (32 / (D / 4 < 32 ? D / 4 : 32));
   sdiff_delta_kernel<T, D><<<static_cast<unsigned>(ceil_div(rows, kPerBlock)), 256, 0, s>>>(p);
   cudaError_t e = cudaGetLastError();

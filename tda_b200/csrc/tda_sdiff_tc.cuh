@@ -45,13 +45,15 @@ __device__ __forceinline__ void mma_score(uint32_t dcol, uint32_t a, uint32_t b)
   }
 }
 
-// D[dcol] (+)= W X: W [128][128] 16-bit in TMEM (64 columns), X an MN-major tile of 128 rows
-template <int D, bool F16>
+// D[dcol] (+)= W X: W [128][128] 16-bit in TMEM, X an MN-major tile of 128 rows.  W fills 64
+// columns, or (HALVES) 32 at wcol and 32 at wcol + 64: each half over the scores it came
+// from, so that the two warps that share a row's scores need not wait for one another.
+template <int D, bool F16, bool HALVES = false>
 __device__ __forceinline__ void mma_weights(uint32_t dcol, uint32_t wcol, uint32_t x, bool accumulate) {
   using G = Geo<D, F16>;
 #pragma unroll
   for (int m = 0; m < kTile / 16; ++m)
-    mma_ts(dcol, wcol + 8 * m, smem_desc_sw128(x + m * 2048, G::kBoxBytes, 1024), G::kIdescMn, (accumulate || m > 0) ? 1u : 0u);
+    mma_ts(dcol, wcol + (HALVES ? 64 * (m >> 2) + 8 * (m & 3) : 8 * m), smem_desc_sw128(x + m * 2048, G::kBoxBytes, 1024), G::kIdescMn, (accumulate || m > 0) ? 1u : 0u);
 }
 
 template <int D, bool F16>

@@ -1,0 +1,613 @@
+// Backward of softmax differential attention on the tensor cores (tcgen05,
+// TMEM, TMA): bf16 or fp16, head_dim 64 / 128.  Formulas in tda_sdiff.h; row
+// table {L_m(i), D_m(i)} from the row-sum pass (rows past Sq: {+inf, 0}).
+//
+// Two kernels, no atomic sums (the same bits every time):
+//   dkv, a CTA a tile of 128 keys of one kv head.  Rows are keys: per query tile
+//     S^T = K_m Q_m^T, dP^T = V dout^T, then dV += P'^T dout, dK_m += dS^T Q_m,
+//     P'_1 = P_1, P'_2 = -lambda P_2.  It walks map 1's query tiles of every head
+//     of the group, writes dK_1, then map 2's: dV sums both maps and all heads in TMEM.
+//   dq, a CTA a tile of 128 queries of one head and map:
+//     S = Q_m K_m^T, dP = dout V^T, dQ_m += dS K_m.
+// Eight warps hold the weights between the two halves of a step: while they
+// exponentiate S, the tensor cores run dK (dQ) of the last step and dP; while
+// they form dS, dV and the next S.  P and dS enter the products as one 16-bit
+// value each (2^-9 / 2^-12 of an element, averaged over a row); sums, the
+// difference dP - D and the exponent stay in fp32.
+#include <cstring>
+
+#include "tda_sdiff_tc.cuh"
+
+namespace tda {
+namespace {
+
+using namespace sd;
+
+constexpr int kThreads = 320;
+constexpr int kWorkThreads = 256;
+constexpr int kTab = 4;
+constexpr int ST_KP = 0x901, ST_KM = 0x902, ST_KW = 0x903, ST_QP = 0xa01, ST_QM = 0xa02, ST_QW = 0xa03;
+
+template <int D, bool F16>
+struct KvC : Geo<D, F16> {
+  using G = Geo<D, F16>;
+  static constexpr int kSlots = 4;
+  static constexpr int kOffRing = 2 * G::kTileBytes;  // K, V, then the Q / dout ring
+  static constexpr int kOffTab = kOffRing + kSlots * G::kTileBytes;
+  static constexpr int kOffBar = kOffTab + kTab * kTile * 8;
+  static constexpr int kSmem = kOffBar + 1024 + 1024;
+  static_assert(kSmem <= kSmemBudget, "shared memory");
+  static constexpr uint32_t kS = 0, kP = 128, kDV = 256, kDK = 384;
+};
+
+struct KvBars {
+  uint64_t k_full, v_full, k_free, s_full, dp_full, p_full, ds_full, map_done, drain;
+  uint64_t slot_full[4], slot_empty[4], tab_full[kTab], tab_empty[kTab];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct KvWork {
+  int b, kvh, kt, i0, per_map;  // first query tile, steps of one map
+};
+
+template <int D, bool F16>
+__device__ void kv_produce(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const WaitCtl& ctl, const KvWork& w, const float2* table,
+                           int pad) {
+  using C = KvC<D, F16>;
+  const SdParams& p = tp.p;
+  mbar_arrive_expect_tx(&bars->v_full, C::kTileBytes);
+  load_tile<D, F16>(smem + C::kTileBytes, &tp.m.v, &bars->v_full, w.kt * kTile, w.kvh, w.b);
+  bool ok = true;
+  int t = 0, idx = 0, n_k = 0;
+  for (int m = 0; m < 2 && ok; ++m) {
+    if (m == 1) ok = mbar_wait(&bars->k_free, 0, ctl, ST_KP);
+    if (!ok) break;
+    mbar_arrive_expect_tx(&bars->k_full, C::kTileBytes);
+    load_tile<D, F16>(smem, &tp.m.k[m], &bars->k_full, w.kt * kTile, w.kvh, w.b);
+    ++n_k;
+    for (int h = w.kvh * p.group; h < (w.kvh + 1) * p.group && ok; ++h) {
+      for (int i = w.i0; i < tp.n_qt; ++i, ++t) {
+        const int e = t % kTab;
+        ok = mbar_wait(&bars->tab_empty[e], ((t / kTab) & 1) ^ 1, ctl, ST_KP);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&bars->tab_full[e], kTile * 8);
+        const long long row = (static_cast<long long>(m) * p.B + w.b) * p.H + h;
+        bulk_load(smem + C::kOffTab + e * kTile * 8, table + row * pad + i * kTile, kTile * 8, &bars->tab_full[e]);
+        for (int x = 0; x < 2; ++x) {
+          const int slot = idx % C::kSlots;
+          ok = mbar_wait(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_KP);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
+          load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, x ? &tp.m.dout : &tp.m.q[m], &bars->slot_full[slot], i * kTile, h,
+                            w.b);
+          ++idx;
+        }
+        if (!ok) {
+          ++t;  // its table entry is in flight
+          break;
+        }
+      }
+    }
+  }
+  if (!ok) {
+    drain_wait(&bars->v_full, 0, ctl);
+    if (n_k > 0) drain_wait(&bars->k_full, (n_k - 1) & 1, ctl);
+    for (int i = idx > C::kSlots ? idx - C::kSlots : 0; i < idx; ++i)
+      drain_wait(&bars->slot_full[i % C::kSlots], (i / C::kSlots) & 1, ctl);
+    for (int i = t > kTab ? t - kTab : 0; i < t; ++i) drain_wait(&bars->tab_full[i % kTab], (i / kTab) & 1, ctl);
+  }
+}
+
+template <int D, bool F16>
+__device__ void kv_issue(uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32_t tmem, int per_map) {
+  using C = KvC<D, F16>;
+  const uint32_t k = smem_u32(smem), v = k + C::kTileBytes, ring = smem_u32(smem + C::kOffRing);
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (ok) ok = mbar_wait(bar, parity, ctl, ST_KM);
+    if (ok) tc_fence_after();
+  };
+  auto acquire = [&](int idx) {
+    wait(&bars->slot_full[idx % C::kSlots], (idx / C::kSlots) & 1);
+    return ring + (idx % C::kSlots) * C::kTileBytes;
+  };
+  auto slot = [&](int idx) { return ring + (idx % C::kSlots) * C::kTileBytes; };
+  auto score = [&](int t) {  // S^T(t) = K Q(t)^T
+    const uint32_t q = acquire(2 * t);
+    if (!ok) return;
+    mma_score<D, F16>(tmem + C::kS, k, q);
+    tc_commit(&bars->s_full);
+  };
+  auto dprob = [&](int t) {  // dP^T(t) = V dout(t)^T
+    const uint32_t g = acquire(2 * t + 1);
+    if (!ok) return;
+    mma_score<D, F16>(tmem + C::kP, v, g);
+    tc_commit(&bars->dp_full);
+  };
+  wait(&bars->v_full, 0);
+  for (int m = 0; m < 2 && ok; ++m) {
+    const int t0 = m * per_map, t1 = t0 + per_map;
+    wait(&bars->k_full, m);
+    score(t0);
+    dprob(t0);
+    for (int t = t0; t < t1 && ok; ++t) {
+      wait(&bars->p_full, t & 1);
+      if (!ok) break;
+      mma_weights<D, F16, true>(tmem + C::kDV, tmem + C::kS, slot(2 * t + 1), t > 0);
+      if (t + 1 < t1) score(t + 1);
+      wait(&bars->ds_full, t & 1);
+      if (!ok) break;
+      mma_weights<D, F16, true>(tmem + C::kDK, tmem + C::kP, slot(2 * t), t > t0);
+      tc_commit(&bars->slot_empty[(2 * t) % C::kSlots]);
+      tc_commit(&bars->slot_empty[(2 * t + 1) % C::kSlots]);
+      if (t + 1 < t1) dprob(t + 1);
+    }
+    if (ok) tc_commit(&bars->map_done);
+  }
+  if (!ok) {
+    tc_commit(&bars->drain);
+    drain_wait(&bars->drain, 0, ctl);
+  }
+}
+
+// 32 accumulator columns of this thread's row, scaled, into the staged 16-bit tile
+template <int D, bool F16>
+__device__ __forceinline__ void stage_accumulator(uint8_t* boxes, uint32_t col, int row, int wg, float scale, bool zero) {
+#pragma unroll
+  for (int x = wg * (D / 2); x < (wg + 1) * (D / 2); x += 32) {
+    float a[32];
+    if (!zero) {
+      uint32_t u[32];
+      tmem_ld32(col + x, u);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) a[i] = __uint_as_float(u[i]) * scale;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) a[i] = 0.f;
+    }
+    stage_16<F16>(boxes, row, x, a);
+  }
+}
+
+template <int D, bool F16>
+__device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32_t tmem, const KvWork& w, int len,
+                        int warp, int lane) {
+  using C = KvC<D, F16>;
+  const SdParams& p = tp.p;
+  const int wg = warp >> 2, row = (warp & 3) * 32 + lane, key = w.kt * kTile + row, off = p.Sk - p.Sq;
+  const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const uint32_t s_col = tmem + lane_off + C::kS + 64 * wg, p_col = tmem + lane_off + C::kP + 64 * wg;
+  const bool dead = key >= len;          // past the sequence's length: no weight, whatever K and V hold there
+  const bool lone = len <= 1;            // weight 1 whatever the score: no dS
+  const float c = p.c;
+  bool ok = true;
+  int t = 0;
+  if (w.per_map > 0) ok = mbar_wait_warp(&bars->v_full, 0, ctl, ST_KW);
+  for (int m = 0; m < 2; ++m) {
+    for (int h = w.kvh * p.group; h < (w.kvh + 1) * p.group && ok; ++h) {
+      const float wt = m ? -lambda_at(p.lam, w.b, h) : 1.0f;
+      for (int i = w.i0; i < tp.n_qt && w.per_map > 0; ++i, ++t) {
+        const int e = t % kTab;
+        ok = mbar_wait_warp(&bars->tab_full[e], (t / kTab) & 1, ctl, ST_KW);
+        if (ok) ok = mbar_wait_warp(&bars->s_full, t & 1, ctl, ST_KW);
+        if (!ok) break;
+        tc_fence_after();
+        const float4* tab = reinterpret_cast<const float4*>(smem + C::kOffTab + e * kTile * 8) + 32 * wg;
+        const bool masked = (w.kt + 1) * kTile > len || (p.causal && i * kTile + off < (w.kt + 1) * kTile - 1) || lone;
+        // queries of this tile in front of `lo` do not see the key
+        const int lo = dead ? kTile : (p.causal ? key - off - i * kTile : 0);
+        float pr[64];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t s[32];
+          tmem_ld32(s_col + 32 * x, s);
+          tmem_wait_ld();
+#pragma unroll
+          for (int y = 0; y < 32; y += 2) {
+            const float4 q = tab[16 * x + y / 2];  // {L, D} of two queries
+            const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(-q.x, -q.z));
+            const float2 r = __fmul2_rn(make_float2(fast_ex2(z.x), fast_ex2(z.y)), make_float2(wt, wt));
+            pr[32 * x + y] = r.x;
+            pr[32 * x + y + 1] = r.y;
+          }
+          if (masked) {
+#pragma unroll
+            for (int y = 0; y < 32; ++y) pr[32 * x + y] = 64 * wg + 32 * x + y >= lo ? pr[32 * x + y] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t u[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) u[y] = pack2<F16>(pr[32 * x + 2 * y], pr[32 * x + 2 * y + 1]);
+          tmem_st16(s_col + 16 * x, u);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full);
+
+        ok = mbar_wait_warp(&bars->dp_full, t & 1, ctl, ST_KW);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t s[32];
+          tmem_ld32(p_col + 32 * x, s);
+          tmem_wait_ld();
+#pragma unroll
+          for (int y = 0; y < 32; y += 2) {
+            const float4 q = tab[16 * x + y / 2];
+            const float2 d = __fadd2_rn(f2u(s[y], s[y + 1]), make_float2(-q.y, -q.w));
+            const float2 r = __fmul2_rn(make_float2(pr[32 * x + y], pr[32 * x + y + 1]), d);
+            pr[32 * x + y] = r.x;
+            pr[32 * x + y + 1] = r.y;
+          }
+          if (masked) {
+#pragma unroll
+            for (int y = 0; y < 32; ++y) pr[32 * x + y] = 64 * wg + 32 * x + y >= lo && !lone ? pr[32 * x + y] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t u[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) u[y] = pack2<F16>(pr[32 * x + 2 * y], pr[32 * x + 2 * y + 1]);
+          tmem_st16(p_col + 16 * x, u);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->ds_full);
+          mbar_arrive(&bars->tab_empty[e]);
+        }
+      }
+    }
+    // dK_m through the K buffer (idle once every product of the map is done), and dV through V's at the end
+    if (ok && w.per_map > 0) ok = mbar_wait_warp(&bars->map_done, m, ctl, ST_KW);
+    tc_fence_after();
+    if (ok) {
+      stage_accumulator<D, F16>(smem, tmem + lane_off + C::kDK, row, wg, p.scale, w.per_map == 0);
+      if (m == 1) stage_accumulator<D, F16>(smem + C::kTileBytes, tmem + lane_off + C::kDV, row, wg, 1.0f, w.per_map == 0);
+      fence_proxy_async_smem();
+    }
+    tc_fence_before();
+    ok = named_barrier_and(1, kWorkThreads, ok);
+    if (!ok) break;
+    if (warp == 0 && lane == 0) {
+      const int at = w.b * p.Hkv + w.kvh;
+      for (int x = 0; x < D / 64; ++x) {
+        tma_store_3d(&tp.m.dk[m], smem + x * C::kBoxBytes, 64 * x, w.kt * kTile, at);
+        if (m == 1) tma_store_3d(&tp.m.dv, smem + C::kTileBytes + x * C::kBoxBytes, 64 * x, w.kt * kTile, at);
+      }
+      bulk_commit_group();
+      bulk_wait_group_read0();
+      if (m == 0 && w.per_map > 0) mbar_arrive(&bars->k_free);
+    }
+    if (w.per_map == 0) named_barrier_and(2, kWorkThreads, true);  // the staged zeros were read before they are written again
+  }
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_constant__ SdTcParams tp, const float2* table, int pad) {
+  using C = KvC<D, F16>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  KvBars* bars = reinterpret_cast<KvBars*>(smem + C::kOffBar);
+  const SdParams& p = tp.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  KvWork w;
+  const int bh = static_cast<int>(blockIdx.x) / tp.n_kt;
+  w.kt = static_cast<int>(blockIdx.x) % tp.n_kt;  // the first keys see the most queries
+  w.b = bh / p.Hkv;
+  w.kvh = bh % p.Hkv;
+  const int len = keys_of(p, w.b);
+  w.i0 = p.causal ? max(0, w.kt * kTile - (p.Sk - p.Sq)) / kTile : 0;
+  w.per_map = w.kt * kTile < len ? p.group * max(0, tp.n_qt - w.i0) : 0;
+  if (threadIdx.x == 0) {
+    uint64_t* one[] = {&bars->k_full, &bars->v_full, &bars->k_free, &bars->s_full, &bars->dp_full, &bars->map_done, &bars->drain};
+    for (uint64_t* x : one) mbar_init(x, 1);
+    mbar_init(&bars->p_full, 8);
+    mbar_init(&bars->ds_full, 8);
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&bars->slot_full[i], 1);
+      mbar_init(&bars->slot_empty[i], 1);
+    }
+    for (int i = 0; i < kTab; ++i) {
+      mbar_init(&bars->tab_full[i], 1);
+      mbar_init(&bars->tab_empty[i], 8);
+    }
+    bars->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const WaitCtl ctl = make_wait_ctl(&bars->abort_flag, tp.status, tp.timeout_ns);
+  if (warp < 8) {
+    kv_work<D, F16>(tp, smem, bars, ctl, tmem, w, len, warp, lane);
+  } else if (w.per_map > 0) {
+    if (warp == 8 && lane == 0) kv_produce<D, F16>(tp, smem, bars, ctl, w, table, pad);
+    if (warp == 9 && lane == 0) kv_issue<D, F16>(smem, bars, ctl, tmem, w.per_map);
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ================================================================== dq
+template <int D, bool F16>
+struct QC : Geo<D, F16> {
+  using G = Geo<D, F16>;
+  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr int kOffRing = 2 * G::kTileBytes;  // Q, dout, then the K / V ring
+  static constexpr int kOffBar = kOffRing + kSlots * G::kTileBytes;
+  static constexpr int kSmem = kOffBar + 1024 + 1024;
+  static_assert(kSmem <= kSmemBudget, "shared memory");
+  static __device__ __forceinline__ constexpr uint32_t s_col(int t) { return (t & 1) ? 128u : 0u; }
+  static constexpr uint32_t kP = 256, kDQ = 384;
+};
+
+struct QBars {
+  uint64_t q_full, o_full, drain, dp_full, dp_free;
+  uint64_t s_full[2], ds_full[2];
+  uint64_t slot_full[8], slot_empty[8];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+// ring order: K(0) V(0) K(1) V(1) ...
+template <int D, bool F16>
+__device__ void q_produce(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, int m, int b, int h, int kvh, int qt, int n) {
+  using C = QC<D, F16>;
+  mbar_arrive_expect_tx(&bars->q_full, 2 * C::kTileBytes);
+  load_tile<D, F16>(smem, &tp.m.q[m], &bars->q_full, qt * kTile, h, b);
+  load_tile<D, F16>(smem + C::kTileBytes, &tp.m.dout, &bars->q_full, qt * kTile, h, b);
+  bool ok = true;
+  int idx = 0;
+  for (; idx < 2 * n; ++idx) {
+    const int slot = idx % C::kSlots;
+    ok = mbar_wait(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_QP);
+    if (!ok) break;
+    mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
+    load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, idx & 1 ? &tp.m.v : &tp.m.k[m], &bars->slot_full[slot], idx / 2 * kTile,
+                      kvh, b);
+  }
+  if (!ok) {
+    drain_wait(&bars->q_full, 0, ctl);
+    for (int i = idx > C::kSlots ? idx - C::kSlots : 0; i < idx; ++i)
+      drain_wait(&bars->slot_full[i % C::kSlots], (i / C::kSlots) & 1, ctl);
+  }
+}
+
+template <int D, bool F16>
+__device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t tmem, int n) {
+  using C = QC<D, F16>;
+  const uint32_t q = smem_u32(smem), g = q + C::kTileBytes, ring = smem_u32(smem + C::kOffRing);
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (ok) ok = mbar_wait(bar, parity, ctl, ST_QM);
+    if (ok) tc_fence_after();
+  };
+  auto acquire = [&](int idx) {
+    wait(&bars->slot_full[idx % C::kSlots], (idx / C::kSlots) & 1);
+    return ring + (idx % C::kSlots) * C::kTileBytes;
+  };
+  auto score = [&](int t) {
+    const uint32_t k = acquire(2 * t);
+    if (!ok) return;
+    mma_score<D, F16>(tmem + C::s_col(t), q, k);
+    tc_commit(&bars->s_full[t & 1]);
+  };
+  auto dprob = [&](int t) {
+    const uint32_t v = acquire(2 * t + 1);
+    if (!ok) return;
+    mma_score<D, F16>(tmem + C::kP, g, v);
+    tc_commit(&bars->slot_empty[(2 * t + 1) % C::kSlots]);
+    tc_commit(&bars->dp_full);
+  };
+  wait(&bars->q_full, 0);
+  score(0);
+  dprob(0);
+  if (n > 1) score(1);
+  for (int t = 0; t < n && ok; ++t) {
+    if (t + 1 < n) {
+      wait(&bars->dp_free, t & 1);
+      dprob(t + 1);
+    }
+    wait(&bars->ds_full[t & 1], (t >> 1) & 1);
+    if (!ok) break;
+    mma_weights<D, F16, true>(tmem + C::kDQ, tmem + C::s_col(t), ring + ((2 * t) % C::kSlots) * C::kTileBytes, t > 0);
+    tc_commit(&bars->slot_empty[(2 * t) % C::kSlots]);
+    if (t + 2 < n) score(t + 2);
+  }
+  if (ok) {
+    tc_commit(&bars->o_full);
+  } else {
+    tc_commit(&bars->drain);
+    drain_wait(&bars->drain, 0, ctl);
+  }
+}
+
+template <int D, bool F16>
+__device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t tmem, const float2* table, int pad,
+                       int m, int b, int h, int qt, int n, int len, int warp, int lane) {
+  using C = QC<D, F16>;
+  const SdParams& p = tp.p;
+  const int wg = warp >> 2, row = (warp & 3) * 32 + lane, grow = qt * kTile + row, off = p.Sk - p.Sq;
+  const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const long long bh = static_cast<long long>(b) * p.H + h;
+  const float2 row_tab = table[(static_cast<long long>(m) * p.B * p.H + bh) * pad + grow];
+  const float L = row_tab.x, del = row_tab.y, c = p.c;
+  const int last = p.causal ? min(len - 1, grow + off) : len - 1;
+  bool ok = true;
+  for (int t = 0; t < n; ++t) {
+    ok = mbar_wait_warp(&bars->s_full[t & 1], (t >> 1) & 1, ctl, ST_QW);
+    if (!ok) break;
+    tc_fence_after();
+    const uint32_t s_col = tmem + lane_off + C::s_col(t);
+    const bool masked = (t + 1) * kTile > len || (p.causal && (t + 1) * kTile - 1 > qt * kTile + off);
+    float pr[64];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      uint32_t s[32];
+      tmem_ld32(s_col + 64 * wg + 32 * x, s);
+      tmem_wait_ld();
+#pragma unroll
+      for (int y = 0; y < 32; y += 2) {
+        const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(-L, -L));
+        pr[32 * x + y] = fast_ex2(z.x);
+        pr[32 * x + y + 1] = fast_ex2(z.y);
+      }
+    }
+    ok = mbar_wait_warp(&bars->dp_full, t & 1, ctl, ST_QW);
+    if (!ok) break;
+    tc_fence_after();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      uint32_t s[32];
+      tmem_ld32(tmem + lane_off + C::kP + 64 * wg + 32 * x, s);
+      tmem_wait_ld();
+      if (x == 1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->dp_free);
+      }
+#pragma unroll
+      for (int y = 0; y < 32; y += 2) {
+        const float2 d = __fadd2_rn(f2u(s[y], s[y + 1]), make_float2(-del, -del));
+        const float2 r = __fmul2_rn(make_float2(pr[32 * x + y], pr[32 * x + y + 1]), d);
+        pr[32 * x + y] = r.x;
+        pr[32 * x + y + 1] = r.y;
+      }
+      if (masked) {
+        const int lim = last - t * kTile - 64 * wg - 32 * x;
+#pragma unroll
+        for (int y = 0; y < 32; ++y) pr[32 * x + y] = y <= lim ? pr[32 * x + y] : 0.f;
+      }
+    }
+    // K rows past the length: zeroed (S is done with them) before the product with dS reads them
+    if (t == n - 1 && len < p.Sk && (t + 1) * kTile > len) {
+      if (wg == 0 && t * kTile + row >= len) zero_row<D>(smem + C::kOffRing + ((2 * t) % C::kSlots) * C::kTileBytes, row);
+      fence_proxy_async_smem();
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      uint32_t u[16];
+#pragma unroll
+      for (int y = 0; y < 16; ++y) u[y] = pack2<F16>(pr[32 * x + 2 * y], pr[32 * x + 2 * y + 1]);
+      tmem_st16(s_col + 64 * wg + 16 * x, u);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->ds_full[t & 1]);
+  }
+  if (ok && n > 0) ok = mbar_wait_warp(&bars->o_full, 0, ctl, ST_QW);
+  tc_fence_after();
+  const float w = (m ? -lambda_at(p.lam, b, h) : 1.0f) * p.scale;
+  uint8_t* stage = smem + C::kOffRing;
+  if (ok) {
+    stage_accumulator<D, F16>(stage, tmem + lane_off + C::kDQ, row, wg, w, n == 0);
+    fence_proxy_async_smem();
+  }
+  ok = named_barrier_and(2, kWorkThreads, ok);
+  if (ok && warp == 0 && lane == 0) {
+    for (int x = 0; x < D / 64; ++x) tma_store_3d(&tp.m.dq[m], stage + x * C::kBoxBytes, 64 * x, qt * kTile, static_cast<int>(bh));
+    bulk_commit_group();
+    bulk_wait_group_read0();
+  }
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_constant__ SdTcParams tp, const float2* table, int pad) {
+  using C = QC<D, F16>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  QBars* bars = reinterpret_cast<QBars*>(smem + C::kOffBar);
+  const SdParams& p = tp.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the heads and maps of one kv group run side by side, each group's longest rows first
+  const int per = 2 * p.group * tp.n_qt;
+  const int g = static_cast<int>(blockIdx.x) / per, r = static_cast<int>(blockIdx.x) % per;
+  const int b = g / p.Hkv, kvh = g % p.Hkv, x = r % (2 * p.group), qt = tp.n_qt - 1 - r / (2 * p.group);
+  const int m = x & 1, h = kvh * p.group + x / 2;
+  const int len = keys_of(p, b);
+  int n_keys = len <= 1 ? 0 : len;  // a lone key's weight is 1 whatever its score: no gradient
+  if (p.causal) n_keys = max(0, min(n_keys, min((qt + 1) * kTile, p.Sq) + p.Sk - p.Sq));
+  const int n = (n_keys + kTile - 1) / kTile;
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->o_full, 1);
+    mbar_init(&bars->drain, 1);
+    mbar_init(&bars->dp_full, 1);
+    mbar_init(&bars->dp_free, 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->ds_full[i], 8);
+    }
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&bars->slot_full[i], 1);
+      mbar_init(&bars->slot_empty[i], 1);
+    }
+    bars->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const WaitCtl ctl = make_wait_ctl(&bars->abort_flag, tp.status, tp.timeout_ns);
+  if (warp < 8) {
+    q_work<D, F16>(tp, smem, bars, ctl, tmem, table, pad, m, b, h, qt, n, len, warp, lane);
+  } else if (n > 0) {
+    if (warp == 8 && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, m, b, h, kvh, qt, n);
+    if (warp == 9 && lane == 0) q_issue<D, F16>(smem, bars, ctl, tmem, n);
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, bool F16>
+cudaError_t launch(const SdTcParams& tp, const float2* table, int pad, cudaStream_t s) {
+  auto kq = sdiff_tc_dq_kernel<D, F16>;
+  auto kk = sdiff_tc_dkv_kernel<D, F16>;
+  if (cudaError_t e = cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, QC<D, F16>::kSmem)) return e;
+  if (cudaError_t e = cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, KvC<D, F16>::kSmem)) return e;
+  kk<<<static_cast<unsigned>(tp.p.B * tp.p.Hkv * tp.n_kt), kThreads, KvC<D, F16>::kSmem, s>>>(tp, table, pad);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  kq<<<static_cast<unsigned>(2 * tp.p.B * tp.p.H * tp.n_qt), kThreads, QC<D, F16>::kSmem, s>>>(tp, table, pad);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_sdiff_tc_bwd(const SdTcParams& tp, int dtype, int D, cudaStream_t s) {
+  const float2* table = tp.p.table;
+  const int pad = tp.p.pad;
+  if (dtype == TDA_BF16) return D == 64 ? launch<64, false>(tp, table, pad, s) : launch<128, false>(tp, table, pad, s);
+  return D == 64 ? launch<64, true>(tp, table, pad, s) : launch<128, true>(tp, table, pad, s);
+}
+
+}  // namespace tda
