@@ -349,7 +349,8 @@ int tda_cache4_attention(int map, const void* q1, const void* q2, int dtype, con
                          int64_t num_pages, int64_t page_size, const int32_t* block_table, int64_t table_stride,
                          int64_t table_width, const int32_t* lengths, const void* lambda, int lambda_dtype,
                          int64_t lambda_stride_b, int64_t lambda_stride_h, float lambda_value, float scale, float beta,
-                         float relu_power, int normalize, void* workspace, size_t workspace_bytes, void* stream);
+                         float relu_power, int normalize, void* workspace, size_t workspace_bytes, int* status,
+                         void* stream);
 
 #ifdef __cplusplus
 }

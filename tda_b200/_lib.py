@@ -59,7 +59,7 @@ SIGNATURES = {
     "tda_cache4_read": (_I, [_P, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I, _P]),
     "tda_cache4_workspace_size": (_SZ, [_I, _I64, _I64, _I64, _I64, _I64, _I64]),
     "tda_cache4_attention": (_I, [_I, _P, _P, _I, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
-                                  _I, _I64, _I64, _F, _F, _F, _F, _I, _P, _SZ, _P]),
+                                  _I, _I64, _I64, _F, _F, _F, _F, _I, _P, _SZ, _P, _P]),
 }
 
 _lib = None

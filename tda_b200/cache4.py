@@ -19,6 +19,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
+from . import ops as _ops
 from .sdiff import _CODE, _on, _stream, lambda_ref, strides_of, view_of
 
 PAGE_SIZES = (16, 32, 64, 128)
@@ -219,8 +220,10 @@ def _attend(what, kind, q1, q2, cache, block_table, lengths, lambda_param, scale
                                       cache.num_pages, cache.page_size, block_table.data_ptr(), stride, width,
                                       lengths.data_ptr(), lp, lc, lsb, lsh, lv, scale, beta, relu_power,
                                       int(cache.normalize_keys), None if ws is None else ws.data_ptr(), ws_n,
-                                      _stream(dev))
+                                      _ops._status_word(dev).data_ptr(), _stream(dev))
     _lib.check(rc)
+    if _ops._SYNC_CHECK:
+        _ops.check_status(dev)
     return out
 
 

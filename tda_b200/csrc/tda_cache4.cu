@@ -174,6 +174,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
   }
 }
 
+// byte offset of the slab that holds a slot's rows of one head
+template <int D>
+__device__ __forceinline__ size_t slab_of(int slot, int h, int heads, int page) {
+  return (static_cast<size_t>(slot / page) * heads + h) * cache4_block_bytes(page, D) +
+         static_cast<size_t>(slot % page / kSlab4) * cache4_slab_bytes(D);
+}
+
 // ================================================================== append
 struct AppendParams {
   const void* x[3];  // k1, k2, v: (tokens, heads, D)
@@ -308,12 +315,11 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const AppendParams p
       word |= static_cast<uint32_t>(c) << (4 * nib);
     }
   }
-  uint8_t* blk = p.cache + (static_cast<size_t>(slot / p.page) * p.heads + h) * cache4_block_bytes(p.page, D);
-  const int at = slot % p.page;
-  uint8_t* codes = blk + cache4_codes_at(xi, p.page, D) + at * cache4_row_bytes(D);
-  *reinterpret_cast<uint32_t*>(codes + l * (is_v ? D / 16 : D / 8) + 4 * w) = word;
+  uint8_t* slab = p.cache + slab_of<D>(slot, h, p.heads, p.page);
+  const int r = slot % kSlab4;
+  *reinterpret_cast<uint32_t*>(slab + cache4_codes_at(xi, D) + (is_v ? cache4_v_word(r, l, w, D) : cache4_k_word(r, l, w, D))) = word;
   if (l == 0) {
-    __nv_bfloat16* s = reinterpret_cast<__nv_bfloat16*>(blk + cache4_scales_at(xi, p.page, D) + at * cache4_scale_bytes(D));
+    __nv_bfloat16* s = reinterpret_cast<__nv_bfloat16*>(slab + cache4_scales_at(xi, D) + r * cache4_scale_bytes(D));
     if (is_v) {
       s[2 * w] = __float2bfloat16_rn(sc[0]);
       s[2 * w + 1] = __float2bfloat16_rn(sc[1]);
@@ -353,12 +359,11 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const ReadParams p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = 0.f;
   if (slot >= 0 && slot < p.num_slots) {
-    const uint8_t* blk = p.cache + (static_cast<size_t>(slot / p.page) * p.heads + h) * cache4_block_bytes(p.page, D);
-    const int at = slot % p.page;
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(blk + cache4_codes_at(xi, p.page, D) +
-                                                             at * cache4_row_bytes(D) + l * (is_v ? D / 16 : D / 8) + 4 * w);
-    const __nv_bfloat16* s =
-        reinterpret_cast<const __nv_bfloat16*>(blk + cache4_scales_at(xi, p.page, D) + at * cache4_scale_bytes(D));
+    const uint8_t* slab = p.cache + slab_of<D>(slot, h, p.heads, p.page);
+    const int rr = slot % kSlab4;
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(
+        slab + cache4_codes_at(xi, D) + (is_v ? cache4_v_word(rr, l, w, D) : cache4_k_word(rr, l, w, D)));
+    const __nv_bfloat16* s = reinterpret_cast<const __nv_bfloat16*>(slab + cache4_scales_at(xi, D) + rr * cache4_scale_bytes(D));
     const float s0 = __bfloat162float(s[is_v ? 2 * w : w]), s1 = __bfloat162float(s[is_v ? 2 * w + 1 : w]);
 #pragma unroll
     for (int r = 0; r < 2; ++r)

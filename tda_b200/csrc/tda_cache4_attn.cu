@@ -5,25 +5,28 @@
 //                    tau = beta sqrt(2 ln(len) / D), qh = q / max(|q|, 1e-12) with a cache of normalized keys
 //
 // Bound by the cache bytes: 3 (D/2 + D/16) a token and kv head (216 at D = 128).
-// A warp takes slabs of 16 tokens straight from global memory, the next slab's
-// loads in flight while it computes on one: K rows and V rows are stored in
-// the order of matrix fragments (tda_cache4.cuh), so nothing passes through
-// shared memory.  The products are m16n8k16 with the cache as the A operand
-// and 8 columns of queries: up to 4 heads of the kv head's group times the two
-// maps, so that both maps share one pass over V:
-//   S^T (16 tokens x 8) = K Q^T       a lane keeps the product of its columns' map
+// Each warp walks slabs of 16 tokens by itself: one bulk copy a slab into its
+// own ring in shared memory, several slabs ahead, no barrier with other warps.
+// The products are m16n8k16 with the cache as the A operand, stored in fragment
+// order (tda_cache4.cuh), and 8 columns of queries: up to 4 heads of the kv
+// head's group times the two maps, so that both maps share one pass over V:
+//   S^T (16 tokens x 8) = K1 [Q1 0]^T + K2 [0 Q2]^T
 //   O^T (D x 8) += V^T (P s)^T
-// Codes become 16-bit floats by the exponent trick: (word >> 4i) & 0x000f000f
-// | magic is 128 + n (bf16) or 1024 + n (fp16), n = code + 8.  For K the
-// product starts from -(136 or 1032) times the sum of the group's q, which
-// removes the offset without an instruction (the cancelled part is exact
-// products summed in fp32: an error near 1e-5 of |q| times a code unit).  V
-// subtracts it (exact).  K's scale multiplies a group's fp32 product, V's
-// scale the weight.  Weights round to bf16.  Softmax: bf16(p s), 2^-9 of a
-// weight, far below the 2^-4 of a code.  The threshold form knows its whole
-// weight w = (p1 - lambda p2) s at once, which takes the columns of one map, so
-// the other four carry what rounding w left: 2^-17, and nothing is lost where
-// the two maps cancel.
+// Codes become fp16 by the exponent trick, (w & 0x000f000f) | 0x6400 = 1024 + n
+// and (w & 0x00f000f0) | 0x6400 = 1024 + 16 n, n = code + 8: one logic operation
+// a register and a shift every fourth (logic operations issue at half rate and
+// are what bounds the kernel next to DRAM).  The factor 16 is divided out of
+// those dims of q, and of those rows of O at the end.  For K the product starts
+// from minus the offset's share, which removes it without an instruction (exact
+// products summed in fp32: an error near 1e-4 of |q| times a code unit); V
+// subtracts it (exact).  K's scale multiplies a group's fp32 product.
+// q enters as fp16 after division by a power of two that brings its largest
+// element to [1, 2): exact but for elements 2^-21 below it.
+// V's scale goes into the weight, w = p s, rounded to fp16 (2^-12) relative to a
+// running bound M >= log2 of the largest w so far (minus 8): weights lie below
+// 2^8 and small scales do not underflow.  The threshold form forms its whole
+// weight (p1 - lambda p2) s at once, which takes the columns of one map, so the
+// other four carry what rounding left: nothing is lost where the maps cancel.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -32,6 +35,7 @@
 #include "tda_cache4.cuh"
 #include "tda_host.h"
 #include "tda_ptx.cuh"
+#include "tda_transform.cuh"
 
 namespace tda {
 
@@ -40,8 +44,19 @@ int cache4_check(const void* cache, int64_t num_pages, int64_t heads, int64_t D,
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kSlab = 16;
 constexpr int kHeadsPerBlock = 4;
+constexpr int ST_CACHE = 0xb01;
+constexpr float kInf = __builtin_huge_valf();
+
+template <int D>
+struct DC {
+  static constexpr int kSlabBytes = cache4_slab_bytes(D);
+  static constexpr int kStages = D == 128 ? 4 : 8;
+  static constexpr int kRing = kStages * kSlabBytes;
+  static constexpr int kStride = D + 4;  // floats of a joined row
+  static constexpr int kSmem = kWarps * kRing;
+  static_assert(kSmem >= kWarps * 8 * kStride * 4, "the ring holds the warps' results at the end");
+};
 
 struct AttnParams {
   const void* q1;
@@ -55,6 +70,8 @@ struct AttnParams {
   long long table_stride;
   long long num_pages;
   LambdaRef lam;
+  int* status;
+  unsigned long long timeout_ns;
   int width;
   int page_log2;
   int B;
@@ -70,7 +87,7 @@ struct AttnParams {
   int normalize;
 };
 
-// floats of one partial result: softmax {m1, l1, m2, l2, -, -, -, -, O1[D], O2[D]}, threshold O[D]
+// floats of one partial result: softmax {M1, l1, M2, l2, -, -, -, -, O1[D], O2[D]}, threshold O[D]
 template <int D, bool THR>
 __host__ __device__ constexpr int part_floats() {
   return THR ? D : 8 + 2 * D;
@@ -82,86 +99,42 @@ __device__ __forceinline__ uint32_t movm(uint32_t x) {
   return y;
 }
 
-template <bool F16>
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1, float c0, float c1, float c2, float c3) {
-  if constexpr (F16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <bool F16>
-__device__ __forceinline__ uint32_t widen(uint32_t w, int i) {
-  return ((w >> (4 * i)) & 0x000f000fu) | (F16 ? 0x64006400u : 0x43004300u);
-}
-
-// 128 + n -> n - 8, exact in bf16
-__device__ __forceinline__ uint32_t widen_v(uint32_t w, int i) {
-  const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+// two nibbles as 1024 + n, and two more as 1024 + 16 n
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return (w & 0x000f000fu) | 0x64006400u; }
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return (w & 0x00f000f0u) | 0x64006400u; }
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x43084308u));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// codes -7..7, and 16 times them
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return sub_f16x2(low_nibbles(w), 0x64086408u); }    // 1032
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return sub_f16x2(high_nibbles(w), 0x64806480u); }  // 1152
 
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
   static_assert(N == 1 || N == 2 || N == 4, "");
   if constexpr (N == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   } else if constexpr (N == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x, w[1] = v.y;
   } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
 __device__ __forceinline__ float scale_of(const uint32_t* w, int i) {
   const uint32_t x = w[i >> 1];
   return __uint_as_float((i & 1) ? (x & 0xffff0000u) : (x << 16));
-}
-
-template <int D>
-struct Slab {
-  uint32_t k[2][2][D / 32];  // map, row g / g + 8
-  uint32_t v[4][D / 64];     // tokens 2t, 2t+1, 2t+8, 2t+9
-  uint32_t ks[2][D / 64];    // K scales of the lane's map, rows g / g + 8
-  uint32_t vs[2][D / 64];
-  bool ok;                   // the page lies in the cache
-};
-
-template <int D>
-__device__ __forceinline__ void load_slab(Slab<D>& s, const AttnParams& p, const int* row, int kvh, int tok, int len,
-                                          int g, int t) {
-  if (tok >= len) return;
-  const int page = 1 << p.page_log2;
-  const int pg = __ldg(row + (tok >> p.page_log2));
-  s.ok = pg >= 0 && pg < p.num_pages;
-  if (!s.ok) return;
-  const uint8_t* blk = p.cache + (static_cast<size_t>(pg) * p.kv_heads + kvh) * cache4_block_bytes(page, D);
-  const int r0 = tok & (page - 1);
-  const int rb = static_cast<int>(cache4_row_bytes(D)), sb = static_cast<int>(cache4_scale_bytes(D));
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      load_words(s.k[m][h], blk + cache4_codes_at(m, page, D) + (r0 + g + 8 * h) * rb + t * (D / 8));
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    load_words(s.ks[h], blk + cache4_scales_at(t >> 1, page, D) + (r0 + g + 8 * h) * sb);
-    load_words(s.vs[h], blk + cache4_scales_at(2, page, D) + (r0 + g + 8 * h) * sb);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    load_words(s.v[i], blk + cache4_codes_at(2, page, D) + (r0 + 2 * t + (i & 1) + 8 * (i >> 1)) * rb + g * (D / 16));
 }
 
 template <int PM>
@@ -176,54 +149,127 @@ __device__ __forceinline__ float relu_pow(float z, float p) {
 // a map's part of the output; nothing was seen where the sum is zero
 __device__ __forceinline__ float share(float o, float l) { return l == 0.0f ? 0.0f : o / l; }
 
+__device__ __forceinline__ int length_of(const AttnParams& p, int b) { return max(0, min(p.lengths[b], p.width << p.page_log2)); }
+
+template <bool F16>
+__device__ __forceinline__ void write_out(const AttnParams& p, int b, int head, int D, int d, float y) {
+  const long long at = (static_cast<long long>(b) * p.heads + head) * D + d;
+  if constexpr (F16)
+    static_cast<__half*>(p.out)[at] = __float2half_rn(y);
+  else
+    static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+}
+
 // one (chunk, kv head x head block, request)
 template <int D, bool THR, bool F16, int PM>
-__global__ void __launch_bounds__(32 * kWarps) cache4_attn_kernel(const AttnParams p) {
-  constexpr int W = D / 32;   // groups
-  constexpr int kStride = D + 4;
+__global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __grid_constant__ AttnParams p) {
+  using C = DC<D>;
+  constexpr int W = D / 32;  // groups
+  constexpr int S = C::kStages;
+  extern __shared__ __align__(128) uint8_t ring_all[];
+  __shared__ uint64_t full[kWarps][S];
   __shared__ float s_m[kWarps][8], s_l[kWarps][8];
-  __shared__ float s_o[kWarps][8][kStride];
+  __shared__ int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int b = blockIdx.z;
   const int kvh = blockIdx.y / p.head_blocks, hb = blockIdx.y % p.head_blocks;
-  const int len = max(0, min(p.lengths[b], p.width << p.page_log2));
+  const int len = length_of(p, b);
   const int lo = blockIdx.x * p.chunk, hi = min(len, lo + p.chunk);
   if (lo >= hi && !(blockIdx.x == 0 && p.n_chunks == 1)) return;
   const int head0 = kvh * p.group + hb * kHeadsPerBlock;
   const int n_heads = min(kHeadsPerBlock, p.group - hb * kHeadsPerBlock);
+  if (lane == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&full[warp][i], 1);
+    if (warp == 0) abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const WaitCtl ctl = make_wait_ctl(&abort_flag, p.status, p.timeout_ns);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // this warp's slabs: tokens lo + 16 (i kWarps + warp)
+  uint8_t* ring = ring_all + warp * C::kRing;
+  const int* row = p.table + b * p.table_stride;
+  const int n = max(0, (hi - lo - 16 * warp + 16 * kWarps - 1) / (16 * kWarps));
+  const int page_mask = (1 << p.page_log2) - 1;
+  auto token = [&](int i) { return lo + 16 * (i * kWarps + warp); };
+  auto page_of = [&](int i) { return i < n ? __ldg(row + (token(i) >> p.page_log2)) : -1; };
+  uint32_t in_cache = 0;  // bit i % 32: slab i's page lies in the cache
+  auto fetch = [&](int i, int pg) {
+    const bool good = pg >= 0 && pg < p.num_pages;
+    in_cache = (in_cache & ~(1u << (i & 31))) | (static_cast<uint32_t>(good) << (i & 31));
+    if (good && lane == 0) {
+      uint64_t* bar = &full[warp][i % S];
+      mbar_arrive_expect_tx(bar, C::kSlabBytes);
+      bulk_load(ring + (i % S) * C::kSlabBytes,
+                p.cache + (static_cast<size_t>(pg) * p.kv_heads + kvh) * cache4_block_bytes(page_mask + 1, D) +
+                    static_cast<size_t>((token(i) & page_mask) >> 4) * C::kSlabBytes,
+                C::kSlabBytes, bar);
+    } else if (lane == 0 && i < n) {
+      mbar_arrive(&full[warp][i % S]);  // nothing to copy: the phase completes all the same
+    }
+  };
+  {
+    int pg[S - 1];
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) pg[i] = page_of(i);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+      if (i < n) fetch(i, pg[i]);
+  }
+  int next_page = page_of(S - 1);
 
   // queries: column g is head g % 4 of map g / 4; lane t holds dims 16 s + 4 t..
-  uint32_t q[2 * W][2];
-  float qsum[W][2];  // of this lane's columns 2t, 2t + 1, times the offset
-  float rq[2] = {1.f, 1.f};
+  uint32_t q1[2 * W][2], q2[2 * W][2];
+  float off[W][2];  // of this lane's columns 2t, 2t + 1: minus the offset's share of a group's product
+  float rq[2];      // what a column's product is multiplied by
   {
     const int m = g >> 2, j = g & 3;
     const bool live = j < n_heads;
-    const char* base = static_cast<const char*>(m ? p.q2 : p.q1) +
-                       2 * (b * p.q_sb[m] + (head0 + (live ? j : 0)) * p.q_sh[m]);
-    float sum[W], ss = 0.f;
+    const char* base = static_cast<const char*>(m ? p.q2 : p.q1) + 2 * (b * p.q_sb[m] + (head0 + (live ? j : 0)) * p.q_sh[m]);
+    float x[2 * W][4], ss = 0.f, top = 0.f;
 #pragma unroll
     for (int s = 0; s < 2 * W; ++s) {
       uint2 v = make_uint2(0u, 0u);
       if (live) v = *reinterpret_cast<const uint2*>(base + 2 * (16 * s + 4 * t));
-      q[s][0] = v.x;
-      q[s][1] = v.y;
-      const float2 x = F16 ? unpack_f16x2(v.x) : unpack_bf16x2(v.x), y = F16 ? unpack_f16x2(v.y) : unpack_bf16x2(v.y);
-      const float add = (x.x + x.y) + (y.x + y.y);
-      sum[s >> 1] = (s & 1) ? sum[s >> 1] + add : add;
-      ss = fmaf(x.x, x.x, fmaf(x.y, x.y, fmaf(y.x, y.x, fmaf(y.y, y.y, ss))));
+      const float2 a = F16 ? unpack_f16x2(v.x) : unpack_bf16x2(v.x), c = F16 ? unpack_f16x2(v.y) : unpack_bf16x2(v.y);
+      x[s][0] = a.x, x[s][1] = a.y, x[s][2] = c.x, x[s][3] = c.y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ss = fmaf(x[s][i], x[s][i], ss);
+        top = fmaxf(top, fabsf(x[s][i]));
+      }
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
+      ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    // 2^e <= top < 2^(e + 1); both powers are normal numbers for any top but 0
+    const uint32_t e = min(max(__float_as_uint(top) >> 23, 2u), 252u);
+    const float up = __uint_as_float(e << 23), down = __uint_as_float((254u - e) << 23);
+    float sum[W];
+#pragma unroll
+    for (int s = 0; s < 2 * W; ++s) {
+      const uint32_t a = pack_f16x2(x[s][0] * down, x[s][1] * down);
+      const uint32_t c = pack_f16x2(x[s][2] * (down * 0.0625f), x[s][3] * (down * 0.0625f));
+      q1[s][0] = m ? 0u : a;
+      q1[s][1] = m ? 0u : c;
+      q2[s][0] = m ? a : 0u;
+      q2[s][1] = m ? c : 0u;
+      const float2 ra = unpack_f16x2(a), rc = unpack_f16x2(c);
+      const float add = -1032.0f * (ra.x + ra.y) - 1152.0f * (rc.x + rc.y);
+      sum[s >> 1] = (s & 1) ? sum[s >> 1] + add : add;
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1)
 #pragma unroll
       for (int w = 0; w < W; ++w) sum[w] += __shfl_xor_sync(0xffffffffu, sum[w], o);
-      ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    }
-    const float r = p.normalize ? 1.0f / fmaxf(sqrtf(ss), 1e-12f) : 1.0f;
+    const float r = up * (THR ? (p.normalize ? 1.0f / fmaxf(sqrtf(ss), 1e-12f) : 1.0f) : p.scale);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int w = 0; w < W; ++w) qsum[w][c] = (F16 ? -1032.0f : -136.0f) * __shfl_sync(0xffffffffu, sum[w], 4 * (2 * t + c));
+      for (int w = 0; w < W; ++w) off[w][c] = __shfl_sync(0xffffffffu, sum[w], 4 * (2 * t + c));
       rq[c] = __shfl_sync(0xffffffffu, r, 4 * (2 * t + c));
     }
   }
@@ -237,115 +283,156 @@ __global__ void __launch_bounds__(32 * kWarps) cache4_attn_kernel(const AttnPara
   float o[D / 16][4];
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const int* row = p.table + b * p.table_stride;
+  float m[2] = {-kInf, -kInf}, l[2] = {0.f, 0.f};  // M and the sum of 2^(score - M), per column
 
-  Slab<D> cur, nxt;
-  cur.ok = nxt.ok = false;
-  int tok = lo + warp * kSlab;
-  load_slab(cur, p, row, kvh, tok, hi, g, t);
-  for (; tok < hi; tok += kWarps * kSlab) {
-    nxt.ok = false;
-    load_slab(nxt, p, row, kvh, tok + kWarps * kSlab, hi, g, t);
-    if (cur.ok) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
+  bool ok = true;
+  int i = 0;
+  for (; i < n; ++i) {
+    ok = mbar_wait_warp(&full[warp][i % S], (i / S) & 1, ctl, ST_CACHE);
+    if (!ok) break;
+    // every lane is done with slab i - 1: its stage takes slab i + S - 1
+    if (i + S - 1 < n) {
+      fetch(i + S - 1, next_page);
+      next_page = page_of(i + S);
+    }
+    if (!((in_cache >> (i & 31)) & 1u)) continue;
+    const uint8_t* slab = ring + (i % S) * C::kSlabBytes;
+    const int tok = token(i);
+    uint32_t vs[2][D / 64];
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    {
+      uint32_t k[2][2][W], ks[2][D / 64];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load_words(k[0][h], slab + cache4_codes_at(0, D) + cache4_k_word(g + 8 * h, t, 0, D));
+        load_words(k[1][h], slab + cache4_codes_at(1, D) + cache4_k_word(g + 8 * h, t, 0, D));
+        load_words(ks[h], slab + cache4_scales_at(0, D) + (second ? kSlab4 * cache4_scale_bytes(D) : 0) + (g + 8 * h) * cache4_scale_bytes(D));
+        load_words(vs[h], slab + cache4_scales_at(2, D) + (g + 8 * h) * cache4_scale_bytes(D));
+      }
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        float acc[2][4];
+        float acc[4] = {off[w][0], off[w][1], off[w][0], off[w][1]};
 #pragma unroll
         for (int mp = 0; mp < 2; ++mp) {
-          const uint32_t x = cur.k[mp][0][w], y = cur.k[mp][1][w];
-          mma16816<F16>(acc[mp], widen<F16>(x, 0), widen<F16>(y, 0), widen<F16>(x, 1), widen<F16>(y, 1), q[2 * w][0],
-                        q[2 * w][1], qsum[w][0], qsum[w][1], qsum[w][0], qsum[w][1]);
-          mma16816<F16>(acc[mp], widen<F16>(x, 2), widen<F16>(y, 2), widen<F16>(x, 3), widen<F16>(y, 3),
-                        q[2 * w + 1][0], q[2 * w + 1][1], acc[mp][0], acc[mp][1], acc[mp][2], acc[mp][3]);
+          const uint32_t x = k[mp][0][w], y = k[mp][1][w], x8 = x >> 8, y8 = y >> 8;
+          const uint32_t(&q)[2 * W][2] = mp ? q2 : q1;
+          mma16816(acc, low_nibbles(x), low_nibbles(y), high_nibbles(x), high_nibbles(y), q[2 * w][0], q[2 * w][1]);
+          mma16816(acc, low_nibbles(x8), low_nibbles(y8), high_nibbles(x8), high_nibbles(y8), q[2 * w + 1][0], q[2 * w + 1][1]);
         }
-        const float s0 = scale_of(cur.ks[0], w), s1 = scale_of(cur.ks[1], w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = fmaf(second ? acc[1][i] : acc[0][i], i < 2 ? s0 : s1, s[i]);
-      }
-      const bool in0 = tok + g < hi, in1 = tok + g + 8 < hi;
-      float pr[4];
-      if constexpr (THR) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float z = fmaf(s[i], rq[i & 1], -tau);
-          pr[i] = (i < 2 ? in0 : in1) ? relu_pow<PM>(z, p.relu_power) : 0.f;
-          const float other = __shfl_xor_sync(0xffffffffu, pr[i], 2);  // the same head's other map
-          pr[i] = second ? fmaf(-lam[i & 1], pr[i], other) : fmaf(-lam[i & 1], other, pr[i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = (i < 2 ? in0 : in1) ? s[i] * p.scale : -INFINITY;
-        // the running maximum moves only when a score passes it by 2^8: weights stay below 256
-        // and most slabs need neither the reduction nor the rescaling
-        const bool grow = fmaxf(s[0], s[2]) > m[0] + 8.f || fmaxf(s[1], s[3]) > m[1] + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
-          float n0 = fmaxf(s[0], s[2]), n1 = fmaxf(s[1], s[3]);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) {
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
-          }
-          n0 = fmaxf(n0, m[0]);
-          n1 = fmaxf(n1, m[1]);
-          const float f0 = m[0] == n0 ? 1.f : fast_ex2(m[0] - n0), f1 = m[1] == n1 ? 1.f : fast_ex2(m[1] - n1);
-          m[0] = n0;
-          m[1] = n1;
-          l[0] *= f0;
-          l[1] *= f1;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            o[i][0] *= f0;
-            o[i][2] *= f0;
-            o[i][1] *= f1;
-            o[i][3] *= f1;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pr[i] = fast_ex2(s[i] - m[i & 1]);
-        l[0] += pr[0] + pr[2];
-        l[1] += pr[1] + pr[3];
-      }
-      bool work = true;
-      if constexpr (THR) work = __any_sync(0xffffffffu, !(pr[0] == 0.f && pr[1] == 0.f && pr[2] == 0.f && pr[3] == 0.f));
-      if (work) {
-        uint32_t bf[W][2];
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          // rows past the length hold no token: their scales may be anything
-          const float s0 = in0 ? scale_of(cur.vs[0], w) : 0.f, s1 = in1 ? scale_of(cur.vs[1], w) : 0.f;
-          uint32_t r0 = pack_bf16x2(pr[0] * s0, pr[1] * s0), r1 = pack_bf16x2(pr[2] * s1, pr[3] * s1);
-          if constexpr (THR) {
-            if (second) {
-              const float2 h0 = unpack_bf16x2(r0), h1 = unpack_bf16x2(r1);
-              r0 = pack_bf16x2(pr[0] * s0 - h0.x, pr[1] * s0 - h0.y);
-              r1 = pack_bf16x2(pr[2] * s1 - h1.x, pr[3] * s1 - h1.y);
-            }
-          }
-          bf[w][0] = movm(r0);
-          bf[w][1] = movm(r1);
-        }
-#pragma unroll
-        for (int u = 0; u < D / 64; ++u) {
-          uint32_t a[2], c[2];
-          a[0] = __byte_perm(cur.v[0][u], cur.v[1][u], 0x5410);
-          a[1] = __byte_perm(cur.v[0][u], cur.v[1][u], 0x7632);
-          c[0] = __byte_perm(cur.v[2][u], cur.v[3][u], 0x5410);
-          c[1] = __byte_perm(cur.v[2][u], cur.v[3][u], 0x7632);
-#pragma unroll
-          for (int mm = 0; mm < 4; ++mm) {
-            const int n = 2 * (mm & 1), x = mm >> 1, mt = 4 * u + mm;
-            mma16816<false>(o[mt], widen_v(a[x], n), widen_v(a[x], n + 1), widen_v(c[x], n), widen_v(c[x], n + 1),
-                            bf[mt >> 1][0], bf[mt >> 1][1], o[mt][0], o[mt][1], o[mt][2], o[mt][3]);
-          }
-        }
+        const float s0 = scale_of(ks[0], w), s1 = scale_of(ks[1], w);
+        s[0] = fmaf(acc[0], s0, s[0]);
+        s[1] = fmaf(acc[1], s0, s[1]);
+        s[2] = fmaf(acc[2], s1, s[2]);
+        s[3] = fmaf(acc[3], s1, s[3]);
       }
     }
-    cur = nxt;
+    // rows past the length hold no token: their scales may be anything
+    const bool in0 = tok + g < hi, in1 = tok + g + 8 < hi;
+    float sv[2][W], svm[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      svm[h] = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        sv[h][w] = (h ? in1 : in0) ? scale_of(vs[h], w) : 0.f;
+        svm[h] = fmaxf(svm[h], sv[h][w]);
+      }
+      svm[h] = fmaxf(svm[h], 0x1p-100f);
+    }
+    float pr[4];
+    bool grow;
+    float top[2];  // log2 of the largest weights of the lane's columns
+    if constexpr (THR) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float z = fmaf(s[x], rq[x & 1], -tau);
+        pr[x] = (x < 2 ? in0 : in1) ? relu_pow<PM>(z, p.relu_power) : 0.f;
+        const float other = __shfl_xor_sync(0xffffffffu, pr[x], 2);  // the same head's other map
+        pr[x] = second ? fmaf(-lam[x & 1], pr[x], other) : fmaf(-lam[x & 1], other, pr[x]);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float y = fmaxf(fabsf(pr[c]) * svm[0], fabsf(pr[2 + c]) * svm[1]);
+        top[c] = y > 0.f ? fast_lg2(y) : -kInf;
+      }
+      if (!__any_sync(0xffffffffu, top[0] != -kInf || top[1] != -kInf || !(pr[0] + pr[1] + pr[2] + pr[3] == 0.f))) continue;
+    } else {
+      const float lg[2] = {fast_lg2(svm[0]), fast_lg2(svm[1])};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[x] = (x < 2 ? in0 : in1) ? s[x] * rq[x & 1] : -kInf;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) top[c] = fmaxf(s[c] + lg[0], s[2 + c] + lg[1]);
+    }
+    // M moves only when a weight passes it by 2^8: most slabs need neither the reduction nor the rescaling
+    grow = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f;
+    if (__any_sync(0xffffffffu, grow)) {
+      float f[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = top[c];
+#pragma unroll
+        for (int y = 4; y < 32; y <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, y));
+        if constexpr (THR) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));  // a head's two columns hold one weight
+        x = THR ? ceilf(fmaxf(x, m[c])) : fmaxf(x, m[c]);
+        f[c] = m[c] == x ? 1.f : fast_ex2(m[c] - x);
+        m[c] = x;
+        l[c] *= f[c];
+      }
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) o[x][y] *= f[y & 1];
+    }
+    if constexpr (THR) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) pr[x] *= m[x & 1] == -kInf ? 1.f : fast_ex2(-m[x & 1]);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) pr[x] = fast_ex2(s[x] - m[x & 1]);
+      l[0] += pr[0] + pr[2];
+      l[1] += pr[1] + pr[3];
+    }
+    uint32_t bf[W][2];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float x0 = pr[0] * sv[0][w], x1 = pr[1] * sv[0][w], x2 = pr[2] * sv[1][w], x3 = pr[3] * sv[1][w];
+      uint32_t r0 = pack_f16x2(x0, x1), r1 = pack_f16x2(x2, x3);
+      if constexpr (THR) {
+        if (second) {
+          const float2 h0 = unpack_f16x2(r0), h1 = unpack_f16x2(r1);
+          r0 = pack_f16x2(x0 - h0.x, x1 - h0.y);
+          r1 = pack_f16x2(x2 - h1.x, x3 - h1.y);
+        }
+      }
+      bf[w][0] = movm(r0);
+      bf[w][1] = movm(r1);
+    }
+    uint32_t v[4][D / 64];
+    {
+      const uint8_t* at = slab + cache4_codes_at(2, D) + lane * 16;
+      const uint4 x = *reinterpret_cast<const uint4*>(at);
+      if constexpr (D == 128) {
+        const uint4 y = *reinterpret_cast<const uint4*>(at + 512);
+        v[0][0] = x.x, v[0][1] = x.y, v[1][0] = x.z, v[1][1] = x.w;
+        v[2][0] = y.x, v[2][1] = y.y, v[3][0] = y.z, v[3][1] = y.w;
+      } else {
+        v[0][0] = x.x, v[1][0] = x.y, v[2][0] = x.z, v[3][0] = x.w;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {  // nibbles 0-3, 4-7 of every word
+        const uint32_t a = __byte_perm(v[0][u], v[1][u], y ? 0x7632 : 0x5410), c = __byte_perm(v[2][u], v[3][u], y ? 0x7632 : 0x5410);
+        const int mt = 4 * u + 2 * y;
+        mma16816(o[mt], low_codes(a), high_codes(a), low_codes(c), high_codes(c), bf[mt >> 1][0], bf[mt >> 1][1]);
+        mma16816(o[mt + 1], low_codes(a >> 8), high_codes(a >> 8), low_codes(c >> 8), high_codes(c >> 8), bf[mt >> 1][0], bf[mt >> 1][1]);
+      }
   }
+  if (!ok)
+    for (int j = i; j < min(n, i + S - 1); ++j) tc::drain_wait(&full[warp][j % S], (j / S) & 1, ctl);
 
-  // join the warps
+  // join the warps, through the ring's memory
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -356,44 +443,38 @@ __global__ void __launch_bounds__(32 * kWarps) cache4_attn_kernel(const AttnPara
     s_l[warp][2 * t] = l[0];
     s_l[warp][2 * t + 1] = l[1];
   }
+  __syncthreads();
+  float* s_o = reinterpret_cast<float*>(ring_all);
 #pragma unroll
   for (int mt = 0; mt < D / 16; ++mt) {
     const int d = 32 * (mt >> 1) + 4 * g + 2 * (mt & 1);
-    *reinterpret_cast<float2*>(&s_o[warp][2 * t][d]) = make_float2(o[mt][0], o[mt][2]);
-    *reinterpret_cast<float2*>(&s_o[warp][2 * t + 1][d]) = make_float2(o[mt][1], o[mt][3]);
+    *reinterpret_cast<float2*>(s_o + (warp * 8 + 2 * t) * C::kStride + d) = make_float2(o[mt][0], o[mt][2] * 0.0625f);
+    *reinterpret_cast<float2*>(s_o + (warp * 8 + 2 * t + 1) * C::kStride + d) = make_float2(o[mt][1], o[mt][3] * 0.0625f);
   }
   __syncthreads();
   constexpr int kPart = part_floats<D, THR>();
-  for (int i = threadIdx.x; i < n_heads * D; i += 32 * kWarps) {
-    const int j = i / D, d = i % D, head = head0 + j;
+  for (int x = threadIdx.x; x < n_heads * D; x += 32 * kWarps) {
+    const int j = x / D, d = x % D, head = head0 + j;
     float mm[2], ll[2], oo[2];
 #pragma unroll
     for (int mp = 0; mp < 2; ++mp) {
       const int c = 4 * mp + j;
-      float top = -INFINITY, sl = 0.f, so = 0.f;
-      if constexpr (!THR)
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][c]);
+      float top = -kInf, sl = 0.f, so = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][c]);
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = THR ? 1.f : (s_m[w][c] == -INFINITY ? 0.f : fast_ex2(s_m[w][c] - top));
-        // a warp without a token adds nothing, whatever its sums are (they are zeros)
+        // a warp that saw nothing adds its zeros; a threshold weight goes back to its own size
+        const float f = s_m[w][c] == -kInf ? 1.f : fast_ex2(THR ? s_m[w][c] : s_m[w][c] - top);
         sl = fmaf(s_l[w][c], f, sl);
-        so = fmaf(s_o[w][c][d], f, so);
+        so = fmaf(s_o[(w * 8 + c) * C::kStride + d], f, so);
       }
       mm[mp] = top;
       ll[mp] = sl;
       oo[mp] = so;
     }
     if (p.n_chunks == 1) {
-      float y;
-      if constexpr (THR)
-        y = oo[0] + oo[1];
-      else
-        y = share(oo[0], ll[0]) - lambda_at(p.lam, b, head) * share(oo[1], ll[1]);
-      const long long at = (static_cast<long long>(b) * p.heads + head) * D + d;
-      if constexpr (F16)
-        static_cast<__half*>(p.out)[at] = __float2half_rn(y);
-      else
-        static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+      write_out<F16>(p, b, head, D, d, THR ? oo[0] + oo[1] : share(oo[0], ll[0]) - lambda_at(p.lam, b, head) * share(oo[1], ll[1]));
     } else {
       float* part = p.part + ((static_cast<long long>(b) * p.heads + head) * p.n_chunks + blockIdx.x) * kPart;
       if constexpr (THR) {
@@ -407,49 +488,58 @@ __global__ void __launch_bounds__(32 * kWarps) cache4_attn_kernel(const AttnPara
   }
 }
 
-// Joins a request's chunks, in order: out of one head a block of D threads.
+// Joins a request's chunks, in order: one head a block of 2 D threads, a thread
+// a map and dim (threshold: half of the chunks and a dim).
 template <int D, bool THR, bool F16>
-__global__ void __launch_bounds__(D) cache4_join_kernel(const AttnParams p) {
-  const int head = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const int len = max(0, min(p.lengths[b], p.width << p.page_log2));
-  const int n = (len + p.chunk - 1) / p.chunk;
+__global__ void __launch_bounds__(2 * D) cache4_join_kernel(const __grid_constant__ AttnParams p) {
+  __shared__ float s_o[2][D], s_l[2];
   constexpr int kPart = part_floats<D, THR>();
+  const int head = blockIdx.x, b = blockIdx.y, mp = threadIdx.x / D, d = threadIdx.x % D;
+  const int n = (length_of(p, b) + p.chunk - 1) / p.chunk;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const float* part = p.part + (static_cast<long long>(b) * p.heads + head) * p.n_chunks * kPart;
-  float y = 0.f;
+  float o = 0.f, l = 0.f;
   if constexpr (THR) {
-    for (int c = 0; c < n; ++c) y += part[static_cast<long long>(c) * kPart + d];
-  } else if (n > 0) {
-    float top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[2] = {0.f, 0.f};
+#pragma unroll 4
+    for (int c = mp; c < n; c += 2) o += part[static_cast<long long>(c) * kPart + d];
+  } else {
+    float top = -kInf;
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) top = fmaxf(top, part[static_cast<long long>(c) * kPart + 2 * mp]);
+#pragma unroll 4
     for (int c = 0; c < n; ++c) {
       const float* q = part + static_cast<long long>(c) * kPart;
-      const float4 s = *reinterpret_cast<const float4*>(q);
-#pragma unroll
-      for (int mp = 0; mp < 2; ++mp) {
-        const float mc = mp ? s.z : s.x, lc = mp ? s.w : s.y, oc = q[8 + mp * D + d];
-        const float nt = fmaxf(top[mp], mc);
-        const float f = top[mp] == -INFINITY ? 0.f : fast_ex2(top[mp] - nt), h = mc == -INFINITY ? 0.f : fast_ex2(mc - nt);
-        l[mp] = l[mp] * f + lc * h;
-        o[mp] = o[mp] * f + oc * h;
-        top[mp] = nt;
-      }
+      const float mc = q[2 * mp], f = mc == -kInf ? 0.f : fast_ex2(mc - top);
+      l = fmaf(q[2 * mp + 1], f, l);
+      o = fmaf(q[8 + mp * D + d], f, o);
     }
-    y = share(o[0], l[0]) - lambda_at(p.lam, b, head) * share(o[1], l[1]);
   }
-  const long long at = (static_cast<long long>(b) * p.heads + head) * D + d;
-  if constexpr (F16)
-    static_cast<__half*>(p.out)[at] = __float2half_rn(y);
-  else
-    static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+  s_o[mp][d] = o;
+  if (d == 0) s_l[mp] = l;
+  __syncthreads();
+  if (mp == 0)
+    write_out<F16>(p, b, head, D, d,
+                   THR ? s_o[0][d] + s_o[1][d] : share(s_o[0][d], s_l[0]) - lambda_at(p.lam, b, head) * share(s_o[1][d], s_l[1]));
 }
 
 template <int D, bool THR, bool F16, int PM>
 cudaError_t launch(const AttnParams& p, cudaStream_t s) {
-  const dim3 grid(p.n_chunks, p.kv_heads * p.head_blocks, p.B);
-  cache4_attn_kernel<D, THR, F16, PM><<<grid, 32 * kWarps, 0, s>>>(p);
+  auto k = cache4_attn_kernel<D, THR, F16, PM>;
+  if (cudaError_t e = allow_shared<cache4_attn_kernel<D, THR, F16, PM>>(DC<D>::kSmem)) return e;
+  k<<<dim3(p.n_chunks, p.kv_heads * p.head_blocks, p.B), 32 * kWarps, DC<D>::kSmem, s>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.n_chunks == 1) return e;
-  cache4_join_kernel<D, THR, F16><<<dim3(p.heads, p.B), D, 0, s>>>(p);
-  return cudaGetLastError();
+  // the join's blocks start while the last chunks run and wait for the grid in front of them
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.heads, p.B);
+  cfg.blockDim = dim3(2 * D);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, cache4_join_kernel<D, THR, F16>, p);
 }
 
 template <int D, bool F16>
@@ -463,10 +553,11 @@ cudaError_t dispatch(const AttnParams& p, bool thr, cudaStream_t s) {
   }
 }
 
-// Tokens a block takes.  Enough blocks to fill the device a few times when the
-// table allows it, and at least 64 tokens (a slab a warp).
+// Tokens a block takes: one wave of resident blocks (4 an SM) where the table's
+// width allows it, at least two slabs a warp, at most 1024 (uneven lengths then
+// still spread over the device).
 int64_t chunk_tokens(int64_t B, int64_t head_groups, int64_t max_len) {
-  const int64_t want = 148 * 8 / (B * head_groups) + 1;  // chunks of one request
+  const int64_t want = 148 * 4 / (B * head_groups) + 1;  // chunks of one request
   int64_t chunk = ceil_div(ceil_div(max_len, want), 64) * 64;
   if (chunk < 128) chunk = 128;
   if (chunk > 1024) chunk = 1024;
@@ -495,7 +586,8 @@ int tda_cache4_attention(int map, const void* q1, const void* q2, int dtype, con
                          int64_t num_pages, int64_t page_size, const int32_t* block_table, int64_t table_stride,
                          int64_t table_width, const int32_t* lengths, const void* lambda, int lambda_dtype,
                          int64_t lambda_stride_b, int64_t lambda_stride_h, float lambda_value, float scale, float beta,
-                         float relu_power, int normalize, void* workspace, size_t workspace_bytes, void* stream) {
+                         float relu_power, int normalize, void* workspace, size_t workspace_bytes, int* status,
+                         void* stream) {
   if (map != TDA_MAP_SOFTMAX && map != TDA_MAP_THRESHOLD) return fail(TDA_ERR_INVALID, "map must be TDA_MAP_SOFTMAX or TDA_MAP_THRESHOLD");
   if (int e = cache4_check(cache, num_pages, kv_heads, head_dim, page_size)) return e;
   if (dtype != TDA_BF16 && dtype != TDA_F16) return fail(TDA_ERR_UNSUPPORTED, "queries must be TDA_BF16 or TDA_F16");
@@ -510,7 +602,10 @@ int tda_cache4_attention(int map, const void* q1, const void* q2, int dtype, con
   if (table_width > 0x7fffffffll / page_size - 8) return fail(TDA_ERR_INVALID, "table width * page_size must fit 31 bits");
   if (map == TDA_MAP_SOFTMAX && !(std::isfinite(scale) && scale > 0.f)) return fail(TDA_ERR_INVALID, "scale must be finite and positive");
   if (map == TDA_MAP_THRESHOLD && !(relu_power == relu_power)) return fail(TDA_ERR_INVALID, "relu_power is NaN");
+  if (!status) return fail(TDA_ERR_INVALID, "status must point to a device int32");
   AttnParams p;
+  p.status = status;
+  p.timeout_ns = wait_timeout_ns();
   p.q1 = q1;
   p.q2 = q2;
   for (int i = 0; i < 2; ++i) {

@@ -2,6 +2,7 @@
 // checks and the wait settings shared by every entry point.
 #pragma once
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -28,6 +29,19 @@ inline int cuda_fail(cudaError_t e, const char* what) {
 }
 
 inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Lets a kernel use `bytes` of dynamic shared memory, once a device.
+template <auto kKernel>
+cudaError_t allow_shared(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  if (cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return cudaSuccess;
+}
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

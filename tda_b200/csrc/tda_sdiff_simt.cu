@@ -414,15 +414,10 @@ __global__ void __launch_bounds__(256) sdiff_simt_dkv_kernel(const SdParams p) {
   }
 }
 
-template <typename K>
-cudaError_t shared_limit(K kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 template <typename T, int D>
 cudaError_t fwd(const SdParams& p, cudaStream_t s) {
   using C = SC<D>;
-  if (cudaError_t e = shared_limit(sdiff_simt_fwd_kernel<T, D>, C::kFwdSmem)) return e;
+  if (cudaError_t e = allow_shared<sdiff_simt_fwd_kernel<T, D>>(C::kFwdSmem)) return e;
   const unsigned grid = static_cast<unsigned>(p.B * p.H * ceil_div(p.Sq, C::BT));
   sdiff_simt_fwd_kernel<T, D><<<grid, 256, C::kFwdSmem, s>>>(p);
   return cudaGetLastError();
@@ -442,8 +437,8 @@ cudaError_t delta(const SdParams& p, cudaStream_t s) {
 template <typename T, int D>
 cudaError_t bwd(const SdParams& p, cudaStream_t s) {
   using C = SC<D>;
-  if (cudaError_t e = shared_limit(sdiff_simt_dq_kernel<T, D>, C::kDqSmem)) return e;
-  if (cudaError_t e = shared_limit(sdiff_simt_dkv_kernel<T, D>, C::kDkvSmem)) return e;
+  if (cudaError_t e = allow_shared<sdiff_simt_dq_kernel<T, D>>(C::kDqSmem)) return e;
+  if (cudaError_t e = allow_shared<sdiff_simt_dkv_kernel<T, D>>(C::kDkvSmem)) return e;
   sdiff_simt_dq_kernel<T, D><<<dim3(static_cast<unsigned>(p.B * p.H * ceil_div(p.Sq, C::BT)), 2), 256, C::kDqSmem, s>>>(p);
   if (cudaError_t e = cudaGetLastError()) return e;
   sdiff_simt_dkv_kernel<T, D><<<static_cast<unsigned>(p.B * p.Hkv * ceil_div(p.Sk, C::BT)), 256, C::kDkvSmem, s>>>(p);

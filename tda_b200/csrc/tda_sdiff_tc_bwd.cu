@@ -593,8 +593,8 @@ template <int D, bool F16>
 cudaError_t launch(const SdTcParams& tp, const float2* table, int pad, cudaStream_t s) {
   auto kq = sdiff_tc_dq_kernel<D, F16>;
   auto kk = sdiff_tc_dkv_kernel<D, F16>;
-  if (cudaError_t e = cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, QC<D, F16>::kSmem)) return e;
-  if (cudaError_t e = cudaFuncSetAttribute(kk, cudaFuncAttributeMaxDynamicSharedMemorySize, KvC<D, F16>::kSmem)) return e;
+  if (cudaError_t e = allow_shared<sdiff_tc_dq_kernel<D, F16>>(QC<D, F16>::kSmem)) return e;
+  if (cudaError_t e = allow_shared<sdiff_tc_dkv_kernel<D, F16>>(KvC<D, F16>::kSmem)) return e;
   kk<<<static_cast<unsigned>(tp.p.B * tp.p.Hkv * tp.n_kt), kThreads, KvC<D, F16>::kSmem, s>>>(tp, table, pad);
   if (cudaError_t e = cudaGetLastError()) return e;
   kq<<<static_cast<unsigned>(2 * tp.p.B * tp.p.H * tp.n_qt), kThreads, QC<D, F16>::kSmem, s>>>(tp, table, pad);

@@ -316,7 +316,7 @@ template <int D, bool F16>
 cudaError_t launch(const SdTcParams& tp, cudaStream_t s) {
   using C = FC<D, F16>;
   auto k = sdiff_tc_fwd_kernel<D, F16>;
-  if (cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem)) return e;
+  if (cudaError_t e = allow_shared<sdiff_tc_fwd_kernel<D, F16>>(C::kSmem)) return e;
   k<<<static_cast<unsigned>(tp.p.B * tp.p.H * tp.n_qt), kThreads, C::kSmem, s>>>(tp);
   return cudaGetLastError();
 }

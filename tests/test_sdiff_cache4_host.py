@@ -62,12 +62,12 @@ def test_cache_entries_refuse():
         assert append(**kw) == _lib.TDA_ERR_INVALID, kw
 
     def attend(map=0, q=16, dtype=_lib.TDA_BF16, B=1, H=2, Hkv=1, D=64, table=16, stride=4, width=4, lens=16, scale=0.1,
-               power=2.0, out=16):
+               power=2.0, out=16, status=16):
         return lib.tda_cache4_attention(map, q, 16, dtype, None, out, B, H, Hkv, D, 16, 4, 16, table, stride, width, lens,
-                                        None, 0, 0, 0, 0.5, scale, 1.0, power, 0, None, 0, None)
+                                        None, 0, 0, 0, 0.5, scale, 1.0, power, 0, None, 0, status, None)
     assert attend(dtype=_lib.TDA_F32) == _lib.TDA_ERR_UNSUPPORTED and attend(D=32) == _lib.TDA_ERR_UNSUPPORTED
     for kw in (dict(map=2), dict(q=None), dict(q=4), dict(out=None), dict(B=0), dict(B=70000), dict(H=3, Hkv=2), dict(table=None),
-               dict(stride=2), dict(width=0), dict(lens=None), dict(scale=-1.0), dict(map=1, power=float("nan")),
+               dict(stride=2), dict(width=0), dict(lens=None), dict(status=None), dict(scale=-1.0), dict(map=1, power=float("nan")),
                dict(width=1 << 28, stride=1 << 28)):
         assert attend(**kw) == _lib.TDA_ERR_INVALID, kw
     assert attend(width=1 << 12, stride=1 << 12) == _lib.TDA_ERR_WORKSPACE
