@@ -13,6 +13,7 @@ bits an element).  There is no CPU fallback.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -20,7 +21,7 @@ import torch
 
 from . import _lib
 from . import ops as _ops
-from .sdiff import _CODE, _on, _stream, lambda_ref, strides_of, view_of
+from .sdiff import _CODE, lambda_ref, launch, strides_of, view_of
 
 PAGE_SIZES = (16, 32, 64, 128)
 
@@ -50,10 +51,7 @@ class Cache4:
         self.normalize_keys = bool(normalize_keys)
         block = _lib.load().tda_cache4_block_bytes(page_size, head_dim)
         self.data = torch.zeros((num_pages, num_kv_heads, block), dtype=torch.uint8, device=device)
-
-    @property
-    def device(self):
-        return self.data.device
+        self.device = self.data.device
 
 
 class PagePlan(NamedTuple):
@@ -75,7 +73,7 @@ def _ints(what, name, t, shape, device):
         raise TypeError(f"{what}: {name} must be an int32 tensor")
     if t.device != device:
         raise RuntimeError(f"{what}: {name} must be on {device}")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what}: {name} must have shape {shape}, got {tuple(t.shape)}")
 
 
@@ -125,14 +123,10 @@ def plan_pages(lengths, new_tokens, block_table, free_pages, free_head, page_siz
     # one allocation: its parts are views
     buf = torch.empty(3 * rows + 2 * B + 3, dtype=torch.int32, device=dev)
     at = buf.data_ptr()
-    lib = _lib.load()
-    with _on(dev):
-        rc = lib.tda_plan_pages(lengths.data_ptr(), new_tokens.data_ptr(), B, block_table.data_ptr(), stride,
-                                block_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_head.data_ptr(),
-                                page_size, rows, at, at + 4 * rows, at + 8 * rows, at + 12 * rows,
-                                at + 4 * (3 * rows + B + 1), at + 4 * (3 * rows + 2 * B + 1),
-                                at + 4 * (3 * rows + 2 * B + 2), _stream(dev))
-    _lib.check(rc)
+    launch(_lib.load().tda_plan_pages, dev, lengths.data_ptr(), new_tokens.data_ptr(), B, block_table.data_ptr(),
+           stride, block_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_head.data_ptr(), page_size,
+           rows, at, at + 4 * rows, at + 8 * rows, at + 12 * rows, at + 4 * (3 * rows + B + 1),
+           at + 4 * (3 * rows + 2 * B + 1), at + 4 * (3 * rows + 2 * B + 2))
     return PagePlan(*buf.split((rows, rows, rows, B + 1, B, 1, 1)))
 
 
@@ -152,7 +146,7 @@ def cache4_append(cache: Cache4, k1, k2, v, slots) -> None:
     shape = (slots.shape[0], cache.num_kv_heads, cache.head_dim)
     for t in (k1, k2, v):
         _cuda(what, t)
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{what}: k1, k2 and v must have shape {shape}, got {tuple(t.shape)}")
         if t.device != cache.device:
             raise RuntimeError(f"{what}: inputs must be on the cache's device")
@@ -161,12 +155,9 @@ def cache4_append(cache: Cache4, k1, k2, v, slots) -> None:
     if slots.shape[0] == 0:
         return
     ts = [view_of(t, t.dtype) for t in (k1, k2, v)]
-    with _on(cache.device):
-        rc = _lib.load().tda_cache4_append(*[t.data_ptr() for t in ts], _CODE[k1.dtype], strides_of(ts),
-                                           slots.data_ptr(), shape[0], cache.data.data_ptr(), cache.num_pages,
-                                           cache.num_kv_heads, cache.head_dim, cache.page_size,
-                                           int(cache.normalize_keys), _stream(cache.device))
-    _lib.check(rc)
+    launch(_lib.load().tda_cache4_append, cache.device, *[t.data_ptr() for t in ts], _CODE[k1.dtype], strides_of(ts),
+           slots.data_ptr(), shape[0], cache.data.data_ptr(), cache.num_pages, cache.num_kv_heads, cache.head_dim,
+           cache.page_size, int(cache.normalize_keys))
 
 
 def cache4_read(cache: Cache4, slots, dtype=torch.bfloat16):
@@ -177,15 +168,17 @@ def cache4_read(cache: Cache4, slots, dtype=torch.bfloat16):
     if dtype not in _CODE:
         raise TypeError(f"{what}: dtype must be bf16, fp16 or fp32, got {dtype}")
     shape = (slots.shape[0], cache.num_kv_heads, cache.head_dim)
-    out = tuple(torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(3))
+    out = torch.empty((3, *shape), dtype=dtype, device=cache.device).unbind(0)
     if slots.shape[0] == 0:
         return out
-    with _on(cache.device):
-        rc = _lib.load().tda_cache4_read(cache.data.data_ptr(), cache.num_pages, cache.num_kv_heads, cache.head_dim,
-                                         cache.page_size, slots.data_ptr(), shape[0], *[t.data_ptr() for t in out],
-                                         _CODE[dtype], _stream(cache.device))
-    _lib.check(rc)
+    launch(_lib.load().tda_cache4_read, cache.device, cache.data.data_ptr(), cache.num_pages, cache.num_kv_heads,
+           cache.head_dim, cache.page_size, slots.data_ptr(), shape[0], *[t.data_ptr() for t in out], _CODE[dtype])
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_size(*sizes) -> int:
+    return _lib.load().tda_cache4_workspace_size(*sizes)
 
 
 def _attend(what, kind, q1, q2, cache, block_table, lengths, lambda_param, scale, beta, relu_power):
@@ -210,20 +203,14 @@ def _attend(what, kind, q1, q2, cache, block_table, lengths, lambda_param, scale
     lengths = lengths.contiguous()
     ts = [view_of(q1, q1.dtype), view_of(q2, q2.dtype)]
     lp, lc, lsb, lsh, lv, keep = lambda_ref(lambda_param, B, H, dev, what)
-    lib = _lib.load()
     width = block_table.shape[1]
-    ws_n = lib.tda_cache4_workspace_size(kind, B, H, cache.num_kv_heads, D, cache.page_size, width)
+    ws_n = _workspace_size(kind, B, H, cache.num_kv_heads, D, cache.page_size, width)
     ws = torch.empty(ws_n, dtype=torch.uint8, device=dev) if ws_n else None
-    with _on(dev):
-        rc = lib.tda_cache4_attention(kind, ts[0].data_ptr(), ts[1].data_ptr(), _CODE[q1.dtype], strides_of(ts),
-                                      out.data_ptr(), B, H, cache.num_kv_heads, D, cache.data.data_ptr(),
-                                      cache.num_pages, cache.page_size, block_table.data_ptr(), stride, width,
-                                      lengths.data_ptr(), lp, lc, lsb, lsh, lv, scale, beta, relu_power,
-                                      int(cache.normalize_keys), None if ws is None else ws.data_ptr(), ws_n,
-                                      _ops._status_word(dev).data_ptr(), _stream(dev))
-    _lib.check(rc)
-    if _ops._SYNC_CHECK:
-        _ops.check_status(dev)
+    launch(_lib.load().tda_cache4_attention, dev, kind, ts[0].data_ptr(), ts[1].data_ptr(), _CODE[q1.dtype],
+           strides_of(ts), out.data_ptr(), B, H, cache.num_kv_heads, D, cache.data.data_ptr(), cache.num_pages,
+           cache.page_size, block_table.data_ptr(), stride, width, lengths.data_ptr(), lp, lc, lsb, lsh, lv, scale,
+           beta, relu_power, int(cache.normalize_keys), None if ws is None else ws.data_ptr(), ws_n,
+           _ops._status_word(dev).data_ptr())
     return out
 
 

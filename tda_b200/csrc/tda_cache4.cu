@@ -176,9 +176,37 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
 
 // byte offset of the slab that holds a slot's rows of one head
 template <int D>
-__device__ __forceinline__ size_t slab_of(int slot, int h, int heads, int page) {
-  return (static_cast<size_t>(slot / page) * heads + h) * cache4_block_bytes(page, D) +
-         static_cast<size_t>(slot % page / kSlab4) * cache4_slab_bytes(D);
+__device__ __forceinline__ size_t slab_of(int slot, int h, int heads, int page_log2) {
+  const int page = 1 << page_log2;
+  return (static_cast<size_t>(slot >> page_log2) * heads + h) * cache4_block_bytes(page, D) +
+         static_cast<size_t>((slot & (page - 1)) / kSlab4) * cache4_slab_bytes(D);
+}
+
+// Both row kernels: a thread takes one 32-bit word of codes (8 elements, two
+// runs of 4) of a token, so D / 8 neighbouring threads take a row; a block
+// takes kPass rows at a time of one head and tensor, kUnroll passes with all
+// loads in front.
+constexpr int kRowThreads = 256;
+template <int D>
+struct RC {
+  static constexpr int kPer = D / 8;
+  static constexpr int kPass = kRowThreads / kPer;
+  static constexpr int kUnroll = 2;
+  static constexpr int kRows = kPass * kUnroll;  // tokens of a block
+};
+
+// word e of a row: its lane in fragment order, word index and the dims of its two runs
+template <bool V>
+__device__ __forceinline__ void word_of(int e, int& lane, int& w, int& d0, int& d1) {
+  w = V ? e / 8 : e / 4;
+  lane = V ? e % 8 : e % 4;
+  d0 = V ? 64 * w + 4 * lane : 32 * w + 4 * lane;
+  d1 = V ? d0 + 32 : d0 + 16;
+}
+// nibble of element j of run r
+template <bool V>
+__device__ __forceinline__ constexpr int nibble_of(int r, int j) {
+  return V ? 4 * r + j : (2 * r + (j >> 1)) + 4 * (j & 1);
 }
 
 // ================================================================== append
@@ -187,10 +215,10 @@ struct AppendParams {
   long long st[3], sh[3];
   const int* slots;
   uint8_t* cache;
-  long long num_slots;
-  long long tokens;
+  int num_slots;
+  int tokens;
   int heads;
-  int page;
+  int page_log2;
   int normalize;
 };
 
@@ -232,101 +260,112 @@ struct Elem<__half> {
   }
 };
 
-// round-half-even of 7 |x| / amax without a division: t is within 2^-20 of the
-// quotient, and the choice between its floor f and f + 1 compares 14 |x| with
-// (2 f + 1) amax, both exact in fp32 for bf16 and fp16 inputs.  A floor that t
-// got wrong by one (a quotient at a whole number) ends at the same code.
-__device__ __forceinline__ int code_of(float x, float amax, float inv7) {
+// round-half-even of 7 x / amax without a division.  c, the nearest whole number
+// to an approximate quotient, is right or one off; the remainder 14 |x| - 2 c amax
+// is exact in fp32 for bf16 and fp16 inputs and says which: past amax the
+// neighbour is nearer, and at amax (a tie) it is taken when c is odd.
+__device__ __forceinline__ uint32_t code_of(float x, float amax, float inv7) {
   const float ax = fabsf(x);
-  const int f = min(7, static_cast<int>(ax * inv7));
-  const float d = fmaf(-static_cast<float>(2 * f + 1), amax, 14.0f * ax);
-  const int c = f + ((d > 0.0f || (d == 0.0f && (f & 1))) ? 1 : 0);
-  return x < 0.0f ? 8 - c : 8 + c;
+  const float shifted = fmaf(ax, inv7, 12582912.0f);  // 1.5 2^23: the sum's last bits are c
+  const uint32_t c = __float_as_uint(shifted) & 7u;
+  const float rem = fmaf(-2.0f * (shifted - 12582912.0f), amax, 14.0f * ax);
+  const float edge = __uint_as_float(__float_as_uint(amax) - (c & 1u));
+  const uint32_t up = fabsf(rem) > edge ? (rem > 0.0f ? 1u : 0xffffffffu) : 0u;
+  const uint32_t m = c + up;
+  return x < 0.0f ? 8u - m : 8u + m;
 }
 
 __device__ __forceinline__ uint32_t max_bits(uint32_t a, float x) { return max(a, __float_as_uint(x) & 0x7fffffffu); }
 
-// A thread makes one 32-bit word of codes from 8 elements (two runs of 4), so
-// D / 8 neighbouring threads make a row; bound by the 2 bytes an element read.
-template <int D, typename T>
-__global__ void __launch_bounds__(256) cache4_append_kernel(const AppendParams p) {
-  constexpr int kPer = D / 8;
-  const long long rows = p.tokens * p.heads;
-  const int xi = blockIdx.y;  // tensor
-  const long long idx = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const long long row = idx / kPer;
-  const int e = static_cast<int>(idx % kPer);
-  const bool in = row < rows;
-  const long long tok = in ? row / p.heads : 0;
-  const int h = in ? static_cast<int>(row % p.heads) : 0;
-  const int slot = in ? p.slots[tok] : -1;
-  const bool live = slot >= 0 && slot < p.num_slots;
-  const bool is_v = xi == 2;
-  // K: word w of lane t; V: word u of lane g
-  const int w = is_v ? e / 8 : e / 4, l = is_v ? e % 8 : e % 4;
-  const int d0 = is_v ? 64 * w + 4 * l : 32 * w + 4 * l;
-  const int d1 = is_v ? d0 + 32 : d0 + 16;
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (live) {
-    const T* src = static_cast<const T*>(p.x[xi]) + tok * p.st[xi] + h * p.sh[xi];
-    Elem<T>::load4(src + d0, x, 0);
-    Elem<T>::load4(src + d1, x, 4);
-  }
+// one word of codes and the scales of its runs' groups from 8 elements
+template <int D, bool V>
+__device__ __forceinline__ uint32_t quantise(const float (&x)[8], bool normalize, float (&sc)[2]) {
   // largest magnitude of each run's group, as bits so that a NaN wins
-  uint32_t m0 = 0, m1 = 0;
+  uint32_t m[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    m0 = max_bits(m0, x[i]);
-    m1 = max_bits(m1, x[4 + i]);
+  for (int i = 0; i < 8; ++i) m[i >> 2] = max_bits(m[i >> 2], x[i]);
+  if (!V) m[0] = m[1] = max(m[0], m[1]);
+#pragma unroll
+  for (int o = 1; o < (V ? 8 : 4); o <<= 1) {
+    m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
+    if (V) m[1] = max(m[1], __shfl_xor_sync(0xffffffffu, m[1], o));
   }
-  if (!is_v) m0 = m1 = max(m0, m1);
-  for (int o = 1; o < (is_v ? 8 : 4); o <<= 1) {
-    m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-    m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-  }
+  if (!V) m[1] = m[0];
   float inv_norm = 1.0f;
-  if (p.normalize && !is_v) {
+  if (normalize && !V) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-    for (int o = 1; o < kPer; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    for (int o = 1; o < RC<D>::kPer; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     inv_norm = 1.0f / fmaxf(sqrtf(ss), 1e-12f);
   }
-  if (!live) return;
   uint32_t word = 0;
-  float sc[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    float amax = __uint_as_float(r ? m1 : m0);
-    const bool finite = (r ? m1 : m0) < 0x7f800000u;
+    float amax = __uint_as_float(m[r]);
+    const bool finite = m[r] < 0x7f800000u;
     sc[r] = finite ? amax / 7.0f * inv_norm : __uint_as_float(0x7fc00000u);
     // far from the ends of the exponent's range, so that neither 7 / amax nor 14 x leaves it
     const float lift = amax < 1e-18f ? 0x1p80f : (amax > 1e18f ? 0x1p-80f : 1.0f);
     amax *= lift;
-    const float inv7 = amax > 0.0f ? __fdividef(7.0f, amax) : 0.0f;
+    const bool any = finite && amax > 0.0f;
+    const float inv7 = __fdividef(7.0f, amax);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = (finite && amax > 0.0f) ? code_of(x[4 * r + j] * lift, amax, inv7) : 8;
-      // K: half r, register 2 r + j / 2, low or high half j % 2; V: run r, element j
-      const int nib = is_v ? 4 * r + j : (2 * r + (j >> 1)) + 4 * (j & 1);
-      word |= static_cast<uint32_t>(c) << (4 * nib);
-    }
+    for (int j = 0; j < 4; ++j)
+      word |= (any ? code_of(x[4 * r + j] * lift, amax, inv7) : 8u) << (4 * nibble_of<V>(r, j));
   }
-  uint8_t* slab = p.cache + slab_of<D>(slot, h, p.heads, p.page);
-  const int r = slot % kSlab4;
-  *reinterpret_cast<uint32_t*>(slab + cache4_codes_at(xi, D) + (is_v ? cache4_v_word(r, l, w, D) : cache4_k_word(r, l, w, D))) = word;
-  if (l == 0) {
-    __nv_bfloat16* s = reinterpret_cast<__nv_bfloat16*>(slab + cache4_scales_at(xi, D) + r * cache4_scale_bytes(D));
-    if (is_v) {
-      s[2 * w] = __float2bfloat16_rn(sc[0]);
-      s[2 * w + 1] = __float2bfloat16_rn(sc[1]);
+  return word;
+}
+
+template <int D, typename T, bool V>
+__device__ __forceinline__ void append_rows(const AppendParams& p, const T* x, long long st, long long sh, int tensor, int h) {
+  using C = RC<D>;
+  int lane, w, d0, d1;
+  word_of<V>(threadIdx.x % C::kPer, lane, w, d0, d1);
+  const int t0 = blockIdx.x * C::kRows + threadIdx.x / C::kPer;
+  float v[C::kUnroll][8];
+  int slot[C::kUnroll];
+#pragma unroll
+  for (int u = 0; u < C::kUnroll; ++u) {
+    const int t = t0 + u * C::kPass;
+    slot[u] = t < p.tokens ? p.slots[t] : -1;
+    if (t < p.tokens) {
+      const T* src = x + t * st + h * sh;
+      Elem<T>::load4(src + d0, v[u], 0);
+      Elem<T>::load4(src + d1, v[u], 4);
     } else {
-      s[w] = __float2bfloat16_rn(sc[0]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
     }
   }
+#pragma unroll
+  for (int u = 0; u < C::kUnroll; ++u) {
+    float sc[2];
+    const uint32_t word = quantise<D, V>(v[u], p.normalize != 0, sc);
+    if (static_cast<unsigned>(slot[u]) >= static_cast<unsigned>(p.num_slots)) continue;
+    uint8_t* slab = p.cache + slab_of<D>(slot[u], h, p.heads, p.page_log2);
+    const int r = slot[u] % kSlab4;
+    *reinterpret_cast<uint32_t*>(slab + cache4_codes_at(tensor, D) + (V ? cache4_v_word(r, lane, w, D) : cache4_k_word(r, lane, w, D))) = word;
+    if (lane == 0) {
+      __nv_bfloat16* s = reinterpret_cast<__nv_bfloat16*>(slab + cache4_scales_at(tensor, D) + r * cache4_scale_bytes(D));
+      if (V)
+        *reinterpret_cast<__nv_bfloat162*>(s + 2 * w) = __floats2bfloat162_rn(sc[0], sc[1]);
+      else
+        s[w] = __float2bfloat16_rn(sc[0]);
+    }
+  }
+}
+
+// grid (token blocks, heads, tensors)
+template <int D, typename T>
+__global__ void __launch_bounds__(kRowThreads) cache4_append_kernel(const __grid_constant__ AppendParams p) {
+  if (blockIdx.z == 0)
+    append_rows<D, T, false>(p, static_cast<const T*>(p.x[0]), p.st[0], p.sh[0], 0, blockIdx.y);
+  else if (blockIdx.z == 1)
+    append_rows<D, T, false>(p, static_cast<const T*>(p.x[1]), p.st[1], p.sh[1], 1, blockIdx.y);
+  else
+    append_rows<D, T, true>(p, static_cast<const T*>(p.x[2]), p.st[2], p.sh[2], 2, blockIdx.y);
 }
 
 // ================================================================== read
@@ -334,56 +373,67 @@ struct ReadParams {
   const uint8_t* cache;
   const int* slots;
   void* y[3];
-  long long num_slots;
-  long long tokens;
+  int num_slots;
+  int tokens;
   int heads;
-  int page;
+  int page_log2;
 };
 
-template <int D, typename T>
-__global__ void __launch_bounds__(256) cache4_read_kernel(const ReadParams p) {
-  constexpr int kPer = D / 8;
-  const int xi = blockIdx.y;
-  const long long idx = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const long long row = idx / kPer;
-  if (row >= p.tokens * p.heads) return;
-  const int e = static_cast<int>(idx % kPer);
-  const long long tok = row / p.heads;
-  const int h = static_cast<int>(row % p.heads);
-  const int slot = p.slots[tok];
-  const bool is_v = xi == 2;
-  const int w = is_v ? e / 8 : e / 4, l = is_v ? e % 8 : e % 4;
-  const int d0 = is_v ? 64 * w + 4 * l : 32 * w + 4 * l;
-  const int d1 = is_v ? d0 + 32 : d0 + 16;
-  float x[8];
+template <int D, typename T, bool V>
+__device__ __forceinline__ void read_rows(const ReadParams& p, T* y, int tensor, int h) {
+  using C = RC<D>;
+  int lane, w, d0, d1;
+  word_of<V>(threadIdx.x % C::kPer, lane, w, d0, d1);
+  const int t0 = blockIdx.x * C::kRows + threadIdx.x / C::kPer;
+  uint32_t word[C::kUnroll];
+  float s[C::kUnroll][2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (slot >= 0 && slot < p.num_slots) {
-    const uint8_t* slab = p.cache + slab_of<D>(slot, h, p.heads, p.page);
-    const int rr = slot % kSlab4;
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(
-        slab + cache4_codes_at(xi, D) + (is_v ? cache4_v_word(rr, l, w, D) : cache4_k_word(rr, l, w, D)));
-    const __nv_bfloat16* s = reinterpret_cast<const __nv_bfloat16*>(slab + cache4_scales_at(xi, D) + rr * cache4_scale_bytes(D));
-    const float s0 = __bfloat162float(s[is_v ? 2 * w : w]), s1 = __bfloat162float(s[is_v ? 2 * w + 1 : w]);
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int nib = is_v ? 4 * r + j : (2 * r + (j >> 1)) + 4 * (j & 1);
-        x[4 * r + j] = static_cast<float>(static_cast<int>((word >> (4 * nib)) & 15u) - 8) * (r ? s1 : s0);
-      }
+  for (int u = 0; u < C::kUnroll; ++u) {
+    const int t = t0 + u * C::kPass;
+    const int slot = t < p.tokens ? p.slots[t] : -1;
+    word[u] = 0x88888888u;
+    s[u][0] = s[u][1] = 0.f;
+    if (static_cast<unsigned>(slot) < static_cast<unsigned>(p.num_slots)) {
+      const uint8_t* slab = p.cache + slab_of<D>(slot, h, p.heads, p.page_log2);
+      const int r = slot % kSlab4;
+      word[u] = *reinterpret_cast<const uint32_t*>(slab + cache4_codes_at(tensor, D) +
+                                                   (V ? cache4_v_word(r, lane, w, D) : cache4_k_word(r, lane, w, D)));
+      const __nv_bfloat16* sp = reinterpret_cast<const __nv_bfloat16*>(slab + cache4_scales_at(tensor, D) + r * cache4_scale_bytes(D));
+      s[u][0] = __bfloat162float(sp[V ? 2 * w : w]);
+      s[u][1] = V ? __bfloat162float(sp[2 * w + 1]) : s[u][0];
+    }
   }
-  T* y = static_cast<T*>(p.y[xi]) + row * D;
-  Elem<T>::store4(y + d0, x);
-  Elem<T>::store4(y + d1, x + 4);
+#pragma unroll
+  for (int u = 0; u < C::kUnroll; ++u) {
+    const int t = t0 + u * C::kPass;
+    if (t >= p.tokens) continue;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)  // 2^23 + n - (2^23 + 8)
+      x[i] = (__uint_as_float(((word[u] >> (4 * nibble_of<V>(i >> 2, i & 3))) & 15u) | 0x4b000000u) - 8388616.0f) * s[u][i >> 2];
+    T* row = y + (static_cast<long long>(t) * p.heads + h) * D;
+    Elem<T>::store4(row + d0, x);
+    Elem<T>::store4(row + d1, x + 4);
+  }
 }
 
-template <typename P, typename K>
-cudaError_t launch_rows(K kernel, const P& p, long long tokens, int heads, int D, cudaStream_t s) {
-  const long long blocks = ceil_div(tokens * heads * (D / 8), 256);
-  kernel<<<dim3(static_cast<unsigned>(blocks), 3), 256, 0, s>>>(p);
+template <int D, typename T>
+__global__ void __launch_bounds__(kRowThreads) cache4_read_kernel(const __grid_constant__ ReadParams p) {
+  if (blockIdx.z == 0)
+    read_rows<D, T, false>(p, static_cast<T*>(p.y[0]), 0, blockIdx.y);
+  else if (blockIdx.z == 1)
+    read_rows<D, T, false>(p, static_cast<T*>(p.y[1]), 1, blockIdx.y);
+  else
+    read_rows<D, T, true>(p, static_cast<T*>(p.y[2]), 2, blockIdx.y);
+}
+
+template <int D, typename P, typename K>
+cudaError_t launch_rows(K kernel, const P& p, cudaStream_t s) {
+  kernel<<<dim3(static_cast<unsigned>(ceil_div(p.tokens, RC<D>::kRows)), p.heads, 3), kRowThreads, 0, s>>>(p);
   return cudaGetLastError();
 }
+
+int log2_page(int64_t page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
 
 int check_cache(const void* cache, int64_t num_pages, int64_t heads, int64_t D, int64_t page) {
   if (D != 64 && D != 128) return fail(TDA_ERR_UNSUPPORTED, "the 4-bit cache needs head_dim 64 or 128 (got %lld)", static_cast<long long>(D));
@@ -395,9 +445,9 @@ int check_cache(const void* cache, int64_t num_pages, int64_t heads, int64_t D, 
   return TDA_OK;
 }
 
-int check_rows(int64_t tokens, int64_t heads, int64_t D) {
-  if (tokens < 1) return fail(TDA_ERR_INVALID, "tokens must be >= 1");
-  if (tokens > 0x7fffffffll * 256 / (heads * (D / 8))) return fail(TDA_ERR_INVALID, "tokens * heads exceed the grid limit");
+int check_rows(int64_t tokens, int64_t heads) {
+  if (tokens < 1 || tokens > 0x7fffffffll - 1024) return fail(TDA_ERR_INVALID, "tokens must be in [1, 2^31 - 1024)");
+  if (heads > 65535) return fail(TDA_ERR_INVALID, "too many kv heads");
   return TDA_OK;
 }
 
@@ -463,7 +513,7 @@ int tda_cache4_append(const void* k1, const void* k2, const void* v, int dtype, 
                       const int32_t* slots, int64_t tokens, void* cache, int64_t num_pages, int64_t kv_heads,
                       int64_t head_dim, int64_t page_size, int normalize_keys, void* stream) {
   if (int e = check_cache(cache, num_pages, kv_heads, head_dim, page_size)) return e;
-  if (int e = check_rows(tokens, kv_heads, head_dim)) return e;
+  if (int e = check_rows(tokens, kv_heads)) return e;
   if (!slots || !aligned(slots, 4)) return fail(TDA_ERR_INVALID, "slots must be non-NULL int32");
   AppendParams p;
   const void* xs[3] = {k1, k2, v};
@@ -477,16 +527,16 @@ int tda_cache4_append(const void* k1, const void* k2, const void* v, int dtype, 
   }
   p.slots = slots;
   p.cache = static_cast<uint8_t*>(cache);
-  p.num_slots = num_pages * page_size;
-  p.tokens = tokens;
+  p.num_slots = static_cast<int>(num_pages * page_size);
+  p.tokens = static_cast<int>(tokens);
   p.heads = static_cast<int>(kv_heads);
-  p.page = static_cast<int>(page_size);
+  p.page_log2 = log2_page(page_size);
   p.normalize = normalize_keys != 0;
   const int D = static_cast<int>(head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-#define TDA_APPEND(T) (D == 64 ? launch_rows(cache4_append_kernel<64, T>, p, tokens, p.heads, D, s) \
-                               : launch_rows(cache4_append_kernel<128, T>, p, tokens, p.heads, D, s))
+#define TDA_APPEND(T) (D == 64 ? launch_rows<64>(cache4_append_kernel<64, T>, p, s) \
+                               : launch_rows<128>(cache4_append_kernel<128, T>, p, s))
   if (dtype == TDA_BF16)
     e = TDA_APPEND(__nv_bfloat16);
   else if (dtype == TDA_F16)
@@ -502,7 +552,7 @@ int tda_cache4_append(const void* k1, const void* k2, const void* v, int dtype, 
 int tda_cache4_read(const void* cache, int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size,
                     const int32_t* slots, int64_t tokens, void* k1, void* k2, void* v, int dtype, void* stream) {
   if (int e = check_cache(cache, num_pages, kv_heads, head_dim, page_size)) return e;
-  if (int e = check_rows(tokens, kv_heads, head_dim)) return e;
+  if (int e = check_rows(tokens, kv_heads)) return e;
   if (!slots || !aligned(slots, 4)) return fail(TDA_ERR_INVALID, "slots must be non-NULL int32");
   ReadParams p;
   void* ys[3] = {k1, k2, v};
@@ -512,15 +562,15 @@ int tda_cache4_read(const void* cache, int64_t num_pages, int64_t kv_heads, int6
   }
   p.cache = static_cast<const uint8_t*>(cache);
   p.slots = slots;
-  p.num_slots = num_pages * page_size;
-  p.tokens = tokens;
+  p.num_slots = static_cast<int>(num_pages * page_size);
+  p.tokens = static_cast<int>(tokens);
   p.heads = static_cast<int>(kv_heads);
-  p.page = static_cast<int>(page_size);
+  p.page_log2 = log2_page(page_size);
   const int D = static_cast<int>(head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-#define TDA_READ(T) (D == 64 ? launch_rows(cache4_read_kernel<64, T>, p, tokens, p.heads, D, s) \
-                             : launch_rows(cache4_read_kernel<128, T>, p, tokens, p.heads, D, s))
+#define TDA_READ(T) (D == 64 ? launch_rows<64>(cache4_read_kernel<64, T>, p, s) \
+                             : launch_rows<128>(cache4_read_kernel<128, T>, p, s))
   if (dtype == TDA_BF16)
     e = TDA_READ(__nv_bfloat16);
   else if (dtype == TDA_F16)

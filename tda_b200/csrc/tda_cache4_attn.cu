@@ -68,10 +68,10 @@ struct AttnParams {
   void* out;
   float* part;  // [b][head][chunk][kPart]
   long long table_stride;
-  long long num_pages;
   LambdaRef lam;
   int* status;
   unsigned long long timeout_ns;
+  int num_pages;
   int width;
   int page_log2;
   int B;
@@ -99,6 +99,21 @@ __device__ __forceinline__ uint32_t movm(uint32_t x) {
   return y;
 }
 
+// d = a b + {c0, c1, c0, c1}
+__device__ __forceinline__ void mma16816_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                              float c0, float c1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -106,17 +121,29 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// two nibbles as 1024 + n, and two more as 1024 + 16 n
-__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) { return (w & 0x000f000fu) | 0x64006400u; }
-__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) { return (w & 0x00f000f0u) | 0x64006400u; }
+// Two nibbles as 1024 + n, and two more as 1024 + 16 n: (w & mask) | 0x6400 twice
+// is one three-input operation, which takes one constant as an immediate; the
+// other one comes from a register that the compiler may not fold back.
+struct Magic {
+  uint32_t base;
+  __device__ __forceinline__ Magic() { asm volatile("mov.b32 %0, 0x64006400;" : "=r"(base)); }
+  template <uint32_t kMask>
+  __device__ __forceinline__ uint32_t take(uint32_t w) const {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(kMask), "r"(base));
+    return r;
+  }
+  __device__ __forceinline__ uint32_t low(uint32_t w) const { return take<0x000f000fu>(w); }
+  __device__ __forceinline__ uint32_t high(uint32_t w) const { return take<0x00f000f0u>(w); }
+};
 __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 // codes -7..7, and 16 times them
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return sub_f16x2(low_nibbles(w), 0x64086408u); }    // 1032
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return sub_f16x2(high_nibbles(w), 0x64806480u); }  // 1152
+__device__ __forceinline__ uint32_t low_codes(const Magic& m, uint32_t w) { return sub_f16x2(m.low(w), 0x64086408u); }    // 1032
+__device__ __forceinline__ uint32_t high_codes(const Magic& m, uint32_t w) { return sub_f16x2(m.high(w), 0x64806480u); }  // 1152
 
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
@@ -195,18 +222,20 @@ __global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __gri
   auto token = [&](int i) { return lo + 16 * (i * kWarps + warp); };
   auto page_of = [&](int i) { return i < n ? __ldg(row + (token(i) >> p.page_log2)) : -1; };
   uint32_t in_cache = 0;  // bit i % 32: slab i's page lies in the cache
+  const size_t page_bytes = p.kv_heads * cache4_block_bytes(page_mask + 1, D);
+  const uint8_t* head_base = p.cache + kvh * cache4_block_bytes(page_mask + 1, D);
   auto fetch = [&](int i, int pg) {
-    const bool good = pg >= 0 && pg < p.num_pages;
+    const bool good = static_cast<unsigned>(pg) < static_cast<unsigned>(p.num_pages);
     in_cache = (in_cache & ~(1u << (i & 31))) | (static_cast<uint32_t>(good) << (i & 31));
-    if (good && lane == 0) {
+    if (lane == 0) {
       uint64_t* bar = &full[warp][i % S];
-      mbar_arrive_expect_tx(bar, C::kSlabBytes);
-      bulk_load(ring + (i % S) * C::kSlabBytes,
-                p.cache + (static_cast<size_t>(pg) * p.kv_heads + kvh) * cache4_block_bytes(page_mask + 1, D) +
-                    static_cast<size_t>((token(i) & page_mask) >> 4) * C::kSlabBytes,
-                C::kSlabBytes, bar);
-    } else if (lane == 0 && i < n) {
-      mbar_arrive(&full[warp][i % S]);  // nothing to copy: the phase completes all the same
+      if (good) {
+        mbar_arrive_expect_tx(bar, C::kSlabBytes);
+        bulk_load(ring + (i % S) * C::kSlabBytes, head_base + pg * page_bytes + ((token(i) & page_mask) >> 4) * C::kSlabBytes,
+                  C::kSlabBytes, bar);
+      } else {
+        mbar_arrive(bar);  // nothing to copy: the phase completes all the same
+      }
     }
   };
   {
@@ -284,7 +313,10 @@ __global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __gri
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-kInf, -kInf}, l[2] = {0.f, 0.f};  // M and the sum of 2^(score - M), per column
+  uint32_t bound = 0u;                                 // the largest scale so far, twice
+  float limit[2] = {THR ? 0.f : -kInf, THR ? 0.f : -kInf}, down[2] = {1.f, 1.f};
 
+  const Magic mg;
   bool ok = true;
   int i = 0;
   for (; i < n; ++i) {
@@ -311,13 +343,16 @@ __global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __gri
       }
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        float acc[4] = {off[w][0], off[w][1], off[w][0], off[w][1]};
+        float acc[4];
 #pragma unroll
         for (int mp = 0; mp < 2; ++mp) {
           const uint32_t x = k[mp][0][w], y = k[mp][1][w], x8 = x >> 8, y8 = y >> 8;
           const uint32_t(&q)[2 * W][2] = mp ? q2 : q1;
-          mma16816(acc, low_nibbles(x), low_nibbles(y), high_nibbles(x), high_nibbles(y), q[2 * w][0], q[2 * w][1]);
-          mma16816(acc, low_nibbles(x8), low_nibbles(y8), high_nibbles(x8), high_nibbles(y8), q[2 * w + 1][0], q[2 * w + 1][1]);
+          if (mp == 0)
+            mma16816_from(acc, mg.low(x), mg.low(y), mg.high(x), mg.high(y), q[2 * w][0], q[2 * w][1], off[w][0], off[w][1]);
+          else
+            mma16816(acc, mg.low(x), mg.low(y), mg.high(x), mg.high(y), q[2 * w][0], q[2 * w][1]);
+          mma16816(acc, mg.low(x8), mg.low(y8), mg.high(x8), mg.high(y8), q[2 * w + 1][0], q[2 * w + 1][1]);
         }
         const float s0 = scale_of(ks[0], w), s1 = scale_of(ks[1], w);
         s[0] = fmaf(acc[0], s0, s[0]);
@@ -326,57 +361,58 @@ __global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __gri
         s[3] = fmaf(acc[3], s1, s[3]);
       }
     }
-    // rows past the length hold no token: their scales may be anything
-    const bool in0 = tok + g < hi, in1 = tok + g + 8 < hi;
-    float sv[2][W], svm[2];
+    if (tok + kSlab4 > hi) {  // rows past the length hold no token: their scales may be anything
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      svm[h] = 0.f;
+      for (int h = 0; h < 2; ++h) {
+        const bool in = tok + g + 8 * h < hi;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        sv[h][w] = (h ? in1 : in0) ? scale_of(vs[h], w) : 0.f;
-        svm[h] = fmaxf(svm[h], sv[h][w]);
+        for (int u = 0; u < D / 64; ++u) vs[h][u] = in ? vs[h][u] : 0u;
+        s[2 * h] = in ? s[2 * h] : -kInf;
+        s[2 * h + 1] = in ? s[2 * h + 1] : -kInf;
       }
-      svm[h] = fmaxf(svm[h], 0x1p-100f);
     }
+    uint32_t big = bound;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int u = 0; u < D / 64; ++u) big = max_bf16x2(big, vs[h][u]);
     float pr[4];
-    bool grow;
-    float top[2];  // log2 of the largest weights of the lane's columns
     if constexpr (THR) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const float z = fmaf(s[x], rq[x & 1], -tau);
-        pr[x] = (x < 2 ? in0 : in1) ? relu_pow<PM>(z, p.relu_power) : 0.f;
+        pr[x] = relu_pow<PM>(fmaf(s[x], rq[x & 1], -tau), p.relu_power);
         const float other = __shfl_xor_sync(0xffffffffu, pr[x], 2);  // the same head's other map
         pr[x] = second ? fmaf(-lam[x & 1], pr[x], other) : fmaf(-lam[x & 1], other, pr[x]);
       }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float y = fmaxf(fabsf(pr[c]) * svm[0], fabsf(pr[2 + c]) * svm[1]);
-        top[c] = y > 0.f ? fast_lg2(y) : -kInf;
-      }
-      if (!__any_sync(0xffffffffu, top[0] != -kInf || top[1] != -kInf || !(pr[0] + pr[1] + pr[2] + pr[3] == 0.f))) continue;
-    } else {
-      const float lg[2] = {fast_lg2(svm[0]), fast_lg2(svm[1])};
-#pragma unroll
-      for (int x = 0; x < 4; ++x) s[x] = (x < 2 ? in0 : in1) ? s[x] * rq[x & 1] : -kInf;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) top[c] = fmaxf(s[c] + lg[0], s[2 + c] + lg[1]);
+      if (!__any_sync(0xffffffffu, !(pr[0] == 0.f && pr[1] == 0.f && pr[2] == 0.f && pr[3] == 0.f))) continue;
     }
-    // M moves only when a weight passes it by 2^8: most slabs need neither the reduction nor the rescaling
-    grow = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f;
-    if (__any_sync(0xffffffffu, grow)) {
+    float top[2];  // largest score (threshold: weight) of the lane's columns
+#pragma unroll
+    for (int c = 0; c < 2; ++c) top[c] = THR ? fmaxf(fabsf(pr[c]), fabsf(pr[2 + c])) : fmaxf(s[c], s[2 + c]) * rq[c];
+    // M moves only when a weight passes it by 2^8: most slabs need neither the reductions nor the rescaling
+    if (__any_sync(0xffffffffu, top[0] > limit[0] || top[1] > limit[1] || big != bound)) {
+#pragma unroll
+      for (int y = 1; y < 32; y <<= 1) big = max_bf16x2(big, __shfl_xor_sync(0xffffffffu, big, y));
+      const float2 halves = unpack_bf16x2(big);
+      const float largest = fmaxf(halves.x, halves.y);
+      bound = pack_bf16x2(largest, largest);
+      const float lb = fast_lg2(fmaxf(largest, 0x1p-100f));
       float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float x = top[c];
 #pragma unroll
         for (int y = 4; y < 32; y <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, y));
-        if constexpr (THR) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));  // a head's two columns hold one weight
-        x = THR ? ceilf(fmaxf(x, m[c])) : fmaxf(x, m[c]);
+        if constexpr (THR) {
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));  // a head's two columns hold one weight
+          x = x > 0.f ? fast_lg2(x) : -kInf;
+        }
+        x = fmaxf(x + lb, m[c]);
         f[c] = m[c] == x ? 1.f : fast_ex2(m[c] - x);
         m[c] = x;
         l[c] *= f[c];
+        limit[c] = THR ? (x == -kInf ? 0.f : fast_ex2(x + 8.f - lb)) : x + 8.f - lb;
+        if constexpr (THR) down[c] = x == -kInf ? 1.f : fast_ex2(-x);
       }
 #pragma unroll
       for (int x = 0; x < D / 16; ++x)
@@ -385,17 +421,18 @@ __global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __gri
     }
     if constexpr (THR) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) pr[x] *= m[x & 1] == -kInf ? 1.f : fast_ex2(-m[x & 1]);
+      for (int x = 0; x < 4; ++x) pr[x] *= down[x & 1];
     } else {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) pr[x] = fast_ex2(s[x] - m[x & 1]);
+      for (int x = 0; x < 4; ++x) pr[x] = fast_ex2(fmaf(s[x], rq[x & 1], -m[x & 1]));
       l[0] += pr[0] + pr[2];
       l[1] += pr[1] + pr[3];
     }
     uint32_t bf[W][2];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float x0 = pr[0] * sv[0][w], x1 = pr[1] * sv[0][w], x2 = pr[2] * sv[1][w], x3 = pr[3] * sv[1][w];
+      const float s0 = scale_of(vs[0], w), s1 = scale_of(vs[1], w);
+      const float x0 = pr[0] * s0, x1 = pr[1] * s0, x2 = pr[2] * s1, x3 = pr[3] * s1;
       uint32_t r0 = pack_f16x2(x0, x1), r1 = pack_f16x2(x2, x3);
       if constexpr (THR) {
         if (second) {
@@ -425,8 +462,8 @@ __global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __gri
       for (int y = 0; y < 2; ++y) {  // nibbles 0-3, 4-7 of every word
         const uint32_t a = __byte_perm(v[0][u], v[1][u], y ? 0x7632 : 0x5410), c = __byte_perm(v[2][u], v[3][u], y ? 0x7632 : 0x5410);
         const int mt = 4 * u + 2 * y;
-        mma16816(o[mt], low_codes(a), high_codes(a), low_codes(c), high_codes(c), bf[mt >> 1][0], bf[mt >> 1][1]);
-        mma16816(o[mt + 1], low_codes(a >> 8), high_codes(a >> 8), low_codes(c >> 8), high_codes(c >> 8), bf[mt >> 1][0], bf[mt >> 1][1]);
+        mma16816(o[mt], low_codes(mg, a), high_codes(mg, a), low_codes(mg, c), high_codes(mg, c), bf[mt >> 1][0], bf[mt >> 1][1]);
+        mma16816(o[mt + 1], low_codes(mg, a >> 8), high_codes(mg, a >> 8), low_codes(mg, c >> 8), high_codes(mg, c >> 8), bf[mt >> 1][0], bf[mt >> 1][1]);
       }
   }
   if (!ok)
@@ -554,13 +591,13 @@ cudaError_t dispatch(const AttnParams& p, bool thr, cudaStream_t s) {
 }
 
 // Tokens a block takes: one wave of resident blocks (4 an SM) where the table's
-// width allows it, at least two slabs a warp, at most 1024 (uneven lengths then
+// width allows it, at least two slabs a warp, at most 2048 (uneven lengths then
 // still spread over the device).
 int64_t chunk_tokens(int64_t B, int64_t head_groups, int64_t max_len) {
   const int64_t want = 148 * 4 / (B * head_groups) + 1;  // chunks of one request
   int64_t chunk = ceil_div(ceil_div(max_len, want), 64) * 64;
   if (chunk < 128) chunk = 128;
-  if (chunk > 1024) chunk = 1024;
+  if (chunk > 2048) chunk = 2048;
   return chunk;
 }
 
@@ -621,7 +658,7 @@ int tda_cache4_attention(int map, const void* q1, const void* q2, int dtype, con
   p.lengths = lengths;
   p.out = out;
   p.table_stride = table_stride;
-  p.num_pages = num_pages;
+  p.num_pages = static_cast<int>(num_pages);
   p.width = static_cast<int>(table_width);
   p.page_log2 = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
   p.B = static_cast<int>(batch);

@@ -34,26 +34,41 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
 }
 
+// Operand descriptors differ in their address field alone (bytes / 16, and all of
+// shared memory fits the field): one 32-bit addition an operand keeps the single
+// issuing thread ahead of the tensor cores.
+__device__ __forceinline__ uint64_t desc_at(uint32_t lo, uint32_t hi, uint32_t bytes) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo + (bytes >> 4)), "r"(hi));
+  return d;
+}
+
 // D[dcol] = A B^T over D: A and B K-major tiles in shared memory
 template <int D, bool F16>
 __device__ __forceinline__ void mma_score(uint32_t dcol, uint32_t a, uint32_t b) {
   using G = Geo<D, F16>;
+  const uint64_t da = smem_desc_sw128(a, 16, 1024), db = smem_desc_sw128(b, 16, 1024);
+  const uint32_t hi = static_cast<uint32_t>(da >> 32), la = static_cast<uint32_t>(da), lb = static_cast<uint32_t>(db);
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
     const uint32_t off = (kk >> 2) * G::kBoxBytes + (kk & 3) * 32;
-    mma_ss(dcol, smem_desc_sw128(a + off, 16, 1024), smem_desc_sw128(b + off, 16, 1024), G::kIdescScore, kk > 0 ? 1u : 0u);
+    mma_ss(dcol, desc_at(la, hi, off), desc_at(lb, hi, off), G::kIdescScore, kk > 0 ? 1u : 0u);
   }
 }
 
 // D[dcol] (+)= W X: W [128][128] 16-bit in TMEM, X an MN-major tile of 128 rows.  W fills 64
 // columns, or (HALVES) 32 at wcol and 32 at wcol + 64: each half over the scores it came
 // from, so that the two warps that share a row's scores need not wait for one another.
-template <int D, bool F16, bool HALVES = false>
+// Rows [16 M0, 16 M1) of X alone: a part of the product, once a part of W is there.
+template <int D, bool F16, bool HALVES = false, int M0 = 0, int M1 = kTile / 16>
 __device__ __forceinline__ void mma_weights(uint32_t dcol, uint32_t wcol, uint32_t x, bool accumulate) {
   using G = Geo<D, F16>;
+  const uint64_t dx = smem_desc_sw128(x, G::kBoxBytes, 1024);
+  const uint32_t hi = static_cast<uint32_t>(dx >> 32), lo = static_cast<uint32_t>(dx);
 #pragma unroll
-  for (int m = 0; m < kTile / 16; ++m)
-    mma_ts(dcol, wcol + (HALVES ? 64 * (m >> 2) + 8 * (m & 3) : 8 * m), smem_desc_sw128(x + m * 2048, G::kBoxBytes, 1024), G::kIdescMn, (accumulate || m > 0) ? 1u : 0u);
+  for (int m = M0; m < M1; ++m)
+    mma_ts(dcol, wcol + (HALVES ? 64 * (m >> 2) + 8 * (m & 3) : 8 * m), desc_at(lo, hi, m * 2048), G::kIdescMn,
+           (accumulate || m > 0) ? 1u : 0u);
 }
 
 template <int D, bool F16>
@@ -71,6 +86,63 @@ __device__ __forceinline__ void zero_row(uint8_t* tile, int r) {
   for (int x = 0; x < D / 64; ++x)
 #pragma unroll
     for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + x * (kTile * 128) + r * 128 + 16 * c) = make_uint4(0, 0, 0, 0);
+}
+
+// 2^x of a pair for -125 <= x <= 126 on the FMA pipe (below: 2^-125): 2^n by the
+// exponent field, 2^f, |f| <= 1/2, by the polynomial of least relative error,
+// 7.5e-5 (degree 3, bf16 weights) or 2.6e-6 (degree 4, fp16 weights).
+template <bool F16>
+__device__ __forceinline__ float2 poly_ex2(float2 x) {
+  x.x = fmaxf(x.x, -125.0f);
+  x.y = fmaxf(x.y, -125.0f);
+  const float2 r = __fadd2_rn(x, make_float2(12582912.0f, 12582912.0f));  // 1.5 2^23: the last bits are n
+  const float2 n = __fadd2_rn(r, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);
+  float2 p;
+  if constexpr (F16) {
+    p = __ffma2_rn(f, make_float2(0.009570102207362652f, 0.009570102207362652f), make_float2(0.05591786280274391f, 0.05591786280274391f));
+    p = __ffma2_rn(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    p = __ffma2_rn(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    p = __ffma2_rn(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  } else {
+    p = __ffma2_rn(f, make_float2(0.0551716685295105f, 0.0551716685295105f), make_float2(0.2426111251115799f, 0.2426111251115799f));
+    p = __ffma2_rn(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
+    p = __ffma2_rn(p, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
+  }
+  return make_float2(__uint_as_float((__float_as_uint(r.x) << 23) + __float_as_uint(p.x)),
+                     __uint_as_float((__float_as_uint(r.y) << 23) + __float_as_uint(p.y)));
+}
+
+// The bounded wait of tda_ptx.cuh without its call: a warp whose register count
+// changes (setmaxnreg) may not call a function.
+__device__ __forceinline__ bool wait_inline(uint64_t* bar, uint32_t parity, const WaitCtl& ctl, int code) {
+  const uint32_t a = smem_u32(bar);
+  if (mbar_try_wait(a, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(a, parity)) {
+    if (*ctl.abort_flag) return false;
+    const uint64_t waited = global_timer_ns() - t0;
+    const bool other = waited > 1000000ull && *reinterpret_cast<volatile int*>(ctl.status) != ctl.status0;
+    if (other || waited > ctl.timeout_ns) {
+      *ctl.abort_flag = 1;
+      if (!other) atomicCAS(ctl.status, 0, code);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ bool wait_inline_warp(uint64_t* bar, uint32_t parity, const WaitCtl& ctl, int code) {
+  const bool ok = wait_inline(bar, parity, ctl, code);
+  return __all_sync(0xffffffffu, ok);
+}
+
+template <int kRegs>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
 __device__ __forceinline__ int keys_of(const SdParams& p, int b) {

@@ -26,10 +26,13 @@ namespace {
 
 using namespace sd;
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;  // warps 10 and 11 fill the third warpgroup
+// registers: 168 a thread at launch (64512); 128 x 72 + 256 x 216 = 64512
+constexpr int kFewRegs = 72, kManyRegs = 216;
 constexpr int kSoftmaxThreads = 256;
 constexpr int ST_PROD = 0x801, ST_MMA = 0x802, ST_SM = 0x803;
 constexpr float kLazy = 8.0f;
+constexpr int kPolyPairs = 3;  // of 8
 
 template <int D, bool F16>
 struct FC : Geo<D, F16> {
@@ -47,7 +50,7 @@ struct FC : Geo<D, F16> {
 
 struct FBars {
   uint64_t q_full, o_full, drain;
-  uint64_t s_full[2], p_full[2];
+  uint64_t s_full[2], p_half[2], p_full[2];
   uint64_t slot_full[8], slot_empty[8];
   uint32_t tmem_base;
   int abort_flag;
@@ -64,7 +67,7 @@ __device__ void produce(const SdTcParams& tp, uint8_t* smem, FBars* bars, const 
   int idx = 0;
   for (; idx < 3 * n; ++idx) {
     const int slot = idx % C::kSlots;
-    ok = mbar_wait(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_PROD);
+    ok = wait_inline(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_PROD);
     if (!ok) break;
     mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
     const int x = idx % 3;
@@ -84,7 +87,7 @@ __device__ void issue(uint8_t* smem, FBars* bars, const WaitCtl& ctl, uint32_t t
   const uint32_t q = smem_u32(smem), ring = smem_u32(smem + C::kOffRing);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok) ok = mbar_wait(bar, parity, ctl, ST_MMA);
+    if (ok) ok = wait_inline(bar, parity, ctl, ST_MMA);
     if (ok) tc_fence_after();
   };
   auto acquire = [&](int idx) {
@@ -105,9 +108,12 @@ __device__ void issue(uint8_t* smem, FBars* bars, const WaitCtl& ctl, uint32_t t
     const uint32_t v = acquire(3 * j + 2);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
+      wait(&bars->p_half[m], j & 1);
+      if (!ok) break;
+      mma_weights<D, F16, false, 0, 4>(tmem + C::o_col(m), tmem + C::s_col(m), v, j > 0);
       wait(&bars->p_full[m], j & 1);
       if (!ok) break;
-      mma_weights<D, F16>(tmem + C::o_col(m), tmem + C::s_col(m), v, j > 0);
+      mma_weights<D, F16, false, 4, 8>(tmem + C::o_col(m), tmem + C::s_col(m), v, true);
       if (m == 1) tc_commit(&bars->slot_empty[(3 * j + 2) % C::kSlots]);
       if (j + 1 < n) score(m, j + 1);
     }
@@ -118,6 +124,21 @@ __device__ void issue(uint8_t* smem, FBars* bars, const WaitCtl& ctl, uint32_t t
     tc_commit(&bars->drain);
     drain_wait(&bars->drain, 0, ctl);
   }
+}
+
+// 32 scores of a row to weights 2^(c s + base), written as 16 bits to TMEM; of
+// every 8 pairs, POLY go to the FMA pipe instead of the exponential unit.
+template <bool F16, int POLY>
+__device__ __forceinline__ void exponentials(const uint32_t (&s)[32], float c, float base, float2 (&sum)[2], uint32_t col) {
+  uint32_t w[16];
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const float2 e = __ffma2_rn(f2u(s[2 * x], s[2 * x + 1]), make_float2(c, c), make_float2(base, base));
+    const float2 pr = (x * POLY) % 8 < POLY ? poly_ex2<F16>(e) : make_float2(fast_ex2(e.x), fast_ex2(e.y));
+    sum[x & 1] = __fadd2_rn(sum[x & 1], pr);
+    w[x] = pack2<F16>(pr.x, pr.y);
+  }
+  tmem_st16(col, w);
 }
 
 template <int D, bool F16>
@@ -132,10 +153,10 @@ __device__ void softmax(const SdTcParams& tp, uint8_t* smem, FBars* bars, const 
   const int last = p.causal ? min(len - 1, grow + off) : len - 1;  // last key the row sees
   const float c = p.c;
   float top = -__builtin_huge_valf();  // running maximum of c s
-  float2 sum = make_float2(0.f, 0.f);
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   bool ok = true;
   for (int j = 0; j < n; ++j) {
-    ok = mbar_wait_warp(&bars->s_full[m], j & 1, ctl, ST_SM);
+    ok = wait_inline_warp(&bars->s_full[m], j & 1, ctl, ST_SM);
     if (!ok) break;
     tc_fence_after();
     uint32_t s[4][32];
@@ -163,8 +184,8 @@ __device__ void softmax(const SdTcParams& tp, uint8_t* smem, FBars* bars, const 
     if (__any_sync(0xffffffffu, grow_m)) {
       const float f = grow_m ? fast_ex2(top - now) : 1.0f;  // 0 for a row's first keys
       if (grow_m) top = now;
-      sum.x *= f;
-      sum.y *= f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sum[i] = __fmul2_rn(sum[i], make_float2(f, f));
       if (j > 0) {
 #pragma unroll
         for (int x = 0; x < D; x += 16) {
@@ -177,39 +198,43 @@ __device__ void softmax(const SdTcParams& tp, uint8_t* smem, FBars* bars, const 
         }
       }
     }
-    const float base = top == -__builtin_huge_valf() ? 0.f : -top;  // a row without keys so far: 2^(-inf)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t w[16];
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const float2 e = __ffma2_rn(f2u(s[i][2 * x], s[i][2 * x + 1]), make_float2(c, c), make_float2(base, base));
-        const float2 pr = make_float2(fast_ex2(e.x), fast_ex2(e.y));
-        sum = __fadd2_rn(sum, pr);
-        w[x] = pack2<F16>(pr.x, pr.y);
-      }
-      tmem_st16(s_col + 16 * i, w);
-    }
     // V rows past the length: zeroed before the product reads them
     if (j == n - 1 && len < p.Sk && (j + 1) * kTile > len) {
       const int idx = 3 * j + 2;
-      ok = mbar_wait_warp(&bars->slot_full[idx % C::kSlots], (idx / C::kSlots) & 1, ctl, ST_SM);
+      ok = wait_inline_warp(&bars->slot_full[idx % C::kSlots], (idx / C::kSlots) & 1, ctl, ST_SM);
       if (!ok) break;
       if (j * kTile + row >= len) zero_row<D>(smem + C::kOffRing + (idx % C::kSlots) * C::kTileBytes, row);
       fence_proxy_async_smem();
     }
-    tmem_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars->p_full[m]);
+    const float base = top == -__builtin_huge_valf() ? 0.f : -top;  // a row without keys so far: 2^(-inf)
+    auto arrive = [&](uint64_t* bar) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    if (masked) {  // hidden keys are -inf: exactly 0 by the hardware's exponential alone
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        exponentials<F16, 0>(s[i], c, base, sum, s_col + 16 * i);
+        if (i == 1) arrive(&bars->p_half[m]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        exponentials<F16, kPolyPairs>(s[i], c, base, sum, s_col + 16 * i);
+        if (i == 1) arrive(&bars->p_half[m]);
+      }
+    }
+    arrive(&bars->p_full[m]);
   }
   // epilogue: out = O1 / l1 - lambda O2 / l2, a warpgroup half of the columns
   float* inv = reinterpret_cast<float*>(smem + C::kOffBar + 1024);
-  const float l = sum.x + sum.y;
+  const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
   inv[m * kTile + row] = l == 0.f ? 0.f : 1.0f / l;
   const long long bh = static_cast<long long>(b) * p.H + h, n_bh = static_cast<long long>(p.B) * p.H;
   if (p.lse && grow < p.Sq) p.lse[(m * n_bh + bh) * p.Sq + grow] = l == 0.f ? __builtin_huge_valf() : top + log2f(l);
-  if (ok && n > 0) ok = mbar_wait_warp(&bars->o_full, 0, ctl, ST_SM);
+  if (ok && n > 0) ok = wait_inline_warp(&bars->o_full, 0, ctl, ST_SM);
   tc_fence_after();
   named_barrier_and(1, kSoftmaxThreads, true);
   const float i1 = inv[row], i2 = inv[kTile + row], lam = lambda_at(p.lam, b, h);
@@ -279,6 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_fwd_kernel(const __grid_
     mbar_init(&bars->drain, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_half[i], 4);
       mbar_init(&bars->p_full[i], 4);
     }
     for (int i = 0; i < C::kSlots; ++i) {
@@ -298,10 +324,12 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_fwd_kernel(const __grid_
   const uint32_t tmem = bars->tmem_base;
   const WaitCtl ctl = make_wait_ctl(&bars->abort_flag, tp.status, tp.timeout_ns);
   if (warp < 8) {
+    more_registers<kManyRegs>();
     softmax<D, F16>(tp, smem, bars, ctl, tmem, b, h, qt, n, len, warp, lane);
-  } else if (n > 0) {
-    if (warp == 8 && lane == 0) produce<D, F16>(tp, smem, bars, ctl, b, h, kvh, qt, n);
-    if (warp == 9 && lane == 0) issue<D, F16>(smem, bars, ctl, tmem, n);
+  } else {
+    fewer_registers<kFewRegs>();
+    if (n > 0 && warp == 8 && lane == 0) produce<D, F16>(tp, smem, bars, ctl, b, h, kvh, qt, n);
+    if (n > 0 && warp == 9 && lane == 0) issue<D, F16>(smem, bars, ctl, tmem, n);
     __syncwarp();
   }
   tc_fence_before();

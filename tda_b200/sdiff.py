@@ -29,23 +29,24 @@ from . import ops as _ops
 _CODE = {torch.float32: _lib.TDA_F32, torch.bfloat16: _lib.TDA_BF16, torch.float16: _lib.TDA_F16}
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# Small calls are bound by the host: a stream object costs 2 us to make, its handle alone 0.1.
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-class _on:
-    """Makes ``device`` current around a launch, at no cost where it already is."""
-
-    def __init__(self, device):
-        self.ctx = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+def launch(entry, device: torch.device, *args) -> None:
+    """Calls a C entry point on ``device``'s current stream (appended to
+    ``args``), making the device current where it is not, and raises on an
+    error code."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, _raw_stream(index))
+    if rc != 0:
+        _lib.check(rc)
+    if _ops._SYNC_CHECK:
+        _ops.check_status(device)
 
 
 def lambda_ref(lam, B: int, H: int, device: torch.device, what: str):
@@ -54,6 +55,12 @@ def lambda_ref(lam, B: int, H: int, device: torch.device, what: str):
     broadcasts over (batch, head) stays on the device in its own type."""
     if not isinstance(lam, torch.Tensor):
         return None, 0, 0, 0, float(lam), None
+    if lam.is_cuda and lam.dtype in _CODE and lam.device == device:  # the usual forms, without views
+        shape = lam.shape
+        if lam.numel() == 1 and len(shape) <= 4:
+            return lam.data_ptr(), _CODE[lam.dtype], 0, 0, 0.0, lam
+        if len(shape) == 4 and shape[0] == 1 and shape[1] == H and shape[2] == 1 and shape[3] == 1:
+            return lam.data_ptr(), _CODE[lam.dtype], 0, lam.stride(1), 0.0, lam
     if not lam.dtype.is_floating_point:
         raise TypeError(f"{what}: lambda must be floating point, got {lam.dtype}")
     if not lam.is_cuda and lam.numel() == 1:
@@ -123,6 +130,8 @@ def view_of(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     dimension of size 1 counts as fitting), 16-byte aligned; else a copy."""
     if t.dtype != dtype:
         t = t.to(dtype)
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
     if ok:
         for n, s in zip(t.shape[:-1], t.stride()[:-1]):
@@ -134,7 +143,9 @@ def view_of(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 def strides_of(ts):
     """Element strides of all but the last dimension, a stride that is never
-    used (size 1) given as the row's length."""
+    used (size 1) given as the row's length; None when all are contiguous."""
+    if all(t.is_contiguous() for t in ts):
+        return None
     out = []
     for t in ts:
         d = t.shape[-1]
@@ -143,8 +154,8 @@ def strides_of(ts):
 
 
 def _lengths32(key_lengths):
-    if key_lengths is None:
-        return None
+    if key_lengths is None or (key_lengths.dtype == torch.int32 and key_lengths.is_contiguous()):
+        return key_lengths
     return key_lengths.to(torch.int32).contiguous()
 
 
@@ -165,16 +176,10 @@ def sdiff_forward(q1, q2, k1, k2, v, lambda_param, scale=None, causal=True, key_
     ts = [view_of(t, dt) for t in (q1, q2, k1, k2, v)]
     kl = _lengths32(key_lengths)
     lp, lc, lsb, lsh, lv, keep = lambda_ref(lambda_param, B, H, q1.device, "differential_softmax_attention")
-    lib = _lib.load()
-    with _on(q1.device):
-        rc = lib.tda_sdiff_fwd(*[t.data_ptr() for t in ts], strides_of(ts), out.data_ptr(),
-                               o12.data_ptr() if save else None, lse.data_ptr() if save else None, _CODE[dt], B, H, Hkv, Sq, Sk, D,
-                               1.0 / math.sqrt(D) if scale is None else float(scale), int(causal),
-                               None if kl is None else kl.data_ptr(), lp, lc, lsb, lsh, lv,
-                               _ops._status_word(q1.device).data_ptr(), _stream(q1.device))
-    _lib.check(rc)
-    if _ops._SYNC_CHECK:
-        _ops.check_status(q1.device)
+    launch(_lib.load().tda_sdiff_fwd, q1.device, *[t.data_ptr() for t in ts], strides_of(ts), out.data_ptr(),
+           o12.data_ptr() if save else None, lse.data_ptr() if save else None, _CODE[dt], B, H, Hkv, Sq, Sk, D,
+           1.0 / math.sqrt(D) if scale is None else float(scale), int(causal), None if kl is None else kl.data_ptr(),
+           lp, lc, lsb, lsh, lv, _ops._status_word(q1.device).data_ptr())
     return out, o12, lse
 
 
@@ -203,16 +208,11 @@ def sdiff_backward(q1, q2, k1, k2, v, dout, o12, lse, lambda_param, scale=None, 
     lib = _lib.load()
     ws_n = lib.tda_sdiff_bwd_workspace_size(B, H, Sq)
     ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = lib.tda_sdiff_bwd(*[t.data_ptr() for t in ts], strides_of(ts), g.data_ptr(), strides_of([g]),
-                               o12.data_ptr(), lse.data_ptr(), *[t.data_ptr() for t in dq + dkv],
-                               dlam.data_ptr() if need_dlam else None, _CODE[dt], B, H, Hkv, Sq, Sk, D,
-                               1.0 / math.sqrt(D) if scale is None else float(scale), int(causal),
-                               None if kl is None else kl.data_ptr(), lp, lc, lsb, lsh, lv, ws.data_ptr(), ws_n,
-                               _ops._status_word(dev).data_ptr(), _stream(dev))
-    _lib.check(rc)
-    if _ops._SYNC_CHECK:
-        _ops.check_status(dev)
+    launch(lib.tda_sdiff_bwd, dev, *[t.data_ptr() for t in ts], strides_of(ts), g.data_ptr(), strides_of([g]),
+           o12.data_ptr(), lse.data_ptr(), *[t.data_ptr() for t in dq + dkv], dlam.data_ptr() if need_dlam else None,
+           _CODE[dt], B, H, Hkv, Sq, Sk, D, 1.0 / math.sqrt(D) if scale is None else float(scale), int(causal),
+           None if kl is None else kl.data_ptr(), lp, lc, lsb, lsh, lv, ws.data_ptr(), ws_n,
+           _ops._status_word(dev).data_ptr())
     return (*dq, *dkv, dlam)
 
 
