@@ -166,7 +166,7 @@ int tda_sdiff_fwd(const void* q1, const void* q2, const void* k1, const void* k2
 
 size_t tda_sdiff_bwd_workspace_size(int64_t batch, int64_t heads, int64_t q_len) {
   if (batch < 1 || heads < 1 || q_len < 1) return 0;
-  return 2 * static_cast<size_t>(batch) * heads * padded_seq(q_len) * sizeof(float2);
+  return 2 * static_cast<size_t>(batch) * heads * padded_seq(q_len) * 2 * sizeof(float);
 }
 
 int tda_sdiff_bwd(const void* q1, const void* q2, const void* k1, const void* k2, const void* v,
@@ -195,7 +195,7 @@ int tda_sdiff_bwd(const void* q1, const void* q2, const void* k1, const void* k2
     return fail(TDA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed", bytes);
   p.o12 = const_cast<float*>(o12);
   p.lse = const_cast<float*>(lse);
-  p.table = static_cast<float2*>(workspace);
+  p.table = static_cast<float*>(workspace);
   p.pad = static_cast<int>(padded_seq(q_len));
   p.dq[0] = dq1;
   p.dq[1] = dq2;

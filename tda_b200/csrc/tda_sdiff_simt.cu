@@ -140,8 +140,9 @@ __device__ __forceinline__ long long row_at(const SdParams& p, int m, int b, int
   return ((static_cast<long long>(m) * p.B + b) * p.H + h) * p.Sq + i;
 }
 
-__device__ __forceinline__ long long table_at(const SdParams& p, int m, int b, int h, int i) {
-  return ((static_cast<long long>(m) * p.B + b) * p.H + h) * p.pad + i;
+// L of row i of map m and (batch, head) bh; its D lies kTile behind
+__device__ __forceinline__ long long table_at(const SdParams& p, int m, long long bh, int i) {
+  return 2 * ((static_cast<long long>(m) * p.B * p.H + bh) * p.pad + i / kTile * kTile) + i % kTile;
 }
 
 // ================================================================== forward
@@ -261,8 +262,12 @@ __global__ void __launch_bounds__(256) sdiff_delta_kernel(const SdParams p) {
     c += __shfl_xor_sync(0xffffffffu, c, o);
   }
   if (row < rows && l == 0) {
-    p.table[row] = make_float2(i < p.Sq ? p.lse[at] : kInf, a);
-    p.table[rows + row] = make_float2(i < p.Sq ? p.lse[all + at] : kInf, c);
+    float* t = p.table + table_at(p, 0, bh, i);
+    t[0] = i < p.Sq ? p.lse[at] : kInf;
+    t[kTile] = a;
+    t += 2 * rows;
+    t[0] = i < p.Sq ? p.lse[all + at] : kInf;
+    t[kTile] = c;
   }
 }
 
@@ -270,9 +275,8 @@ __global__ void __launch_bounds__(256) sdiff_delta_kernel(const SdParams p) {
 __global__ void __launch_bounds__(256) sdiff_dlam_kernel(const SdParams p) {
   __shared__ float part[256];
   const long long bh = blockIdx.x;
-  const float2* d = p.table + (static_cast<long long>(p.B) * p.H + bh) * p.pad;
   float s = 0.f;
-  for (int i = threadIdx.x; i < p.Sq; i += 256) s += d[i].y;
+  for (int i = threadIdx.x; i < p.Sq; i += 256) s += p.table[table_at(p, 1, bh, i) + kTile];
   part[threadIdx.x] = s;
   __syncthreads();
   for (int o = 128; o > 0; o >>= 1) {
@@ -302,9 +306,9 @@ __global__ void __launch_bounds__(256) sdiff_simt_dq_kernel(const SdParams p) {
 #pragma unroll
   for (int r = 0; r < C::R; ++r) {
     const int i = i0 + ty * C::R + r;
-    const float2 t = i < p.Sq ? p.table[table_at(p, m, b, h, i)] : make_float2(kInf, 0.f);
-    lse[r] = t.x;
-    del[r] = t.y;
+    const float* t = p.table + table_at(p, m, bh, min(i, p.Sq - 1));
+    lse[r] = i < p.Sq ? t[0] : kInf;
+    del[r] = t[kTile];
 #pragma unroll
     for (int c = 0; c < C::C; ++c) o[r][c] = 0.f;
   }
@@ -372,9 +376,9 @@ __global__ void __launch_bounds__(256) sdiff_simt_dkv_kernel(const SdParams p) {
         load_tile<T, D>(gs, p.dout, b, h, i0, p.Sq);
         if (threadIdx.x < C::BT) {
           const int i = i0 + threadIdx.x;
-          const float2 t = i < p.Sq ? p.table[table_at(p, m, b, h, i)] : make_float2(kInf, 0.f);
-          ls[threadIdx.x] = t.x;
-          es[threadIdx.x] = t.y;
+          const float* t = p.table + table_at(p, m, static_cast<long long>(b) * p.H + h, min(i, p.Sq - 1));
+          ls[threadIdx.x] = i < p.Sq ? t[0] : kInf;
+          es[threadIdx.x] = t[kTile];
         }
         __syncthreads();
         float s[C::R][C::R], dp[C::R][C::R];

@@ -1,6 +1,6 @@
 // Backward of softmax differential attention on the tensor cores (tcgen05,
 // TMEM, TMA): bf16 or fp16, head_dim 64 / 128.  Formulas in tda_sdiff.h; row
-// table {L_m(i), D_m(i)} from the row-sum pass (rows past Sq: {+inf, 0}).
+// table L_m(i), D_m(i) from the row-sum pass (rows past Sq: +inf, 0).
 //
 // Two kernels, no atomic sums (the same bits every time):
 //   dkv, a CTA a tile of 128 keys of one kv head.  Rows are keys: per query tile
@@ -23,7 +23,10 @@ namespace {
 
 using namespace sd;
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;  // warps 10 and 11 fill the third warpgroup
+// registers: 168 a thread at launch (64512); 128 x 72 + 256 x 216 = 64512
+constexpr int kFewRegs = 72, kManyRegs = 216;
+constexpr int kPolyPairs = 3;  // of 8 go to the FMA pipe instead of the exponential unit
 constexpr int kWorkThreads = 256;
 constexpr int kTab = 4;
 constexpr int ST_KP = 0x901, ST_KM = 0x902, ST_KW = 0x903, ST_QP = 0xa01, ST_QM = 0xa02, ST_QW = 0xa03;
@@ -52,7 +55,7 @@ struct KvWork {
 };
 
 template <int D, bool F16>
-__device__ void kv_produce(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const WaitCtl& ctl, const KvWork& w, const float2* table,
+__device__ void kv_produce(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const WaitCtl& ctl, const KvWork& w, const float* table,
                            int pad) {
   using C = KvC<D, F16>;
   const SdParams& p = tp.p;
@@ -61,7 +64,7 @@ __device__ void kv_produce(const SdTcParams& tp, uint8_t* smem, KvBars* bars, co
   bool ok = true;
   int t = 0, idx = 0, n_k = 0;
   for (int m = 0; m < 2 && ok; ++m) {
-    if (m == 1) ok = mbar_wait(&bars->k_free, 0, ctl, ST_KP);
+    if (m == 1) ok = wait_inline(&bars->k_free, 0, ctl, ST_KP);
     if (!ok) break;
     mbar_arrive_expect_tx(&bars->k_full, C::kTileBytes);
     load_tile<D, F16>(smem, &tp.m.k[m], &bars->k_full, w.kt * kTile, w.kvh, w.b);
@@ -69,14 +72,14 @@ __device__ void kv_produce(const SdTcParams& tp, uint8_t* smem, KvBars* bars, co
     for (int h = w.kvh * p.group; h < (w.kvh + 1) * p.group && ok; ++h) {
       for (int i = w.i0; i < tp.n_qt; ++i, ++t) {
         const int e = t % kTab;
-        ok = mbar_wait(&bars->tab_empty[e], ((t / kTab) & 1) ^ 1, ctl, ST_KP);
+        ok = wait_inline(&bars->tab_empty[e], ((t / kTab) & 1) ^ 1, ctl, ST_KP);
         if (!ok) break;
         mbar_arrive_expect_tx(&bars->tab_full[e], kTile * 8);
         const long long row = (static_cast<long long>(m) * p.B + w.b) * p.H + h;
-        bulk_load(smem + C::kOffTab + e * kTile * 8, table + row * pad + i * kTile, kTile * 8, &bars->tab_full[e]);
+        bulk_load(smem + C::kOffTab + e * kTile * 8, table + 2 * (row * pad + i * kTile), kTile * 8, &bars->tab_full[e]);
         for (int x = 0; x < 2; ++x) {
           const int slot = idx % C::kSlots;
-          ok = mbar_wait(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_KP);
+          ok = wait_inline(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_KP);
           if (!ok) break;
           mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
           load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, x ? &tp.m.dout : &tp.m.q[m], &bars->slot_full[slot], i * kTile, h,
@@ -105,7 +108,7 @@ __device__ void kv_issue(uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32
   const uint32_t k = smem_u32(smem), v = k + C::kTileBytes, ring = smem_u32(smem + C::kOffRing);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok) ok = mbar_wait(bar, parity, ctl, ST_KM);
+    if (ok) ok = wait_inline(bar, parity, ctl, ST_KM);
     if (ok) tc_fence_after();
   };
   auto acquire = [&](int idx) {
@@ -184,38 +187,45 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
   const float c = p.c;
   bool ok = true;
   int t = 0;
-  if (w.per_map > 0) ok = mbar_wait_warp(&bars->v_full, 0, ctl, ST_KW);
+  if (w.per_map > 0) ok = wait_inline_warp(&bars->v_full, 0, ctl, ST_KW);
   for (int m = 0; m < 2; ++m) {
     for (int h = w.kvh * p.group; h < (w.kvh + 1) * p.group && ok; ++h) {
       const float wt = m ? -lambda_at(p.lam, w.b, h) : 1.0f;
       for (int i = w.i0; i < tp.n_qt && w.per_map > 0; ++i, ++t) {
         const int e = t % kTab;
-        ok = mbar_wait_warp(&bars->tab_full[e], (t / kTab) & 1, ctl, ST_KW);
-        if (ok) ok = mbar_wait_warp(&bars->s_full, t & 1, ctl, ST_KW);
+        ok = wait_inline_warp(&bars->tab_full[e], (t / kTab) & 1, ctl, ST_KW);
+        if (ok) ok = wait_inline_warp(&bars->s_full, t & 1, ctl, ST_KW);
         if (!ok) break;
         tc_fence_after();
-        const float4* tab = reinterpret_cast<const float4*>(smem + C::kOffTab + e * kTile * 8) + 32 * wg;
+        const float4* tab = reinterpret_cast<const float4*>(smem + C::kOffTab + e * kTile * 8) + 16 * wg;
         const bool masked = (w.kt + 1) * kTile > len || (p.causal && i * kTile + off < (w.kt + 1) * kTile - 1) || lone;
         // queries of this tile in front of `lo` do not see the key
         const int lo = dead ? kTile : (p.causal ? key - off - i * kTile : 0);
         float pr[64];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          uint32_t s[32];
-          tmem_ld32(s_col + 32 * x, s);
+        {
+          uint32_t s[2][32];
+          tmem_ld32(s_col, s[0]);
+          tmem_ld32(s_col + 32, s[1]);
           tmem_wait_ld();
 #pragma unroll
-          for (int y = 0; y < 32; y += 2) {
-            const float4 q = tab[16 * x + y / 2];  // {L, D} of two queries
-            const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(-q.x, -q.z));
-            const float2 r = __fmul2_rn(make_float2(fast_ex2(z.x), fast_ex2(z.y)), make_float2(wt, wt));
-            pr[32 * x + y] = r.x;
-            pr[32 * x + y + 1] = r.y;
-          }
-          if (masked) {
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int y = 0; y < 32; ++y) pr[32 * x + y] = 64 * wg + 32 * x + y >= lo ? pr[32 * x + y] : 0.f;
-          }
+            for (int y = 0; y < 32; y += 4) {
+              const float4 q = tab[8 * x + y / 4];  // L of four queries
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                const float2 z = __ffma2_rn(f2u(s[x][y + i], s[x][y + i + 1]), make_float2(c, c),
+                                            i ? make_float2(-q.z, -q.w) : make_float2(-q.x, -q.y));
+                const float2 ez = ((y + i) / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
+                const float2 r = __fmul2_rn(ez, make_float2(wt, wt));
+                pr[32 * x + y + i] = r.x;
+                pr[32 * x + y + i + 1] = r.y;
+              }
+            }
+        }
+        if (masked) {
+#pragma unroll
+          for (int y = 0; y < 64; ++y) pr[y] = 64 * wg + y >= lo ? pr[y] : 0.f;
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -229,26 +239,31 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->p_full);
 
-        ok = mbar_wait_warp(&bars->dp_full, t & 1, ctl, ST_KW);
+        ok = wait_inline_warp(&bars->dp_full, t & 1, ctl, ST_KW);
         if (!ok) break;
         tc_fence_after();
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          uint32_t s[32];
-          tmem_ld32(p_col + 32 * x, s);
+        {
+          uint32_t s[2][32];
+          tmem_ld32(p_col, s[0]);
+          tmem_ld32(p_col + 32, s[1]);
           tmem_wait_ld();
 #pragma unroll
-          for (int y = 0; y < 32; y += 2) {
-            const float4 q = tab[16 * x + y / 2];
-            const float2 d = __fadd2_rn(f2u(s[y], s[y + 1]), make_float2(-q.y, -q.w));
-            const float2 r = __fmul2_rn(make_float2(pr[32 * x + y], pr[32 * x + y + 1]), d);
-            pr[32 * x + y] = r.x;
-            pr[32 * x + y + 1] = r.y;
-          }
-          if (masked) {
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int y = 0; y < 32; ++y) pr[32 * x + y] = 64 * wg + 32 * x + y >= lo && !lone ? pr[32 * x + y] : 0.f;
-          }
+            for (int y = 0; y < 32; y += 4) {
+              const float4 q = tab[32 + 8 * x + y / 4];  // D of four queries
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                const float2 d = __fadd2_rn(f2u(s[x][y + i], s[x][y + i + 1]), i ? make_float2(-q.z, -q.w) : make_float2(-q.x, -q.y));
+                const float2 r = __fmul2_rn(make_float2(pr[32 * x + y + i], pr[32 * x + y + i + 1]), d);
+                pr[32 * x + y + i] = r.x;
+                pr[32 * x + y + i + 1] = r.y;
+              }
+            }
+        }
+        if (masked) {
+#pragma unroll
+          for (int y = 0; y < 64; ++y) pr[y] = 64 * wg + y >= lo && !lone ? pr[y] : 0.f;
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -267,7 +282,7 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
       }
     }
     // dK_m through the K buffer (idle once every product of the map is done), and dV through V's at the end
-    if (ok && w.per_map > 0) ok = mbar_wait_warp(&bars->map_done, m, ctl, ST_KW);
+    if (ok && w.per_map > 0) ok = wait_inline_warp(&bars->map_done, m, ctl, ST_KW);
     tc_fence_after();
     if (ok) {
       stage_accumulator<D, F16>(smem, tmem + lane_off + C::kDK, row, wg, p.scale, w.per_map == 0);
@@ -292,7 +307,7 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
 }
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_constant__ SdTcParams tp, const float2* table, int pad) {
+__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_constant__ SdTcParams tp, const float* table, int pad) {
   using C = KvC<D, F16>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -333,10 +348,12 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
   const uint32_t tmem = bars->tmem_base;
   const WaitCtl ctl = make_wait_ctl(&bars->abort_flag, tp.status, tp.timeout_ns);
   if (warp < 8) {
+    more_registers<kManyRegs>();
     kv_work<D, F16>(tp, smem, bars, ctl, tmem, w, len, warp, lane);
-  } else if (w.per_map > 0) {
-    if (warp == 8 && lane == 0) kv_produce<D, F16>(tp, smem, bars, ctl, w, table, pad);
-    if (warp == 9 && lane == 0) kv_issue<D, F16>(smem, bars, ctl, tmem, w.per_map);
+  } else {
+    fewer_registers<kFewRegs>();
+    if (w.per_map > 0 && warp == 8 && lane == 0) kv_produce<D, F16>(tp, smem, bars, ctl, w, table, pad);
+    if (w.per_map > 0 && warp == 9 && lane == 0) kv_issue<D, F16>(smem, bars, ctl, tmem, w.per_map);
     __syncwarp();
   }
   tc_fence_before();
@@ -379,7 +396,7 @@ __device__ void q_produce(const SdTcParams& tp, uint8_t* smem, QBars* bars, cons
   int idx = 0;
   for (; idx < 2 * n; ++idx) {
     const int slot = idx % C::kSlots;
-    ok = mbar_wait(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_QP);
+    ok = wait_inline(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_QP);
     if (!ok) break;
     mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
     load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, idx & 1 ? &tp.m.v : &tp.m.k[m], &bars->slot_full[slot], idx / 2 * kTile,
@@ -398,7 +415,7 @@ __device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t
   const uint32_t q = smem_u32(smem), g = q + C::kTileBytes, ring = smem_u32(smem + C::kOffRing);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok) ok = mbar_wait(bar, parity, ctl, ST_QM);
+    if (ok) ok = wait_inline(bar, parity, ctl, ST_QM);
     if (ok) tc_fence_after();
   };
   auto acquire = [&](int idx) {
@@ -442,61 +459,64 @@ __device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t
 }
 
 template <int D, bool F16>
-__device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t tmem, const float2* table, int pad,
+__device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t tmem, const float* table, int pad,
                        int m, int b, int h, int qt, int n, int len, int warp, int lane) {
   using C = QC<D, F16>;
   const SdParams& p = tp.p;
   const int wg = warp >> 2, row = (warp & 3) * 32 + lane, grow = qt * kTile + row, off = p.Sk - p.Sq;
   const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
   const long long bh = static_cast<long long>(b) * p.H + h;
-  const float2 row_tab = table[(static_cast<long long>(m) * p.B * p.H + bh) * pad + grow];
-  const float L = row_tab.x, del = row_tab.y, c = p.c;
+  const float* row_tab = table + 2 * ((static_cast<long long>(m) * p.B * p.H + bh) * pad + qt * kTile) + row;
+  const float L = row_tab[0], del = row_tab[kTile], c = p.c;
   const int last = p.causal ? min(len - 1, grow + off) : len - 1;
   bool ok = true;
   for (int t = 0; t < n; ++t) {
-    ok = mbar_wait_warp(&bars->s_full[t & 1], (t >> 1) & 1, ctl, ST_QW);
+    ok = wait_inline_warp(&bars->s_full[t & 1], (t >> 1) & 1, ctl, ST_QW);
     if (!ok) break;
     tc_fence_after();
     const uint32_t s_col = tmem + lane_off + C::s_col(t);
     const bool masked = (t + 1) * kTile > len || (p.causal && (t + 1) * kTile - 1 > qt * kTile + off);
     float pr[64];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      uint32_t s[32];
-      tmem_ld32(s_col + 64 * wg + 32 * x, s);
+    {
+      uint32_t s[2][32];
+      tmem_ld32(s_col + 64 * wg, s[0]);
+      tmem_ld32(s_col + 64 * wg + 32, s[1]);
       tmem_wait_ld();
 #pragma unroll
-      for (int y = 0; y < 32; y += 2) {
-        const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(-L, -L));
-        pr[32 * x + y] = fast_ex2(z.x);
-        pr[32 * x + y + 1] = fast_ex2(z.y);
-      }
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 32; y += 2) {
+          const float2 z = __ffma2_rn(f2u(s[x][y], s[x][y + 1]), make_float2(c, c), make_float2(-L, -L));
+          const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
+          pr[32 * x + y] = ez.x;
+          pr[32 * x + y + 1] = ez.y;
+        }
     }
-    ok = mbar_wait_warp(&bars->dp_full, t & 1, ctl, ST_QW);
+    ok = wait_inline_warp(&bars->dp_full, t & 1, ctl, ST_QW);
     if (!ok) break;
     tc_fence_after();
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      uint32_t s[32];
-      tmem_ld32(tmem + lane_off + C::kP + 64 * wg + 32 * x, s);
+    {
+      uint32_t s[2][32];
+      tmem_ld32(tmem + lane_off + C::kP + 64 * wg, s[0]);
+      tmem_ld32(tmem + lane_off + C::kP + 64 * wg + 32, s[1]);
       tmem_wait_ld();
-      if (x == 1) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->dp_free);
-      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->dp_free);
 #pragma unroll
-      for (int y = 0; y < 32; y += 2) {
-        const float2 d = __fadd2_rn(f2u(s[y], s[y + 1]), make_float2(-del, -del));
-        const float2 r = __fmul2_rn(make_float2(pr[32 * x + y], pr[32 * x + y + 1]), d);
-        pr[32 * x + y] = r.x;
-        pr[32 * x + y + 1] = r.y;
-      }
-      if (masked) {
-        const int lim = last - t * kTile - 64 * wg - 32 * x;
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int y = 0; y < 32; ++y) pr[32 * x + y] = y <= lim ? pr[32 * x + y] : 0.f;
-      }
+        for (int y = 0; y < 32; y += 2) {
+          const float2 d = __fadd2_rn(f2u(s[x][y], s[x][y + 1]), make_float2(-del, -del));
+          const float2 r = __fmul2_rn(make_float2(pr[32 * x + y], pr[32 * x + y + 1]), d);
+          pr[32 * x + y] = r.x;
+          pr[32 * x + y + 1] = r.y;
+        }
+    }
+    if (masked) {
+      const int lim = last - t * kTile - 64 * wg;
+#pragma unroll
+      for (int y = 0; y < 64; ++y) pr[y] = y <= lim ? pr[y] : 0.f;
     }
     // K rows past the length: zeroed (S is done with them) before the product with dS reads them
     if (t == n - 1 && len < p.Sk && (t + 1) * kTile > len) {
@@ -515,7 +535,7 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars->ds_full[t & 1]);
   }
-  if (ok && n > 0) ok = mbar_wait_warp(&bars->o_full, 0, ctl, ST_QW);
+  if (ok && n > 0) ok = wait_inline_warp(&bars->o_full, 0, ctl, ST_QW);
   tc_fence_after();
   const float w = (m ? -lambda_at(p.lam, b, h) : 1.0f) * p.scale;
   uint8_t* stage = smem + C::kOffRing;
@@ -532,7 +552,7 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
 }
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_constant__ SdTcParams tp, const float2* table, int pad) {
+__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_constant__ SdTcParams tp, const float* table, int pad) {
   using C = QC<D, F16>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -575,10 +595,12 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
   const uint32_t tmem = bars->tmem_base;
   const WaitCtl ctl = make_wait_ctl(&bars->abort_flag, tp.status, tp.timeout_ns);
   if (warp < 8) {
+    more_registers<kManyRegs>();
     q_work<D, F16>(tp, smem, bars, ctl, tmem, table, pad, m, b, h, qt, n, len, warp, lane);
-  } else if (n > 0) {
-    if (warp == 8 && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, m, b, h, kvh, qt, n);
-    if (warp == 9 && lane == 0) q_issue<D, F16>(smem, bars, ctl, tmem, n);
+  } else {
+    fewer_registers<kFewRegs>();
+    if (n > 0 && warp == 8 && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, m, b, h, kvh, qt, n);
+    if (n > 0 && warp == 9 && lane == 0) q_issue<D, F16>(smem, bars, ctl, tmem, n);
     __syncwarp();
   }
   tc_fence_before();
@@ -590,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
 }
 
 template <int D, bool F16>
-cudaError_t launch(const SdTcParams& tp, const float2* table, int pad, cudaStream_t s) {
+cudaError_t launch(const SdTcParams& tp, const float* table, int pad, cudaStream_t s) {
   auto kq = sdiff_tc_dq_kernel<D, F16>;
   auto kk = sdiff_tc_dkv_kernel<D, F16>;
   if (cudaError_t e = allow_shared<sdiff_tc_dq_kernel<D, F16>>(QC<D, F16>::kSmem)) return e;
@@ -604,7 +626,7 @@ cudaError_t launch(const SdTcParams& tp, const float2* table, int pad, cudaStrea
 }  // namespace
 
 cudaError_t launch_sdiff_tc_bwd(const SdTcParams& tp, int dtype, int D, cudaStream_t s) {
-  const float2* table = tp.p.table;
+  const float* table = tp.p.table;
   const int pad = tp.p.pad;
   if (dtype == TDA_BF16) return D == 64 ? launch<64, false>(tp, table, pad, s) : launch<128, false>(tp, table, pad, s);
   return D == 64 ? launch<64, true>(tp, table, pad, s) : launch<128, true>(tp, table, pad, s);
