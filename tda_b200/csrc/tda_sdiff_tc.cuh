@@ -34,6 +34,22 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
 }
 
+// The issuing warp stays converged: every lane runs the waits and the address
+// arithmetic, so that descriptors and TMEM addresses live in uniform registers,
+// and one elected lane (the same every time) issues.  With a branch on the lane
+// index instead, each product's operands are moved there one by one, about 60-100
+// cycles a product against 64 of tensor work.
+__device__ __forceinline__ bool elected() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if (elected()) tc_commit(bar);
+  __syncwarp();
+}
+
 // Operand descriptors differ in their address field alone (bytes / 16, and all of
 // shared memory fits the field): one 32-bit addition an operand keeps the single
 // issuing thread ahead of the tensor cores.
@@ -49,11 +65,14 @@ __device__ __forceinline__ void mma_score(uint32_t dcol, uint32_t a, uint32_t b)
   using G = Geo<D, F16>;
   const uint64_t da = smem_desc_sw128(a, 16, 1024), db = smem_desc_sw128(b, 16, 1024);
   const uint32_t hi = static_cast<uint32_t>(da >> 32), la = static_cast<uint32_t>(da), lb = static_cast<uint32_t>(db);
+  if (elected()) {
 #pragma unroll
-  for (int kk = 0; kk < D / 16; ++kk) {
-    const uint32_t off = (kk >> 2) * G::kBoxBytes + (kk & 3) * 32;
-    mma_ss(dcol, desc_at(la, hi, off), desc_at(lb, hi, off), G::kIdescScore, kk > 0 ? 1u : 0u);
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint32_t off = (kk >> 2) * G::kBoxBytes + (kk & 3) * 32;
+      mma_ss(dcol, desc_at(la, hi, off), desc_at(lb, hi, off), G::kIdescScore, kk > 0 ? 1u : 0u);
+    }
   }
+  __syncwarp();
 }
 
 // D[dcol] (+)= W X: W [128][128] 16-bit in TMEM, X an MN-major tile of 128 rows.  W fills 64
@@ -65,10 +84,13 @@ __device__ __forceinline__ void mma_weights(uint32_t dcol, uint32_t wcol, uint32
   using G = Geo<D, F16>;
   const uint64_t dx = smem_desc_sw128(x, G::kBoxBytes, 1024);
   const uint32_t hi = static_cast<uint32_t>(dx >> 32), lo = static_cast<uint32_t>(dx);
+  if (elected()) {
 #pragma unroll
-  for (int m = M0; m < M1; ++m)
-    mma_ts(dcol, wcol + (HALVES ? 64 * (m >> 2) + 8 * (m & 3) : 8 * m), desc_at(lo, hi, m * 2048), G::kIdescMn,
-           (accumulate || m > 0) ? 1u : 0u);
+    for (int m = M0; m < M1; ++m)
+      mma_ts(dcol, wcol + (HALVES ? 64 * (m >> 2) + 8 * (m & 3) : 8 * m), desc_at(lo, hi, m * 2048), G::kIdescMn,
+             (accumulate || m > 0) ? 1u : 0u);
+  }
+  __syncwarp();
 }
 
 template <int D, bool F16>

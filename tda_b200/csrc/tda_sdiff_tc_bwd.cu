@@ -108,7 +108,7 @@ __device__ void kv_issue(uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32
   const uint32_t k = smem_u32(smem), v = k + C::kTileBytes, ring = smem_u32(smem + C::kOffRing);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok) ok = wait_inline(bar, parity, ctl, ST_KM);
+    if (ok) ok = wait_inline_warp(bar, parity, ctl, ST_KM);
     if (ok) tc_fence_after();
   };
   auto acquire = [&](int idx) {
@@ -120,13 +120,13 @@ __device__ void kv_issue(uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32
     const uint32_t q = acquire(2 * t);
     if (!ok) return;
     mma_score<D, F16>(tmem + C::kS, k, q);
-    tc_commit(&bars->s_full);
+    commit(&bars->s_full);
   };
   auto dprob = [&](int t) {  // dP^T(t) = V dout(t)^T
     const uint32_t g = acquire(2 * t + 1);
     if (!ok) return;
     mma_score<D, F16>(tmem + C::kP, v, g);
-    tc_commit(&bars->dp_full);
+    commit(&bars->dp_full);
   };
   wait(&bars->v_full, 0);
   for (int m = 0; m < 2 && ok; ++m) {
@@ -142,14 +142,14 @@ __device__ void kv_issue(uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32
       wait(&bars->ds_full, t & 1);
       if (!ok) break;
       mma_weights<D, F16, true>(tmem + C::kDK, tmem + C::kP, slot(2 * t), t > t0);
-      tc_commit(&bars->slot_empty[(2 * t) % C::kSlots]);
-      tc_commit(&bars->slot_empty[(2 * t + 1) % C::kSlots]);
+      commit(&bars->slot_empty[(2 * t) % C::kSlots]);
+      commit(&bars->slot_empty[(2 * t + 1) % C::kSlots]);
       if (t + 1 < t1) dprob(t + 1);
     }
-    if (ok) tc_commit(&bars->map_done);
+    if (ok) commit(&bars->map_done);
   }
   if (!ok) {
-    tc_commit(&bars->drain);
+    commit(&bars->drain);
     drain_wait(&bars->drain, 0, ctl);
   }
 }
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
   } else {
     fewer_registers<kFewRegs>();
     if (w.per_map > 0 && warp == 8 && lane == 0) kv_produce<D, F16>(tp, smem, bars, ctl, w, table, pad);
-    if (w.per_map > 0 && warp == 9 && lane == 0) kv_issue<D, F16>(smem, bars, ctl, tmem, w.per_map);
+    if (w.per_map > 0 && warp == 9) kv_issue<D, F16>(smem, bars, ctl, uniform(tmem), w.per_map);
     __syncwarp();
   }
   tc_fence_before();
@@ -415,7 +415,7 @@ __device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t
   const uint32_t q = smem_u32(smem), g = q + C::kTileBytes, ring = smem_u32(smem + C::kOffRing);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok) ok = wait_inline(bar, parity, ctl, ST_QM);
+    if (ok) ok = wait_inline_warp(bar, parity, ctl, ST_QM);
     if (ok) tc_fence_after();
   };
   auto acquire = [&](int idx) {
@@ -426,14 +426,14 @@ __device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t
     const uint32_t k = acquire(2 * t);
     if (!ok) return;
     mma_score<D, F16>(tmem + C::s_col(t), q, k);
-    tc_commit(&bars->s_full[t & 1]);
+    commit(&bars->s_full[t & 1]);
   };
   auto dprob = [&](int t) {
     const uint32_t v = acquire(2 * t + 1);
     if (!ok) return;
     mma_score<D, F16>(tmem + C::kP, g, v);
-    tc_commit(&bars->slot_empty[(2 * t + 1) % C::kSlots]);
-    tc_commit(&bars->dp_full);
+    commit(&bars->slot_empty[(2 * t + 1) % C::kSlots]);
+    commit(&bars->dp_full);
   };
   wait(&bars->q_full, 0);
   score(0);
@@ -447,13 +447,13 @@ __device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t
     wait(&bars->ds_full[t & 1], (t >> 1) & 1);
     if (!ok) break;
     mma_weights<D, F16, true>(tmem + C::kDQ, tmem + C::s_col(t), ring + ((2 * t) % C::kSlots) * C::kTileBytes, t > 0);
-    tc_commit(&bars->slot_empty[(2 * t) % C::kSlots]);
+    commit(&bars->slot_empty[(2 * t) % C::kSlots]);
     if (t + 2 < n) score(t + 2);
   }
   if (ok) {
-    tc_commit(&bars->o_full);
+    commit(&bars->o_full);
   } else {
-    tc_commit(&bars->drain);
+    commit(&bars->drain);
     drain_wait(&bars->drain, 0, ctl);
   }
 }
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
   } else {
     fewer_registers<kFewRegs>();
     if (n > 0 && warp == 8 && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, m, b, h, kvh, qt, n);
-    if (n > 0 && warp == 9 && lane == 0) q_issue<D, F16>(smem, bars, ctl, tmem, n);
+    if (n > 0 && warp == 9) q_issue<D, F16>(smem, bars, ctl, uniform(tmem), n);
     __syncwarp();
   }
   tc_fence_before();

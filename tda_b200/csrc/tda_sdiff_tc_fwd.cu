@@ -87,7 +87,7 @@ __device__ void issue(uint8_t* smem, FBars* bars, const WaitCtl& ctl, uint32_t t
   const uint32_t q = smem_u32(smem), ring = smem_u32(smem + C::kOffRing);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ok) ok = wait_inline(bar, parity, ctl, ST_MMA);
+    if (ok) ok = wait_inline_warp(bar, parity, ctl, ST_MMA);
     if (ok) tc_fence_after();
   };
   auto acquire = [&](int idx) {
@@ -98,8 +98,8 @@ __device__ void issue(uint8_t* smem, FBars* bars, const WaitCtl& ctl, uint32_t t
     const uint32_t k = acquire(3 * j + m);
     if (!ok) return;
     mma_score<D, F16>(tmem + C::s_col(m), q + m * C::kTileBytes, k);
-    tc_commit(&bars->slot_empty[(3 * j + m) % C::kSlots]);
-    tc_commit(&bars->s_full[m]);
+    commit(&bars->slot_empty[(3 * j + m) % C::kSlots]);
+    commit(&bars->s_full[m]);
   };
   wait(&bars->q_full, 0);
   score(0, 0);
@@ -114,14 +114,14 @@ __device__ void issue(uint8_t* smem, FBars* bars, const WaitCtl& ctl, uint32_t t
       wait(&bars->p_full[m], j & 1);
       if (!ok) break;
       mma_weights<D, F16, false, 4, 8>(tmem + C::o_col(m), tmem + C::s_col(m), v, true);
-      if (m == 1) tc_commit(&bars->slot_empty[(3 * j + 2) % C::kSlots]);
+      if (m == 1) commit(&bars->slot_empty[(3 * j + 2) % C::kSlots]);
       if (j + 1 < n) score(m, j + 1);
     }
   }
   if (ok) {
-    tc_commit(&bars->o_full);
+    commit(&bars->o_full);
   } else {
-    tc_commit(&bars->drain);
+    commit(&bars->drain);
     drain_wait(&bars->drain, 0, ctl);
   }
 }
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_fwd_kernel(const __grid_
   } else {
     fewer_registers<kFewRegs>();
     if (n > 0 && warp == 8 && lane == 0) produce<D, F16>(tp, smem, bars, ctl, b, h, kvh, qt, n);
-    if (n > 0 && warp == 9 && lane == 0) issue<D, F16>(smem, bars, ctl, tmem, n);
+    if (n > 0 && warp == 9) issue<D, F16>(smem, bars, ctl, uniform(tmem), n);
     __syncwarp();
   }
   tc_fence_before();
