@@ -76,10 +76,10 @@ __device__ __forceinline__ void mma_score(uint32_t dcol, uint32_t a, uint32_t b)
 }
 
 // D[dcol] (+)= W X: W [128][128] 16-bit in TMEM, X an MN-major tile of 128 rows.  W fills 64
-// columns, or (HALVES) 32 at wcol and 32 at wcol + 64: each half over the scores it came
-// from, so that the two warps that share a row's scores need not wait for one another.
+// columns, or (QUARTERS) 16 of each 32: each quarter over the scores it came from, so that
+// the four warps that share a row's scores need not wait for one another.
 // Rows [16 M0, 16 M1) of X alone: a part of the product, once a part of W is there.
-template <int D, bool F16, bool HALVES = false, int M0 = 0, int M1 = kTile / 16>
+template <int D, bool F16, bool QUARTERS = false, int M0 = 0, int M1 = kTile / 16>
 __device__ __forceinline__ void mma_weights(uint32_t dcol, uint32_t wcol, uint32_t x, bool accumulate) {
   using G = Geo<D, F16>;
   const uint64_t dx = smem_desc_sw128(x, G::kBoxBytes, 1024);
@@ -87,7 +87,7 @@ __device__ __forceinline__ void mma_weights(uint32_t dcol, uint32_t wcol, uint32
   if (elected()) {
 #pragma unroll
     for (int m = M0; m < M1; ++m)
-      mma_ts(dcol, wcol + (HALVES ? 64 * (m >> 2) + 8 * (m & 3) : 8 * m), desc_at(lo, hi, m * 2048), G::kIdescMn,
+      mma_ts(dcol, wcol + (QUARTERS ? 32 * (m >> 1) + 8 * (m & 1) : 8 * m), desc_at(lo, hi, m * 2048), G::kIdescMn,
              (accumulate || m > 0) ? 1u : 0u);
   }
   __syncwarp();

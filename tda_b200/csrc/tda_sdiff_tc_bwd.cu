@@ -9,7 +9,7 @@
 //     of the group, writes dK_1, then map 2's: dV sums both maps and all heads in TMEM.
 //   dq, a CTA a tile of 128 queries of one head and map:
 //     S = Q_m K_m^T, dP = dout V^T, dQ_m += dS K_m.
-// Eight warps hold the weights between the two halves of a step: while they
+// Sixteen warps (a row's 128 columns over four) hold the weights between the two halves of a step: while they
 // exponentiate S, the tensor cores run dK (dQ) of the last step and dP; while
 // they form dS, dV and the next S.  P and dS enter the products as one 16-bit
 // value each (2^-9 / 2^-12 of an element, averaged over a row); sums, the
@@ -23,11 +23,12 @@ namespace {
 
 using namespace sd;
 
-constexpr int kThreads = 384;  // warps 10 and 11 fill the third warpgroup
-// registers: 168 a thread at launch (64512); 128 x 72 + 256 x 216 = 64512
-constexpr int kFewRegs = 72, kManyRegs = 216;
+constexpr int kProd = 16, kIssue = 17;  // warps after the sixteen; two more fill their warpgroup
+constexpr int kThreads = 640;
+// registers: 96 a thread at launch (61440); 128 x 64 + 512 x 104 = 61440
+constexpr int kFewRegs = 64, kManyRegs = 104;
 constexpr int kPolyPairs = 3;  // of 8 go to the FMA pipe instead of the exponential unit
-constexpr int kWorkThreads = 256;
+constexpr int kWorkThreads = 512;
 constexpr int kTab = 4;
 constexpr int ST_KP = 0x901, ST_KM = 0x902, ST_KW = 0x903, ST_QP = 0xa01, ST_QM = 0xa02, ST_QW = 0xa03;
 
@@ -158,7 +159,7 @@ __device__ void kv_issue(uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32
 template <int D, bool F16>
 __device__ __forceinline__ void stage_accumulator(uint8_t* boxes, uint32_t col, int row, int wg, float scale, bool zero) {
 #pragma unroll
-  for (int x = wg * (D / 2); x < (wg + 1) * (D / 2); x += 32) {
+  for (int x = 32 * wg; x < D; x += 128) {
     float a[32];
     if (!zero) {
       uint32_t u[32];
@@ -174,6 +175,15 @@ __device__ __forceinline__ void stage_accumulator(uint8_t* boxes, uint32_t col, 
   }
 }
 
+// a thread's 32 weights as 16-bit values in the first 16 of its 32 columns
+template <bool F16>
+__device__ __forceinline__ void store_weights(uint32_t col, const float (&x)[32]) {
+  uint32_t u[16];
+#pragma unroll
+  for (int y = 0; y < 16; ++y) u[y] = pack2<F16>(x[2 * y], x[2 * y + 1]);
+  tmem_st16(col, u);
+}
+
 template <int D, bool F16>
 __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32_t tmem, const KvWork& w, int len,
                         int warp, int lane) {
@@ -181,7 +191,7 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
   const SdParams& p = tp.p;
   const int wg = warp >> 2, row = (warp & 3) * 32 + lane, key = w.kt * kTile + row, off = p.Sk - p.Sq;
   const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-  const uint32_t s_col = tmem + lane_off + C::kS + 64 * wg, p_col = tmem + lane_off + C::kP + 64 * wg;
+  const uint32_t s_col = tmem + lane_off + C::kS + 32 * wg, p_col = tmem + lane_off + C::kP + 32 * wg;
   const bool dead = key >= len;          // past the sequence's length: no weight, whatever K and V hold there
   const bool lone = len <= 1;            // weight 1 whatever the score: no dS
   const float c = p.c;
@@ -197,43 +207,33 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
         if (ok) ok = wait_inline_warp(&bars->s_full, t & 1, ctl, ST_KW);
         if (!ok) break;
         tc_fence_after();
-        const float4* tab = reinterpret_cast<const float4*>(smem + C::kOffTab + e * kTile * 8) + 16 * wg;
+        const float4* tab = reinterpret_cast<const float4*>(smem + C::kOffTab + e * kTile * 8) + 8 * wg;
         const bool masked = (w.kt + 1) * kTile > len || (p.causal && i * kTile + off < (w.kt + 1) * kTile - 1) || lone;
         // queries of this tile in front of `lo` do not see the key
         const int lo = dead ? kTile : (p.causal ? key - off - i * kTile : 0);
-        float pr[64];
+        float pr[32];
         {
-          uint32_t s[2][32];
-          tmem_ld32(s_col, s[0]);
-          tmem_ld32(s_col + 32, s[1]);
+          uint32_t s[32];
+          tmem_ld32(s_col, s);
           tmem_wait_ld();
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+          for (int y = 0; y < 32; y += 4) {
+            const float4 q = tab[y / 4];  // L of four queries
 #pragma unroll
-            for (int y = 0; y < 32; y += 4) {
-              const float4 q = tab[8 * x + y / 4];  // L of four queries
-#pragma unroll
-              for (int i = 0; i < 4; i += 2) {
-                const float2 z = __ffma2_rn(f2u(s[x][y + i], s[x][y + i + 1]), make_float2(c, c),
-                                            i ? make_float2(-q.z, -q.w) : make_float2(-q.x, -q.y));
-                const float2 ez = ((y + i) / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
-                const float2 r = __fmul2_rn(ez, make_float2(wt, wt));
-                pr[32 * x + y + i] = r.x;
-                pr[32 * x + y + i + 1] = r.y;
-              }
+            for (int i = 0; i < 4; i += 2) {
+              const float2 z = __ffma2_rn(f2u(s[y + i], s[y + i + 1]), make_float2(c, c), i ? make_float2(-q.z, -q.w) : make_float2(-q.x, -q.y));
+              const float2 ez = ((y + i) / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
+              const float2 r = __fmul2_rn(ez, make_float2(wt, wt));
+              pr[y + i] = r.x;
+              pr[y + i + 1] = r.y;
             }
+          }
         }
         if (masked) {
 #pragma unroll
-          for (int y = 0; y < 64; ++y) pr[y] = 64 * wg + y >= lo ? pr[y] : 0.f;
+          for (int y = 0; y < 32; ++y) pr[y] = 32 * wg + y >= lo ? pr[y] : 0.f;
         }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          uint32_t u[16];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) u[y] = pack2<F16>(pr[32 * x + 2 * y], pr[32 * x + 2 * y + 1]);
-          tmem_st16(s_col + 16 * x, u);
-        }
+        store_weights<F16>(s_col, pr);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -243,35 +243,26 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
         if (!ok) break;
         tc_fence_after();
         {
-          uint32_t s[2][32];
-          tmem_ld32(p_col, s[0]);
-          tmem_ld32(p_col + 32, s[1]);
+          uint32_t s[32];
+          tmem_ld32(p_col, s);
           tmem_wait_ld();
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+          for (int y = 0; y < 32; y += 4) {
+            const float4 q = tab[32 + y / 4];  // D of four queries
 #pragma unroll
-            for (int y = 0; y < 32; y += 4) {
-              const float4 q = tab[32 + 8 * x + y / 4];  // D of four queries
-#pragma unroll
-              for (int i = 0; i < 4; i += 2) {
-                const float2 d = __fadd2_rn(f2u(s[x][y + i], s[x][y + i + 1]), i ? make_float2(-q.z, -q.w) : make_float2(-q.x, -q.y));
-                const float2 r = __fmul2_rn(make_float2(pr[32 * x + y + i], pr[32 * x + y + i + 1]), d);
-                pr[32 * x + y + i] = r.x;
-                pr[32 * x + y + i + 1] = r.y;
-              }
+            for (int i = 0; i < 4; i += 2) {
+              const float2 d = __fadd2_rn(f2u(s[y + i], s[y + i + 1]), i ? make_float2(-q.z, -q.w) : make_float2(-q.x, -q.y));
+              const float2 r = __fmul2_rn(make_float2(pr[y + i], pr[y + i + 1]), d);
+              pr[y + i] = r.x;
+              pr[y + i + 1] = r.y;
             }
+          }
         }
         if (masked) {
 #pragma unroll
-          for (int y = 0; y < 64; ++y) pr[y] = 64 * wg + y >= lo && !lone ? pr[y] : 0.f;
+          for (int y = 0; y < 32; ++y) pr[y] = 32 * wg + y >= lo && !lone ? pr[y] : 0.f;
         }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          uint32_t u[16];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) u[y] = pack2<F16>(pr[32 * x + 2 * y], pr[32 * x + 2 * y + 1]);
-          tmem_st16(p_col + 16 * x, u);
-        }
+        store_weights<F16>(p_col, pr);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -325,20 +316,20 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
   if (threadIdx.x == 0) {
     uint64_t* one[] = {&bars->k_full, &bars->v_full, &bars->k_free, &bars->s_full, &bars->dp_full, &bars->map_done, &bars->drain};
     for (uint64_t* x : one) mbar_init(x, 1);
-    mbar_init(&bars->p_full, 8);
-    mbar_init(&bars->ds_full, 8);
+    mbar_init(&bars->p_full, 16);
+    mbar_init(&bars->ds_full, 16);
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&bars->slot_full[i], 1);
       mbar_init(&bars->slot_empty[i], 1);
     }
     for (int i = 0; i < kTab; ++i) {
       mbar_init(&bars->tab_full[i], 1);
-      mbar_init(&bars->tab_empty[i], 8);
+      mbar_init(&bars->tab_empty[i], 16);
     }
     bars->abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kIssue) {
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
@@ -347,18 +338,18 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   const WaitCtl ctl = make_wait_ctl(&bars->abort_flag, tp.status, tp.timeout_ns);
-  if (warp < 8) {
+  if (warp < kProd) {
     more_registers<kManyRegs>();
     kv_work<D, F16>(tp, smem, bars, ctl, tmem, w, len, warp, lane);
   } else {
     fewer_registers<kFewRegs>();
-    if (w.per_map > 0 && warp == 8 && lane == 0) kv_produce<D, F16>(tp, smem, bars, ctl, w, table, pad);
-    if (w.per_map > 0 && warp == 9) kv_issue<D, F16>(smem, bars, ctl, uniform(tmem), w.per_map);
+    if (w.per_map > 0 && warp == kProd && lane == 0) kv_produce<D, F16>(tp, smem, bars, ctl, w, table, pad);
+    if (w.per_map > 0 && warp == kIssue) kv_issue<D, F16>(smem, bars, ctl, uniform(tmem), w.per_map);
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kIssue) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -474,62 +465,50 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
     ok = wait_inline_warp(&bars->s_full[t & 1], (t >> 1) & 1, ctl, ST_QW);
     if (!ok) break;
     tc_fence_after();
-    const uint32_t s_col = tmem + lane_off + C::s_col(t);
+    const uint32_t s_col = tmem + lane_off + C::s_col(t) + 32 * wg;
     const bool masked = (t + 1) * kTile > len || (p.causal && (t + 1) * kTile - 1 > qt * kTile + off);
-    float pr[64];
+    float pr[32];
     {
-      uint32_t s[2][32];
-      tmem_ld32(s_col + 64 * wg, s[0]);
-      tmem_ld32(s_col + 64 * wg + 32, s[1]);
+      uint32_t s[32];
+      tmem_ld32(s_col, s);
       tmem_wait_ld();
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 32; y += 2) {
-          const float2 z = __ffma2_rn(f2u(s[x][y], s[x][y + 1]), make_float2(c, c), make_float2(-L, -L));
-          const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
-          pr[32 * x + y] = ez.x;
-          pr[32 * x + y + 1] = ez.y;
-        }
+      for (int y = 0; y < 32; y += 2) {
+        const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(-L, -L));
+        const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
+        pr[y] = ez.x;
+        pr[y + 1] = ez.y;
+      }
     }
     ok = wait_inline_warp(&bars->dp_full, t & 1, ctl, ST_QW);
     if (!ok) break;
     tc_fence_after();
     {
-      uint32_t s[2][32];
-      tmem_ld32(tmem + lane_off + C::kP + 64 * wg, s[0]);
-      tmem_ld32(tmem + lane_off + C::kP + 64 * wg + 32, s[1]);
+      uint32_t s[32];
+      tmem_ld32(tmem + lane_off + C::kP + 32 * wg, s);
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->dp_free);
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int y = 0; y < 32; y += 2) {
-          const float2 d = __fadd2_rn(f2u(s[x][y], s[x][y + 1]), make_float2(-del, -del));
-          const float2 r = __fmul2_rn(make_float2(pr[32 * x + y], pr[32 * x + y + 1]), d);
-          pr[32 * x + y] = r.x;
-          pr[32 * x + y + 1] = r.y;
-        }
+      for (int y = 0; y < 32; y += 2) {
+        const float2 d = __fadd2_rn(f2u(s[y], s[y + 1]), make_float2(-del, -del));
+        const float2 r = __fmul2_rn(make_float2(pr[y], pr[y + 1]), d);
+        pr[y] = r.x;
+        pr[y + 1] = r.y;
+      }
     }
     if (masked) {
-      const int lim = last - t * kTile - 64 * wg;
+      const int lim = last - t * kTile - 32 * wg;
 #pragma unroll
-      for (int y = 0; y < 64; ++y) pr[y] = y <= lim ? pr[y] : 0.f;
+      for (int y = 0; y < 32; ++y) pr[y] = y <= lim ? pr[y] : 0.f;
     }
     // K rows past the length: zeroed (S is done with them) before the product with dS reads them
     if (t == n - 1 && len < p.Sk && (t + 1) * kTile > len) {
       if (wg == 0 && t * kTile + row >= len) zero_row<D>(smem + C::kOffRing + ((2 * t) % C::kSlots) * C::kTileBytes, row);
       fence_proxy_async_smem();
     }
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      uint32_t u[16];
-#pragma unroll
-      for (int y = 0; y < 16; ++y) u[y] = pack2<F16>(pr[32 * x + 2 * y], pr[32 * x + 2 * y + 1]);
-      tmem_st16(s_col + 64 * wg + 16 * x, u);
-    }
+    store_weights<F16>(s_col, pr);
     tmem_wait_st();
     tc_fence_before();
     __syncwarp();
@@ -573,10 +552,10 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
     mbar_init(&bars->o_full, 1);
     mbar_init(&bars->drain, 1);
     mbar_init(&bars->dp_full, 1);
-    mbar_init(&bars->dp_free, 8);
+    mbar_init(&bars->dp_free, 16);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
-      mbar_init(&bars->ds_full[i], 8);
+      mbar_init(&bars->ds_full[i], 16);
     }
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&bars->slot_full[i], 1);
@@ -585,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
     bars->abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kIssue) {
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
@@ -594,18 +573,18 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   const WaitCtl ctl = make_wait_ctl(&bars->abort_flag, tp.status, tp.timeout_ns);
-  if (warp < 8) {
+  if (warp < kProd) {
     more_registers<kManyRegs>();
     q_work<D, F16>(tp, smem, bars, ctl, tmem, table, pad, m, b, h, qt, n, len, warp, lane);
   } else {
     fewer_registers<kFewRegs>();
-    if (n > 0 && warp == 8 && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, m, b, h, kvh, qt, n);
-    if (n > 0 && warp == 9) q_issue<D, F16>(smem, bars, ctl, uniform(tmem), n);
+    if (n > 0 && warp == kProd && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, m, b, h, kvh, qt, n);
+    if (n > 0 && warp == kIssue) q_issue<D, F16>(smem, bars, ctl, uniform(tmem), n);
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kIssue) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
