@@ -38,7 +38,7 @@ struct SdParams {
   float c;         // scale log2(e)
   // backward
   SdView dout;
-  float* table;    // [2][B][H][pad / 128][2][128]: L_m, then D_m of each row; +inf, 0 past Sq
+  float* table;    // [2][B][H][pad / 128][2][128]: -L_m, then -D_m of each row; -inf, 0 past Sq
   int pad;         // Sq rounded up to a tile of 128
   void* dq[2];     // contiguous, of the inputs' type
   void* dk[2];

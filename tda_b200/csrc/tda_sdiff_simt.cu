@@ -140,7 +140,7 @@ __device__ __forceinline__ long long row_at(const SdParams& p, int m, int b, int
   return ((static_cast<long long>(m) * p.B + b) * p.H + h) * p.Sq + i;
 }
 
-// L of row i of map m and (batch, head) bh; its D lies kTile behind
+// -L of row i of map m and (batch, head) bh; its -D lies kTile behind
 __device__ __forceinline__ long long table_at(const SdParams& p, int m, long long bh, int i) {
   return 2 * ((static_cast<long long>(m) * p.B * p.H + bh) * p.pad + i / kTile * kTile) + i % kTile;
 }
@@ -263,11 +263,11 @@ __global__ void __launch_bounds__(256) sdiff_delta_kernel(const SdParams p) {
   }
   if (row < rows && l == 0) {
     float* t = p.table + table_at(p, 0, bh, i);
-    t[0] = i < p.Sq ? p.lse[at] : kInf;
-    t[kTile] = a;
+    t[0] = i < p.Sq ? -p.lse[at] : -kInf;
+    t[kTile] = -a;
     t += 2 * rows;
-    t[0] = i < p.Sq ? p.lse[all + at] : kInf;
-    t[kTile] = c;
+    t[0] = i < p.Sq ? -p.lse[all + at] : -kInf;
+    t[kTile] = -c;
   }
 }
 
@@ -276,14 +276,14 @@ __global__ void __launch_bounds__(256) sdiff_dlam_kernel(const SdParams p) {
   __shared__ float part[256];
   const long long bh = blockIdx.x;
   float s = 0.f;
-  for (int i = threadIdx.x; i < p.Sq; i += 256) s += p.table[table_at(p, 1, bh, i) + kTile];
+  for (int i = threadIdx.x; i < p.Sq; i += 256) s += p.table[table_at(p, 1, bh, i) + kTile];  // -D_2
   part[threadIdx.x] = s;
   __syncthreads();
   for (int o = 128; o > 0; o >>= 1) {
     if (threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
     __syncthreads();
   }
-  if (threadIdx.x == 0) p.dlam[bh] = -part[0];
+  if (threadIdx.x == 0) p.dlam[bh] = part[0];
 }
 
 // dq of one map and tile of queries
@@ -307,8 +307,8 @@ __global__ void __launch_bounds__(256) sdiff_simt_dq_kernel(const SdParams p) {
   for (int r = 0; r < C::R; ++r) {
     const int i = i0 + ty * C::R + r;
     const float* t = p.table + table_at(p, m, bh, min(i, p.Sq - 1));
-    lse[r] = i < p.Sq ? t[0] : kInf;
-    del[r] = t[kTile];
+    lse[r] = i < p.Sq ? -t[0] : kInf;
+    del[r] = -t[kTile];
 #pragma unroll
     for (int c = 0; c < C::C; ++c) o[r][c] = 0.f;
   }
@@ -377,8 +377,8 @@ __global__ void __launch_bounds__(256) sdiff_simt_dkv_kernel(const SdParams p) {
         if (threadIdx.x < C::BT) {
           const int i = i0 + threadIdx.x;
           const float* t = p.table + table_at(p, m, static_cast<long long>(b) * p.H + h, min(i, p.Sq - 1));
-          ls[threadIdx.x] = i < p.Sq ? t[0] : kInf;
-          es[threadIdx.x] = t[kTile];
+          ls[threadIdx.x] = i < p.Sq ? -t[0] : kInf;
+          es[threadIdx.x] = -t[kTile];
         }
         __syncthreads();
         float s[C::R][C::R], dp[C::R][C::R];

@@ -1,6 +1,6 @@
 // Backward of softmax differential attention on the tensor cores (tcgen05,
 // TMEM, TMA): bf16 or fp16, head_dim 64 / 128.  Formulas in tda_sdiff.h; row
-// table L_m(i), D_m(i) from the row-sum pass (rows past Sq: +inf, 0).
+// table -L_m(i), -D_m(i) from the row-sum pass (rows past Sq: -inf, 0).
 //
 // Two kernels, no atomic sums (the same bits every time):
 //   dkv, a CTA a tile of 128 keys of one kv head.  Rows are keys: per query tile
@@ -8,7 +8,8 @@
 //     P'_1 = P_1, P'_2 = -lambda P_2.  It walks map 1's query tiles of every head
 //     of the group, writes dK_1, then map 2's: dV sums both maps and all heads in TMEM.
 //   dq, a CTA a tile of 128 queries of one head and map:
-//     S = Q_m K_m^T, dP = dout V^T, dQ_m += dS K_m.
+//     S = Q_m K_m^T, dP = dout V^T, dQ_m += dS K_m, with Q_m and dout held in TMEM;
+//     dS replaces dP, so the next S needs S read, not used.
 // Sixteen warps (a row's 128 columns over four) hold the weights between the two halves of a step: while they
 // exponentiate S, the tensor cores run dK (dQ) of the last step and dP; while
 // they form dS, dV and the next S.  P and dS enter the products as one 16-bit
@@ -218,10 +219,10 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
           tmem_wait_ld();
 #pragma unroll
           for (int y = 0; y < 32; y += 4) {
-            const float4 q = tab[y / 4];  // L of four queries
+            const float4 q = tab[y / 4];  // -L of four queries
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-              const float2 z = __ffma2_rn(f2u(s[y + i], s[y + i + 1]), make_float2(c, c), i ? make_float2(-q.z, -q.w) : make_float2(-q.x, -q.y));
+              const float2 z = __ffma2_rn(f2u(s[y + i], s[y + i + 1]), make_float2(c, c), i ? make_float2(q.z, q.w) : make_float2(q.x, q.y));
               const float2 ez = ((y + i) / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
               const float2 r = __fmul2_rn(ez, make_float2(wt, wt));
               pr[y + i] = r.x;
@@ -248,10 +249,10 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
           tmem_wait_ld();
 #pragma unroll
           for (int y = 0; y < 32; y += 4) {
-            const float4 q = tab[32 + y / 4];  // D of four queries
+            const float4 q = tab[32 + y / 4];  // -D of four queries
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-              const float2 d = __fadd2_rn(f2u(s[y + i], s[y + i + 1]), i ? make_float2(-q.z, -q.w) : make_float2(-q.x, -q.y));
+              const float2 d = __fadd2_rn(f2u(s[y + i], s[y + i + 1]), i ? make_float2(q.z, q.w) : make_float2(q.x, q.y));
               const float2 r = __fmul2_rn(make_float2(pr[y + i], pr[y + i + 1]), d);
               pr[y + i] = r.x;
               pr[y + i + 1] = r.y;
@@ -364,13 +365,11 @@ struct QC : Geo<D, F16> {
   static constexpr int kOffBar = kOffRing + kSlots * G::kTileBytes;
   static constexpr int kSmem = kOffBar + 1024 + 1024;
   static_assert(kSmem <= kSmemBudget, "shared memory");
-  static __device__ __forceinline__ constexpr uint32_t s_col(int t) { return (t & 1) ? 128u : 0u; }
-  static constexpr uint32_t kP = 256, kDQ = 384;
+  static constexpr uint32_t kS = 0, kP = 128, kDQ = 256, kQ = 384, kG = 448;  // dS over dP; Q and dout as operands
 };
 
 struct QBars {
-  uint64_t q_full, o_full, drain, dp_full, dp_free;
-  uint64_t s_full[2], ds_full[2];
+  uint64_t q_full, ops_full, o_full, drain, s_full, s_free, dp_full, ds_full;
   uint64_t slot_full[8], slot_empty[8];
   uint32_t tmem_base;
   int abort_flag;
@@ -403,7 +402,7 @@ __device__ void q_produce(const SdTcParams& tp, uint8_t* smem, QBars* bars, cons
 template <int D, bool F16>
 __device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t tmem, int n) {
   using C = QC<D, F16>;
-  const uint32_t q = smem_u32(smem), g = q + C::kTileBytes, ring = smem_u32(smem + C::kOffRing);
+  const uint32_t ring = smem_u32(smem + C::kOffRing);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (ok) ok = wait_inline_warp(bar, parity, ctl, ST_QM);
@@ -416,30 +415,31 @@ __device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t
   auto score = [&](int t) {
     const uint32_t k = acquire(2 * t);
     if (!ok) return;
-    mma_score<D, F16>(tmem + C::s_col(t), q, k);
-    commit(&bars->s_full[t & 1]);
+    mma_score_ts<D, F16>(tmem + C::kS, tmem + C::kQ, k);
+    commit(&bars->s_full);
   };
   auto dprob = [&](int t) {
     const uint32_t v = acquire(2 * t + 1);
     if (!ok) return;
-    mma_score<D, F16>(tmem + C::kP, g, v);
+    mma_score_ts<D, F16>(tmem + C::kP, tmem + C::kG, v);
     commit(&bars->slot_empty[(2 * t + 1) % C::kSlots]);
     commit(&bars->dp_full);
   };
-  wait(&bars->q_full, 0);
-  score(0);
-  dprob(0);
-  if (n > 1) score(1);
+  wait(&bars->ops_full, 0);
+  if (ok) {
+    score(0);
+    dprob(0);
+  }
   for (int t = 0; t < n && ok; ++t) {
     if (t + 1 < n) {
-      wait(&bars->dp_free, t & 1);
-      dprob(t + 1);
+      wait(&bars->s_free, t & 1);
+      if (ok) score(t + 1);
     }
-    wait(&bars->ds_full[t & 1], (t >> 1) & 1);
+    wait(&bars->ds_full, t & 1);
     if (!ok) break;
-    mma_weights<D, F16, true>(tmem + C::kDQ, tmem + C::s_col(t), ring + ((2 * t) % C::kSlots) * C::kTileBytes, t > 0);
+    mma_weights<D, F16, true>(tmem + C::kDQ, tmem + C::kP, ring + ((2 * t) % C::kSlots) * C::kTileBytes, t > 0);
     commit(&bars->slot_empty[(2 * t) % C::kSlots]);
-    if (t + 2 < n) score(t + 2);
+    if (t + 1 < n) dprob(t + 1);
   }
   if (ok) {
     commit(&bars->o_full);
@@ -458,23 +458,37 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
   const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
   const long long bh = static_cast<long long>(b) * p.H + h;
   const float* row_tab = table + 2 * ((static_cast<long long>(m) * p.B * p.H + bh) * pad + qt * kTile) + row;
-  const float L = row_tab[0], del = row_tab[kTile], c = p.c;
+  const float minus_l = row_tab[0], minus_d = row_tab[kTile], c = p.c;
   const int last = p.causal ? min(len - 1, grow + off) : len - 1;
+  const uint32_t p_col = tmem + lane_off + C::kP + 32 * wg;
   bool ok = true;
-  for (int t = 0; t < n; ++t) {
-    ok = wait_inline_warp(&bars->s_full[t & 1], (t >> 1) & 1, ctl, ST_QW);
+  if (n > 0) {  // Q and dout become TMEM operands: a warpgroup a box of 64 columns
+    ok = wait_inline_warp(&bars->q_full, 0, ctl, ST_QW);
+    if (ok && wg < 2 * C::kBoxes) {
+      const int x = wg / C::kBoxes, box = wg % C::kBoxes;
+      tile_row_to_tmem(smem + x * C::kTileBytes + box * C::kBoxBytes, row, tmem + lane_off + (x ? C::kG : C::kQ) + 32 * box);
+      tmem_wait_st();
+      tc_fence_before();
+    }
+    __syncwarp();
+    if (ok && lane == 0) mbar_arrive(&bars->ops_full);
+  }
+  for (int t = 0; t < n && ok; ++t) {
+    ok = wait_inline_warp(&bars->s_full, t & 1, ctl, ST_QW);
     if (!ok) break;
     tc_fence_after();
-    const uint32_t s_col = tmem + lane_off + C::s_col(t) + 32 * wg;
     const bool masked = (t + 1) * kTile > len || (p.causal && (t + 1) * kTile - 1 > qt * kTile + off);
     float pr[32];
     {
       uint32_t s[32];
-      tmem_ld32(s_col, s);
+      tmem_ld32(tmem + lane_off + C::kS + 32 * wg, s);
       tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->s_free);
 #pragma unroll
       for (int y = 0; y < 32; y += 2) {
-        const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(-L, -L));
+        const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(minus_l, minus_l));
         const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
         pr[y] = ez.x;
         pr[y + 1] = ez.y;
@@ -485,14 +499,11 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
     tc_fence_after();
     {
       uint32_t s[32];
-      tmem_ld32(tmem + lane_off + C::kP + 32 * wg, s);
+      tmem_ld32(p_col, s);
       tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->dp_free);
 #pragma unroll
       for (int y = 0; y < 32; y += 2) {
-        const float2 d = __fadd2_rn(f2u(s[y], s[y + 1]), make_float2(-del, -del));
+        const float2 d = __fadd2_rn(f2u(s[y], s[y + 1]), make_float2(minus_d, minus_d));
         const float2 r = __fmul2_rn(make_float2(pr[y], pr[y + 1]), d);
         pr[y] = r.x;
         pr[y + 1] = r.y;
@@ -508,11 +519,11 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
       if (wg == 0 && t * kTile + row >= len) zero_row<D>(smem + C::kOffRing + ((2 * t) % C::kSlots) * C::kTileBytes, row);
       fence_proxy_async_smem();
     }
-    store_weights<F16>(s_col, pr);
+    store_weights<F16>(p_col, pr);
     tmem_wait_st();
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&bars->ds_full[t & 1]);
+    if (lane == 0) mbar_arrive(&bars->ds_full);
   }
   if (ok && n > 0) ok = wait_inline_warp(&bars->o_full, 0, ctl, ST_QW);
   tc_fence_after();
@@ -552,11 +563,10 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
     mbar_init(&bars->o_full, 1);
     mbar_init(&bars->drain, 1);
     mbar_init(&bars->dp_full, 1);
-    mbar_init(&bars->dp_free, 16);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->s_full[i], 1);
-      mbar_init(&bars->ds_full[i], 16);
-    }
+    mbar_init(&bars->s_full, 1);
+    mbar_init(&bars->ops_full, 16);
+    mbar_init(&bars->s_free, 16);
+    mbar_init(&bars->ds_full, 16);
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&bars->slot_full[i], 1);
       mbar_init(&bars->slot_empty[i], 1);
