@@ -18,6 +18,10 @@
 
 namespace tda {
 
+constexpr int kAuxTileBytes = 128 * 16 * 2;
+// fp16 holds -L / c up to 2^24 as a multiple of this
+constexpr float aux_unit(bool f16) { return f16 ? 256.0f : 1.0f; }
+
 struct SdView {  // (batch, head, seq, dim) view: element strides, dim contiguous
   const void* p;
   long long sb, sh, ss;
@@ -39,6 +43,10 @@ struct SdParams {
   // backward
   SdView dout;
   float* table;    // [2][B][H][pad / 128][2][128]: -L_m, then -D_m of each row; -inf, 0 past Sq
+  // The same numbers as products read them (16-bit types): per tile of 128 rows
+  // [128][16] for -L / c, then for -D, three values a row that add up to it over
+  // aux_unit, in core-matrix order.
+  void* aux;
   int pad;         // Sq rounded up to a tile of 128
   void* dq[2];     // contiguous, of the inputs' type
   void* dk[2];

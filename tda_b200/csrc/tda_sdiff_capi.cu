@@ -166,7 +166,8 @@ int tda_sdiff_fwd(const void* q1, const void* q2, const void* k1, const void* k2
 
 size_t tda_sdiff_bwd_workspace_size(int64_t batch, int64_t heads, int64_t q_len) {
   if (batch < 1 || heads < 1 || q_len < 1) return 0;
-  return 2 * static_cast<size_t>(batch) * heads * padded_seq(q_len) * 2 * sizeof(float);
+  // per map, head and padded row: two floats and two rows of 16 16-bit values
+  return 2 * static_cast<size_t>(batch) * heads * padded_seq(q_len) * (2 * sizeof(float) + 64);
 }
 
 int tda_sdiff_bwd(const void* q1, const void* q2, const void* k1, const void* k2, const void* v,
@@ -197,6 +198,7 @@ int tda_sdiff_bwd(const void* q1, const void* q2, const void* k1, const void* k2
   p.lse = const_cast<float*>(lse);
   p.table = static_cast<float*>(workspace);
   p.pad = static_cast<int>(padded_seq(q_len));
+  if (on_tensor_cores(dtype, head_dim)) p.aux = p.table + 4 * batch * heads * padded_seq(q_len);
   p.dq[0] = dq1;
   p.dq[1] = dq2;
   p.dk[0] = dk1;

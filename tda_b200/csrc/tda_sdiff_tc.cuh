@@ -123,6 +123,20 @@ __device__ __forceinline__ void mma_weights(uint32_t dcol, uint32_t wcol, uint32
   __syncwarp();
 }
 
+// One more step of 16 along the contracted dimension: D[dcol] += ones aux^T, with
+// `aux` a [128][16] table in shared memory (unswizzled: 8 x 16-byte core matrices,
+// 128 bytes apart along the columns, 256 along the rows) whose first three columns
+// add up to a number a row, and `ones` of the same form.  It subtracts L or D of
+// the query from a column of scores without a load in the threads that use them:
+// 16 shared-memory loads a thread and step cost more than the product.
+template <bool F16>
+__device__ __forceinline__ void mma_offsets(uint32_t dcol, uint32_t ones, uint32_t aux) {
+  constexpr uint64_t kForm = (static_cast<uint64_t>(128 >> 4) << 16) | (static_cast<uint64_t>(256 >> 4) << 32) | (1ull << 46);
+  if (elected())
+    mma_ss(dcol, kForm | ((ones >> 4) & 0x3FFFu), kForm | ((aux >> 4) & 0x3FFFu), idesc_f16(128, 128, !F16, false), 1u);
+  __syncwarp();
+}
+
 template <int D, bool F16>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int h, int b) {
   using G = Geo<D, F16>;

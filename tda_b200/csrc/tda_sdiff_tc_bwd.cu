@@ -5,7 +5,7 @@
 // Two kernels, no atomic sums (the same bits every time):
 //   dkv, a CTA a tile of 128 keys of one kv head.  Rows are keys: per query tile
 //     S^T = K_m Q_m^T, dP^T = V dout^T, then dV += P'^T dout, dK_m += dS^T Q_m,
-//     P'_1 = P_1, P'_2 = -lambda P_2.  It walks map 1's query tiles of every head
+//     P'_1 = P_1, P'_2 = -lambda P_2 (L and D are subtracted by the products).  It walks map 1's query tiles of every head
 //     of the group, writes dK_1, then map 2's: dV sums both maps and all heads in TMEM.
 //   dq, a CTA a tile of 128 queries of one head and map:
 //     S = Q_m K_m^T, dP = dout V^T, dQ_m += dS K_m, with Q_m and dout held in TMEM;
@@ -30,7 +30,7 @@ constexpr int kThreads = 640;
 constexpr int kFewRegs = 64, kManyRegs = 104;
 constexpr int kPolyPairs = 3;  // of 8 go to the FMA pipe instead of the exponential unit
 constexpr int kWorkThreads = 512;
-constexpr int kTab = 4;
+constexpr int kTab = 2;
 constexpr int ST_KP = 0x901, ST_KM = 0x902, ST_KW = 0x903, ST_QP = 0xa01, ST_QM = 0xa02, ST_QW = 0xa03;
 
 template <int D, bool F16>
@@ -38,8 +38,10 @@ struct KvC : Geo<D, F16> {
   using G = Geo<D, F16>;
   static constexpr int kSlots = 4;
   static constexpr int kOffRing = 2 * G::kTileBytes;  // K, V, then the Q / dout ring
-  static constexpr int kOffTab = kOffRing + kSlots * G::kTileBytes;
-  static constexpr int kOffBar = kOffTab + kTab * kTile * 8;
+  static constexpr int kOffTab = kOffRing + kSlots * G::kTileBytes;  // L and D tables of a step, kTab steps
+  static constexpr int kTabBytes = 2 * kAuxTileBytes;
+  static constexpr int kOffOnes = kOffTab + kTab * kTabBytes;
+  static constexpr int kOffBar = kOffOnes + kAuxTileBytes;
   static constexpr int kSmem = kOffBar + 1024 + 1024;
   static_assert(kSmem <= kSmemBudget, "shared memory");
   static constexpr uint32_t kS = 0, kP = 128, kDV = 256, kDK = 384;
@@ -57,8 +59,7 @@ struct KvWork {
 };
 
 template <int D, bool F16>
-__device__ void kv_produce(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const WaitCtl& ctl, const KvWork& w, const float* table,
-                           int pad) {
+__device__ void kv_produce(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const WaitCtl& ctl, const KvWork& w) {
   using C = KvC<D, F16>;
   const SdParams& p = tp.p;
   mbar_arrive_expect_tx(&bars->v_full, C::kTileBytes);
@@ -76,9 +77,10 @@ __device__ void kv_produce(const SdTcParams& tp, uint8_t* smem, KvBars* bars, co
         const int e = t % kTab;
         ok = wait_inline(&bars->tab_empty[e], ((t / kTab) & 1) ^ 1, ctl, ST_KP);
         if (!ok) break;
-        mbar_arrive_expect_tx(&bars->tab_full[e], kTile * 8);
-        const long long row = (static_cast<long long>(m) * p.B + w.b) * p.H + h;
-        bulk_load(smem + C::kOffTab + e * kTile * 8, table + 2 * (row * pad + i * kTile), kTile * 8, &bars->tab_full[e]);
+        mbar_arrive_expect_tx(&bars->tab_full[e], C::kTabBytes);
+        const long long tile = ((static_cast<long long>(m) * p.B + w.b) * p.H + h) * (p.pad / kTile) + i;
+        bulk_load(smem + C::kOffTab + e * C::kTabBytes, static_cast<const uint8_t*>(p.aux) + tile * C::kTabBytes, C::kTabBytes,
+                  &bars->tab_full[e]);
         for (int x = 0; x < 2; ++x) {
           const int slot = idx % C::kSlots;
           ok = wait_inline(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_KP);
@@ -108,6 +110,7 @@ template <int D, bool F16>
 __device__ void kv_issue(uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32_t tmem, int per_map) {
   using C = KvC<D, F16>;
   const uint32_t k = smem_u32(smem), v = k + C::kTileBytes, ring = smem_u32(smem + C::kOffRing);
+  const uint32_t tab = smem_u32(smem + C::kOffTab), ones = smem_u32(smem + C::kOffOnes);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (ok) ok = wait_inline_warp(bar, parity, ctl, ST_KM);
@@ -120,14 +123,18 @@ __device__ void kv_issue(uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32
   auto slot = [&](int idx) { return ring + (idx % C::kSlots) * C::kTileBytes; };
   auto score = [&](int t) {  // S^T(t) = K Q(t)^T
     const uint32_t q = acquire(2 * t);
+    wait(&bars->tab_full[t % kTab], (t / kTab) & 1);
     if (!ok) return;
     mma_score<D, F16>(tmem + C::kS, k, q);
+    mma_offsets<F16>(tmem + C::kS, ones, tab + (t % kTab) * C::kTabBytes);
     commit(&bars->s_full);
   };
   auto dprob = [&](int t) {  // dP^T(t) = V dout(t)^T
     const uint32_t g = acquire(2 * t + 1);
     if (!ok) return;
     mma_score<D, F16>(tmem + C::kP, v, g);
+    mma_offsets<F16>(tmem + C::kP, ones, tab + (t % kTab) * C::kTabBytes + kAuxTileBytes);
+    commit(&bars->tab_empty[t % kTab]);
     commit(&bars->dp_full);
   };
   wait(&bars->v_full, 0);
@@ -203,12 +210,9 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
     for (int h = w.kvh * p.group; h < (w.kvh + 1) * p.group && ok; ++h) {
       const float wt = m ? -lambda_at(p.lam, w.b, h) : 1.0f;
       for (int i = w.i0; i < tp.n_qt && w.per_map > 0; ++i, ++t) {
-        const int e = t % kTab;
-        ok = wait_inline_warp(&bars->tab_full[e], (t / kTab) & 1, ctl, ST_KW);
-        if (ok) ok = wait_inline_warp(&bars->s_full, t & 1, ctl, ST_KW);
+        ok = wait_inline_warp(&bars->s_full, t & 1, ctl, ST_KW);
         if (!ok) break;
         tc_fence_after();
-        const float4* tab = reinterpret_cast<const float4*>(smem + C::kOffTab + e * kTile * 8) + 8 * wg;
         const bool masked = (w.kt + 1) * kTile > len || (p.causal && i * kTile + off < (w.kt + 1) * kTile - 1) || lone;
         // queries of this tile in front of `lo` do not see the key
         const int lo = dead ? kTile : (p.causal ? key - off - i * kTile : 0);
@@ -218,16 +222,12 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
           tmem_ld32(s_col, s);
           tmem_wait_ld();
 #pragma unroll
-          for (int y = 0; y < 32; y += 4) {
-            const float4 q = tab[y / 4];  // -L of four queries
-#pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              const float2 z = __ffma2_rn(f2u(s[y + i], s[y + i + 1]), make_float2(c, c), i ? make_float2(q.z, q.w) : make_float2(q.x, q.y));
-              const float2 ez = ((y + i) / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
-              const float2 r = __fmul2_rn(ez, make_float2(wt, wt));
-              pr[y + i] = r.x;
-              pr[y + i + 1] = r.y;
-            }
+          for (int y = 0; y < 32; y += 2) {
+            const float2 z = __fmul2_rn(f2u(s[y], s[y + 1]), make_float2(c, c));  // s - L / c
+            const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
+            const float2 r = __fmul2_rn(ez, make_float2(wt, wt));
+            pr[y] = r.x;
+            pr[y + 1] = r.y;
           }
         }
         if (masked) {
@@ -248,15 +248,10 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
           tmem_ld32(p_col, s);
           tmem_wait_ld();
 #pragma unroll
-          for (int y = 0; y < 32; y += 4) {
-            const float4 q = tab[32 + y / 4];  // -D of four queries
-#pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              const float2 d = __fadd2_rn(f2u(s[y + i], s[y + i + 1]), i ? make_float2(q.z, q.w) : make_float2(q.x, q.y));
-              const float2 r = __fmul2_rn(make_float2(pr[y + i], pr[y + i + 1]), d);
-              pr[y + i] = r.x;
-              pr[y + i + 1] = r.y;
-            }
+          for (int y = 0; y < 32; y += 2) {
+            const float2 r = __fmul2_rn(make_float2(pr[y], pr[y + 1]), f2u(s[y], s[y + 1]));  // P (dP - D)
+            pr[y] = r.x;
+            pr[y + 1] = r.y;
           }
         }
         if (masked) {
@@ -267,10 +262,7 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars->ds_full);
-          mbar_arrive(&bars->tab_empty[e]);
-        }
+        if (lane == 0) mbar_arrive(&bars->ds_full);
       }
     }
     // dK_m through the K buffer (idle once every product of the map is done), and dV through V's at the end
@@ -299,7 +291,7 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
 }
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_constant__ SdTcParams tp, const float* table, int pad) {
+__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_constant__ SdTcParams tp) {
   using C = KvC<D, F16>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -325,10 +317,18 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
     }
     for (int i = 0; i < kTab; ++i) {
       mbar_init(&bars->tab_full[i], 1);
-      mbar_init(&bars->tab_empty[i], 16);
+      mbar_init(&bars->tab_empty[i], 1);
     }
     bars->abort_flag = 0;
     fence_mbar_init();
+  }
+  if (threadIdx.x >= 128 && threadIdx.x < 256) {  // the unit in three columns of every row
+    const int r = threadIdx.x - 128;
+    const uint32_t u = pack2<F16>(aux_unit(F16), aux_unit(F16));
+    uint4* at = reinterpret_cast<uint4*>(smem + C::kOffOnes + (r >> 3) * 256 + (r & 7) * 16);
+    at[0] = make_uint4(u, u & 0xffffu, 0, 0);
+    at[8] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
   }
   if (warp == kIssue) {
     tmem_alloc(&bars->tmem_base, 512);
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
     kv_work<D, F16>(tp, smem, bars, ctl, tmem, w, len, warp, lane);
   } else {
     fewer_registers<kFewRegs>();
-    if (w.per_map > 0 && warp == kProd && lane == 0) kv_produce<D, F16>(tp, smem, bars, ctl, w, table, pad);
+    if (w.per_map > 0 && warp == kProd && lane == 0) kv_produce<D, F16>(tp, smem, bars, ctl, w);
     if (w.per_map > 0 && warp == kIssue) kv_issue<D, F16>(smem, bars, ctl, uniform(tmem), w.per_map);
     __syncwarp();
   }
@@ -606,7 +606,7 @@ cudaError_t launch(const SdTcParams& tp, const float* table, int pad, cudaStream
   auto kk = sdiff_tc_dkv_kernel<D, F16>;
   if (cudaError_t e = allow_shared<sdiff_tc_dq_kernel<D, F16>>(QC<D, F16>::kSmem)) return e;
   if (cudaError_t e = allow_shared<sdiff_tc_dkv_kernel<D, F16>>(KvC<D, F16>::kSmem)) return e;
-  kk<<<static_cast<unsigned>(tp.p.B * tp.p.Hkv * tp.n_kt), kThreads, KvC<D, F16>::kSmem, s>>>(tp, table, pad);
+  kk<<<static_cast<unsigned>(tp.p.B * tp.p.Hkv * tp.n_kt), kThreads, KvC<D, F16>::kSmem, s>>>(tp);
   if (cudaError_t e = cudaGetLastError()) return e;
   kq<<<static_cast<unsigned>(2 * tp.p.B * tp.p.H * tp.n_qt), kThreads, QC<D, F16>::kSmem, s>>>(tp, table, pad);
   return cudaGetLastError();

@@ -40,9 +40,9 @@ def test_forward_refuses_strides():
 def test_backward_refuses():
     lib = _lib.load()
     ws = lib.tda_sdiff_bwd_workspace_size(2, 3, 100)
-    assert ws == 2 * 2 * 3 * 128 * 8 and lib.tda_sdiff_bwd_workspace_size(0, 3, 100) == 0
+    assert ws == 2 * 2 * 3 * 128 * 72 and lib.tda_sdiff_bwd_workspace_size(0, 3, 100) == 0
 
-    def call(dout=16, ds=None, dq=16, lse=16, w=16, n=2 * 2 * 128 * 8):
+    def call(dout=16, ds=None, dq=16, lse=16, w=16, n=2 * 2 * 128 * 72):
         return lib.tda_sdiff_bwd(16, 16, 16, 16, 16, None, dout, ds, 16, lse, dq, 16, 16, 16, 16, None, _lib.TDA_BF16, 1,
                                  2, 1, 8, 8, 64, 0.1, 1, None, None, 0, 0, 0, 0.5, w, n, 16, None)
     assert call(dout=None) == call(dq=8) == call(lse=None) == _lib.TDA_ERR_INVALID
