@@ -234,27 +234,20 @@ __global__ void __launch_bounds__(256) sdiff_simt_fwd_kernel(const SdParams p) {
 }
 
 // ================================================================== backward
-// Row `row` (counted over maps, heads and padded rows) of the product tables: a
-// number as three values of T; a row without keys gets one that no score reaches.
+// A number of one row of the product tables as three values of T and zeros.
 template <typename T>
-__device__ __forceinline__ void put_aux(const SdParams& p, long long row, float l, float d) {
-  uint8_t* tile = static_cast<uint8_t*>(p.aux) + row / kTile * (2 * kAuxTileBytes);
-  const int r = static_cast<int>(row % kTile);
+__device__ __forceinline__ void put_aux(uint8_t* table, int r, float x) {
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
-  const float x[2] = {l, d};
+  float rest = fmaxf(x / aux_unit(kF16), kF16 ? -65504.0f : -1e30f);  // a row without keys: what no score reaches
+  T part[8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float rest = fmaxf(x[i] / aux_unit(kF16), kF16 ? -65504.0f : -1e30f);
-    T part[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      store1(part + k, k < 3 ? rest : 0.f);
-      if (k < 3) rest -= static_cast<float>(part[k]);
-    }
-    uint4* at = reinterpret_cast<uint4*>(tile + i * kAuxTileBytes + (r >> 3) * 256 + (r & 7) * 16);
-    at[0] = *reinterpret_cast<uint4*>(part);
-    at[8] = make_uint4(0, 0, 0, 0);
+  for (int k = 0; k < 8; ++k) {
+    store1(part + k, k < 3 ? rest : 0.f);
+    if (k < 3) rest -= static_cast<float>(part[k]);
   }
+  uint4* at = reinterpret_cast<uint4*>(table + (r >> 3) * 256 + (r & 7) * 16);
+  at[0] = *reinterpret_cast<uint4*>(part);
+  at[8] = make_uint4(0, 0, 0, 0);
 }
 
 // D_1 = dout . O_1 and D_2 = dout . O_2, a warp a row.
@@ -286,18 +279,15 @@ __global__ void __launch_bounds__(256) sdiff_delta_kernel(const SdParams p) {
     a += __shfl_xor_sync(0xffffffffu, a, o);
     c += __shfl_xor_sync(0xffffffffu, c, o);
   }
-  if (row < rows && l == 0) {
-    float* t = p.table + table_at(p, 0, bh, i);
-    t[0] = i < p.Sq ? -p.lse[at] : -kInf;
-    t[kTile] = -a;
-    t[2 * rows] = i < p.Sq ? -p.lse[all + at] : -kInf;
-    t[2 * rows + kTile] = -c;
-    if constexpr (sizeof(T) == 2) {
-      if (p.aux) {
-        put_aux<T>(p, row, t[0] / p.c, t[kTile]);
-        put_aux<T>(p, rows + row, t[2 * rows] / p.c, t[2 * rows + kTile]);
-      }
-    }
+  // four lanes, a number each: -L_1, -D_1, -L_2, -D_2
+  if (row < rows && l < 4) {
+    const int m = l >> 1;
+    const float x = l & 1 ? -(m ? c : a) : (i < p.Sq ? -p.lse[m * all + at] : -kInf);
+    p.table[table_at(p, m, bh, i) + (l & 1) * kTile] = x;
+    if constexpr (sizeof(T) == 2)
+      if (p.aux)
+        put_aux<T>(static_cast<uint8_t*>(p.aux) + ((m * rows + row) / kTile * 2 + (l & 1)) * kAuxTileBytes, static_cast<int>(row % kTile),
+                   l & 1 ? x : x / p.c);
   }
 }
 

@@ -75,36 +75,6 @@ __device__ __forceinline__ void mma_score(uint32_t dcol, uint32_t a, uint32_t b)
   __syncwarp();
 }
 
-// The same with A [128][D] in TMEM (16-bit, D / 2 columns): half the operand bytes
-// from shared memory, which feeds 64 a cycle, so a product of two shared-memory
-// operands of this shape takes 128 cycles and this one 64.
-template <int D, bool F16>
-__device__ __forceinline__ void mma_score_ts(uint32_t dcol, uint32_t acol, uint32_t b) {
-  using G = Geo<D, F16>;
-  const uint64_t db = smem_desc_sw128(b, 16, 1024);
-  const uint32_t hi = static_cast<uint32_t>(db >> 32), lb = static_cast<uint32_t>(db);
-  if (elected()) {
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk)
-      mma_ts(dcol, acol + 8 * kk, desc_at(lb, hi, (kk >> 2) * G::kBoxBytes + (kk & 3) * 32), G::kIdescScore, kk > 0 ? 1u : 0u);
-  }
-  __syncwarp();
-}
-
-// 32 words (64 elements) of row r of a tile, from shared memory to TMEM column `col` of this thread's lane
-__device__ __forceinline__ void tile_row_to_tmem(const uint8_t* box, int r, uint32_t col) {
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint32_t w[16];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint4 v = *reinterpret_cast<const uint4*>(box + r * 128 + (((4 * half + c) ^ (r & 7)) << 4));
-      w[4 * c] = v.x, w[4 * c + 1] = v.y, w[4 * c + 2] = v.z, w[4 * c + 3] = v.w;
-    }
-    tmem_st16(col + 16 * half, w);
-  }
-}
-
 // D[dcol] (+)= W X: W [128][128] 16-bit in TMEM, X an MN-major tile of 128 rows.  W fills 64
 // columns, or (QUARTERS) 16 of each 32: each quarter over the scores it came from, so that
 // the four warps that share a row's scores need not wait for one another.

@@ -7,9 +7,10 @@
 //     S^T = K_m Q_m^T, dP^T = V dout^T, then dV += P'^T dout, dK_m += dS^T Q_m,
 //     P'_1 = P_1, P'_2 = -lambda P_2 (L and D are subtracted by the products).  It walks map 1's query tiles of every head
 //     of the group, writes dK_1, then map 2's: dV sums both maps and all heads in TMEM.
-//   dq, a CTA a tile of 128 queries of one head and map:
-//     S = Q_m K_m^T, dP = dout V^T, dQ_m += dS K_m, with Q_m and dout held in TMEM;
-//     dS replaces dP, so the next S needs S read, not used.
+//   dq, a CTA a tile of 128 queries of one head, both maps: per key tile
+//     S1 = Q1 K1^T and dP = dout V^T, dP into registers for both maps, S2 = Q2 K2^T
+//     over dP, then dQ1 += dS1 K1, dQ2 += dS2 K2: five products instead of six, and
+//     each map's S is computed while the other map's weights are formed.
 // Sixteen warps (a row's 128 columns over four) hold the weights between the two halves of a step: while they
 // exponentiate S, the tensor cores run dK (dQ) of the last step and dP; while
 // they form dS, dV and the next S.  P and dS enter the products as one 16-bit
@@ -360,36 +361,39 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
 template <int D, bool F16>
 struct QC : Geo<D, F16> {
   using G = Geo<D, F16>;
-  static constexpr int kSlots = D == 128 ? 5 : 8;
-  static constexpr int kOffRing = 2 * G::kTileBytes;  // Q, dout, then the K / V ring
+  static constexpr int kSlots = D == 128 ? 4 : 8;
+  static constexpr int kOffRing = 3 * G::kTileBytes;  // Q1, Q2, dout, then the K1 / V / K2 ring
   static constexpr int kOffBar = kOffRing + kSlots * G::kTileBytes;
   static constexpr int kSmem = kOffBar + 1024 + 1024;
   static_assert(kSmem <= kSmemBudget, "shared memory");
-  static constexpr uint32_t kS = 0, kP = 128, kDQ = 256, kQ = 384, kG = 448;  // dS over dP; Q and dout as operands
+  static constexpr uint32_t kA = 0, kB = 128;  // S1, then dS1 / dP, then S2, then dS2
+  static __device__ __forceinline__ constexpr uint32_t dq_col(int m) { return 256u + 128u * m; }
 };
 
 struct QBars {
-  uint64_t q_full, ops_full, o_full, drain, s_full, s_free, dp_full, ds_full;
+  uint64_t q_full, o_full, drain, dp_full, dp_free;
+  uint64_t s_full[2], ds_full[2];  // per map
   uint64_t slot_full[8], slot_empty[8];
   uint32_t tmem_base;
   int abort_flag;
 };
 
-// ring order: K(0) V(0) K(1) V(1) ...
+// ring order: K1(t) V(t) K2(t)
 template <int D, bool F16>
-__device__ void q_produce(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, int m, int b, int h, int kvh, int qt, int n) {
+__device__ void q_produce(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, int b, int h, int kvh, int qt, int n) {
   using C = QC<D, F16>;
-  mbar_arrive_expect_tx(&bars->q_full, 2 * C::kTileBytes);
-  load_tile<D, F16>(smem, &tp.m.q[m], &bars->q_full, qt * kTile, h, b);
-  load_tile<D, F16>(smem + C::kTileBytes, &tp.m.dout, &bars->q_full, qt * kTile, h, b);
+  mbar_arrive_expect_tx(&bars->q_full, 3 * C::kTileBytes);
+  load_tile<D, F16>(smem, &tp.m.q[0], &bars->q_full, qt * kTile, h, b);
+  load_tile<D, F16>(smem + 2 * C::kTileBytes, &tp.m.dout, &bars->q_full, qt * kTile, h, b);
+  load_tile<D, F16>(smem + C::kTileBytes, &tp.m.q[1], &bars->q_full, qt * kTile, h, b);
   bool ok = true;
   int idx = 0;
-  for (; idx < 2 * n; ++idx) {
-    const int slot = idx % C::kSlots;
+  for (; idx < 3 * n; ++idx) {
+    const int slot = idx % C::kSlots, x = idx % 3;
     ok = wait_inline(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_QP);
     if (!ok) break;
     mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
-    load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, idx & 1 ? &tp.m.v : &tp.m.k[m], &bars->slot_full[slot], idx / 2 * kTile,
+    load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, x == 1 ? &tp.m.v : &tp.m.k[x >> 1], &bars->slot_full[slot], idx / 3 * kTile,
                       kvh, b);
   }
   if (!ok) {
@@ -402,43 +406,47 @@ __device__ void q_produce(const SdTcParams& tp, uint8_t* smem, QBars* bars, cons
 template <int D, bool F16>
 __device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t tmem, int n) {
   using C = QC<D, F16>;
-  const uint32_t ring = smem_u32(smem + C::kOffRing);
+  const uint32_t q = smem_u32(smem), g = q + 2 * C::kTileBytes, ring = smem_u32(smem + C::kOffRing);
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (ok) ok = wait_inline_warp(bar, parity, ctl, ST_QM);
     if (ok) tc_fence_after();
   };
+  auto slot = [&](int idx) { return ring + (idx % C::kSlots) * C::kTileBytes; };
   auto acquire = [&](int idx) {
     wait(&bars->slot_full[idx % C::kSlots], (idx / C::kSlots) & 1);
-    return ring + (idx % C::kSlots) * C::kTileBytes;
+    return slot(idx);
   };
-  auto score = [&](int t) {
-    const uint32_t k = acquire(2 * t);
+  auto score = [&](int t, int m) {
+    const uint32_t k = acquire(3 * t + 2 * m);
     if (!ok) return;
-    mma_score_ts<D, F16>(tmem + C::kS, tmem + C::kQ, k);
-    commit(&bars->s_full);
+    mma_score<D, F16>(tmem + (m ? C::kB : C::kA), q + m * C::kTileBytes, k);
+    commit(&bars->s_full[m]);
   };
   auto dprob = [&](int t) {
-    const uint32_t v = acquire(2 * t + 1);
+    const uint32_t v = acquire(3 * t + 1);
     if (!ok) return;
-    mma_score_ts<D, F16>(tmem + C::kP, tmem + C::kG, v);
-    commit(&bars->slot_empty[(2 * t + 1) % C::kSlots]);
+    mma_score<D, F16>(tmem + C::kB, g, v);
+    commit(&bars->slot_empty[(3 * t + 1) % C::kSlots]);
     commit(&bars->dp_full);
   };
-  wait(&bars->ops_full, 0);
+  wait(&bars->q_full, 0);
   if (ok) {
-    score(0);
+    score(0, 0);
     dprob(0);
   }
   for (int t = 0; t < n && ok; ++t) {
-    if (t + 1 < n) {
-      wait(&bars->s_free, t & 1);
-      if (ok) score(t + 1);
-    }
-    wait(&bars->ds_full, t & 1);
+    wait(&bars->dp_free, t & 1);
+    if (ok) score(t, 1);
+    wait(&bars->ds_full[0], t & 1);
     if (!ok) break;
-    mma_weights<D, F16, true>(tmem + C::kDQ, tmem + C::kP, ring + ((2 * t) % C::kSlots) * C::kTileBytes, t > 0);
-    commit(&bars->slot_empty[(2 * t) % C::kSlots]);
+    mma_weights<D, F16, true>(tmem + C::dq_col(0), tmem + C::kA, slot(3 * t), t > 0);
+    commit(&bars->slot_empty[(3 * t) % C::kSlots]);
+    if (t + 1 < n) score(t + 1, 0);
+    wait(&bars->ds_full[1], t & 1);
+    if (!ok) break;
+    mma_weights<D, F16, true>(tmem + C::dq_col(1), tmem + C::kB, slot(3 * t + 2), t > 0);
+    commit(&bars->slot_empty[(3 * t + 2) % C::kSlots]);
     if (t + 1 < n) dprob(t + 1);
   }
   if (ok) {
@@ -450,110 +458,114 @@ __device__ void q_issue(uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t
 }
 
 template <int D, bool F16>
-__device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t tmem, const float* table, int pad,
-                       int m, int b, int h, int qt, int n, int len, int warp, int lane) {
+__device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, uint32_t tmem, int b, int h, int qt, int n,
+                       int len, int warp, int lane) {
   using C = QC<D, F16>;
   const SdParams& p = tp.p;
   const int wg = warp >> 2, row = (warp & 3) * 32 + lane, grow = qt * kTile + row, off = p.Sk - p.Sq;
   const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const uint32_t a_col = tmem + lane_off + C::kA + 32 * wg, b_col = tmem + lane_off + C::kB + 32 * wg;
   const long long bh = static_cast<long long>(b) * p.H + h;
-  const float* row_tab = table + 2 * ((static_cast<long long>(m) * p.B * p.H + bh) * pad + qt * kTile) + row;
-  const float minus_l = row_tab[0], minus_d = row_tab[kTile], c = p.c;
-  const int last = p.causal ? min(len - 1, grow + off) : len - 1;
-  const uint32_t p_col = tmem + lane_off + C::kP + 32 * wg;
-  bool ok = true;
-  if (n > 0) {  // Q and dout become TMEM operands: a warpgroup a box of 64 columns
-    ok = wait_inline_warp(&bars->q_full, 0, ctl, ST_QW);
-    if (ok && wg < 2 * C::kBoxes) {
-      const int x = wg / C::kBoxes, box = wg % C::kBoxes;
-      tile_row_to_tmem(smem + x * C::kTileBytes + box * C::kBoxBytes, row, tmem + lane_off + (x ? C::kG : C::kQ) + 32 * box);
-      tmem_wait_st();
-      tc_fence_before();
-    }
-    __syncwarp();
-    if (ok && lane == 0) mbar_arrive(&bars->ops_full);
+  float minus_l[2], minus_d[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float* t = p.table + 2 * ((static_cast<long long>(m) * p.B * p.H + bh) * p.pad + qt * kTile) + row;
+    minus_l[m] = t[0];
+    minus_d[m] = t[kTile];
   }
+  const float c = p.c;
+  const int last = p.causal ? min(len - 1, grow + off) : len - 1;
+  bool ok = true;
   for (int t = 0; t < n && ok; ++t) {
-    ok = wait_inline_warp(&bars->s_full, t & 1, ctl, ST_QW);
-    if (!ok) break;
-    tc_fence_after();
     const bool masked = (t + 1) * kTile > len || (p.causal && (t + 1) * kTile - 1 > qt * kTile + off);
-    float pr[32];
-    {
-      uint32_t s[32];
-      tmem_ld32(tmem + lane_off + C::kS + 32 * wg, s);
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->s_free);
+    const bool tail = t == n - 1 && len < p.Sk && (t + 1) * kTile > len;
+    const int lim = last - t * kTile - 32 * wg;
+    float dp[32];
 #pragma unroll
-      for (int y = 0; y < 32; y += 2) {
-        const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(minus_l, minus_l));
-        const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
-        pr[y] = ez.x;
-        pr[y + 1] = ez.y;
+    for (int m = 0; m < 2; ++m) {
+      ok = wait_inline_warp(&bars->s_full[m], t & 1, ctl, ST_QW);
+      if (!ok) break;
+      tc_fence_after();
+      float pr[32];
+      {
+        uint32_t s[32];
+        tmem_ld32(m ? b_col : a_col, s);
+        tmem_wait_ld();
+#pragma unroll
+        for (int y = 0; y < 32; y += 2) {
+          const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(minus_l[m], minus_l[m]));
+          const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
+          pr[y] = ez.x;
+          pr[y + 1] = ez.y;
+        }
       }
-    }
-    ok = wait_inline_warp(&bars->dp_full, t & 1, ctl, ST_QW);
-    if (!ok) break;
-    tc_fence_after();
-    {
-      uint32_t s[32];
-      tmem_ld32(p_col, s);
-      tmem_wait_ld();
+      if (m == 0) {  // dP serves both maps
+        ok = wait_inline_warp(&bars->dp_full, t & 1, ctl, ST_QW);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[32];
+        tmem_ld32(b_col, s);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->dp_free);
+#pragma unroll
+        for (int y = 0; y < 32; ++y) dp[y] = __uint_as_float(s[y]);
+      }
 #pragma unroll
       for (int y = 0; y < 32; y += 2) {
-        const float2 d = __fadd2_rn(f2u(s[y], s[y + 1]), make_float2(minus_d, minus_d));
+        const float2 d = __fadd2_rn(make_float2(dp[y], dp[y + 1]), make_float2(minus_d[m], minus_d[m]));
         const float2 r = __fmul2_rn(make_float2(pr[y], pr[y + 1]), d);
         pr[y] = r.x;
         pr[y + 1] = r.y;
       }
-    }
-    if (masked) {
-      const int lim = last - t * kTile - 32 * wg;
+      if (masked) {
 #pragma unroll
-      for (int y = 0; y < 32; ++y) pr[y] = y <= lim ? pr[y] : 0.f;
+        for (int y = 0; y < 32; ++y) pr[y] = y <= lim ? pr[y] : 0.f;
+      }
+      // K rows past the length: zeroed (S is done with them) before the product with dS reads them
+      if (tail) {
+        if (wg == 0 && t * kTile + row >= len) zero_row<D>(smem + C::kOffRing + ((3 * t + 2 * m) % C::kSlots) * C::kTileBytes, row);
+        fence_proxy_async_smem();
+      }
+      store_weights<F16>(m ? b_col : a_col, pr);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->ds_full[m]);
     }
-    // K rows past the length: zeroed (S is done with them) before the product with dS reads them
-    if (t == n - 1 && len < p.Sk && (t + 1) * kTile > len) {
-      if (wg == 0 && t * kTile + row >= len) zero_row<D>(smem + C::kOffRing + ((2 * t) % C::kSlots) * C::kTileBytes, row);
-      fence_proxy_async_smem();
-    }
-    store_weights<F16>(p_col, pr);
-    tmem_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars->ds_full);
   }
   if (ok && n > 0) ok = wait_inline_warp(&bars->o_full, 0, ctl, ST_QW);
   tc_fence_after();
-  const float w = (m ? -lambda_at(p.lam, b, h) : 1.0f) * p.scale;
   uint8_t* stage = smem + C::kOffRing;
   if (ok) {
-    stage_accumulator<D, F16>(stage, tmem + lane_off + C::kDQ, row, wg, w, n == 0);
+    const float w2 = -lambda_at(p.lam, b, h) * p.scale;
+    stage_accumulator<D, F16>(stage, tmem + lane_off + C::dq_col(0), row, wg, p.scale, n == 0);
+    stage_accumulator<D, F16>(stage + C::kTileBytes, tmem + lane_off + C::dq_col(1), row, wg, w2, n == 0);
     fence_proxy_async_smem();
   }
   ok = named_barrier_and(2, kWorkThreads, ok);
   if (ok && warp == 0 && lane == 0) {
-    for (int x = 0; x < D / 64; ++x) tma_store_3d(&tp.m.dq[m], stage + x * C::kBoxBytes, 64 * x, qt * kTile, static_cast<int>(bh));
+    for (int m = 0; m < 2; ++m)
+      for (int x = 0; x < D / 64; ++x)
+        tma_store_3d(&tp.m.dq[m], stage + m * C::kTileBytes + x * C::kBoxBytes, 64 * x, qt * kTile, static_cast<int>(bh));
     bulk_commit_group();
     bulk_wait_group_read0();
   }
 }
 
 template <int D, bool F16>
-__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_constant__ SdTcParams tp, const float* table, int pad) {
+__global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_constant__ SdTcParams tp) {
   using C = QC<D, F16>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   QBars* bars = reinterpret_cast<QBars*>(smem + C::kOffBar);
   const SdParams& p = tp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the heads and maps of one kv group run side by side, each group's longest rows first
-  const int per = 2 * p.group * tp.n_qt;
+  // the heads of one kv group run side by side, each group's longest rows first
+  const int per = p.group * tp.n_qt;
   const int g = static_cast<int>(blockIdx.x) / per, r = static_cast<int>(blockIdx.x) % per;
-  const int b = g / p.Hkv, kvh = g % p.Hkv, x = r % (2 * p.group), qt = tp.n_qt - 1 - r / (2 * p.group);
-  const int m = x & 1, h = kvh * p.group + x / 2;
+  const int b = g / p.Hkv, kvh = g % p.Hkv, h = kvh * p.group + r % p.group, qt = tp.n_qt - 1 - r / p.group;
   const int len = keys_of(p, b);
   int n_keys = len <= 1 ? 0 : len;  // a lone key's weight is 1 whatever its score: no gradient
   if (p.causal) n_keys = max(0, min(n_keys, min((qt + 1) * kTile, p.Sq) + p.Sk - p.Sq));
@@ -563,10 +575,11 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
     mbar_init(&bars->o_full, 1);
     mbar_init(&bars->drain, 1);
     mbar_init(&bars->dp_full, 1);
-    mbar_init(&bars->s_full, 1);
-    mbar_init(&bars->ops_full, 16);
-    mbar_init(&bars->s_free, 16);
-    mbar_init(&bars->ds_full, 16);
+    mbar_init(&bars->dp_free, 16);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->ds_full[i], 16);
+    }
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&bars->slot_full[i], 1);
       mbar_init(&bars->slot_empty[i], 1);
@@ -585,10 +598,10 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
   const WaitCtl ctl = make_wait_ctl(&bars->abort_flag, tp.status, tp.timeout_ns);
   if (warp < kProd) {
     more_registers<kManyRegs>();
-    q_work<D, F16>(tp, smem, bars, ctl, tmem, table, pad, m, b, h, qt, n, len, warp, lane);
+    q_work<D, F16>(tp, smem, bars, ctl, tmem, b, h, qt, n, len, warp, lane);
   } else {
     fewer_registers<kFewRegs>();
-    if (n > 0 && warp == kProd && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, m, b, h, kvh, qt, n);
+    if (n > 0 && warp == kProd && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, b, h, kvh, qt, n);
     if (n > 0 && warp == kIssue) q_issue<D, F16>(smem, bars, ctl, uniform(tmem), n);
     __syncwarp();
   }
@@ -601,24 +614,22 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
 }
 
 template <int D, bool F16>
-cudaError_t launch(const SdTcParams& tp, const float* table, int pad, cudaStream_t s) {
+cudaError_t launch(const SdTcParams& tp, cudaStream_t s) {
   auto kq = sdiff_tc_dq_kernel<D, F16>;
   auto kk = sdiff_tc_dkv_kernel<D, F16>;
   if (cudaError_t e = allow_shared<sdiff_tc_dq_kernel<D, F16>>(QC<D, F16>::kSmem)) return e;
   if (cudaError_t e = allow_shared<sdiff_tc_dkv_kernel<D, F16>>(KvC<D, F16>::kSmem)) return e;
   kk<<<static_cast<unsigned>(tp.p.B * tp.p.Hkv * tp.n_kt), kThreads, KvC<D, F16>::kSmem, s>>>(tp);
   if (cudaError_t e = cudaGetLastError()) return e;
-  kq<<<static_cast<unsigned>(2 * tp.p.B * tp.p.H * tp.n_qt), kThreads, QC<D, F16>::kSmem, s>>>(tp, table, pad);
+  kq<<<static_cast<unsigned>(tp.p.B * tp.p.H * tp.n_qt), kThreads, QC<D, F16>::kSmem, s>>>(tp);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_sdiff_tc_bwd(const SdTcParams& tp, int dtype, int D, cudaStream_t s) {
-  const float* table = tp.p.table;
-  const int pad = tp.p.pad;
-  if (dtype == TDA_BF16) return D == 64 ? launch<64, false>(tp, table, pad, s) : launch<128, false>(tp, table, pad, s);
-  return D == 64 ? launch<64, true>(tp, table, pad, s) : launch<128, true>(tp, table, pad, s);
+  if (dtype == TDA_BF16) return D == 64 ? launch<64, false>(tp, s) : launch<128, false>(tp, s);
+  return D == 64 ? launch<64, true>(tp, s) : launch<128, true>(tp, s);
 }
 
 }  // namespace tda
