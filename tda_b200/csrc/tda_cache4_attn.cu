@@ -36,6 +36,7 @@
 #include "tda_host.h"
 #include "tda_ptx.cuh"
 #include "tda_transform.cuh"
+#include "tda_wait.cuh"
 
 namespace tda {
 
@@ -51,7 +52,9 @@ constexpr float kInf = __builtin_huge_valf();
 template <int D>
 struct DC {
   static constexpr int kSlabBytes = cache4_slab_bytes(D);
-  static constexpr int kStages = D == 128 ? 4 : 8;
+  // blocks an SM: at D = 128 registers without spills beat a fourth block (381 against 410 us)
+  static constexpr int kResident = D == 128 ? 3 : 4;
+  static constexpr int kStages = D == 128 ? 5 : 8;
   static constexpr int kRing = kStages * kSlabBytes;
   static constexpr int kStride = D + 4;  // floats of a joined row
   static constexpr int kSmem = kWarps * kRing;
@@ -189,7 +192,7 @@ __device__ __forceinline__ void write_out(const AttnParams& p, int b, int head, 
 
 // one (chunk, kv head x head block, request)
 template <int D, bool THR, bool F16, int PM>
-__global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(32 * kWarps, DC<D>::kResident) cache4_attn_kernel(const __grid_constant__ AttnParams p) {
   using C = DC<D>;
   constexpr int W = D / 32;  // groups
   constexpr int S = C::kStages;
@@ -320,7 +323,7 @@ __global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __gri
   bool ok = true;
   int i = 0;
   for (; i < n; ++i) {
-    ok = mbar_wait_warp(&full[warp][i % S], (i / S) & 1, ctl, ST_CACHE);
+    ok = wait_inline_warp(&full[warp][i % S], (i / S) & 1, ctl, ST_CACHE);
     if (!ok) break;
     // every lane is done with slab i - 1: its stage takes slab i + S - 1
     if (i + S - 1 < n) {
@@ -525,38 +528,84 @@ __global__ void __launch_bounds__(32 * kWarps, 4) cache4_attn_kernel(const __gri
   }
 }
 
-// Joins a request's chunks, in order: one head a block of 2 D threads, a thread
-// a map and dim (threshold: half of the chunks and a dim).
-template <int D, bool THR, bool F16>
-__global__ void __launch_bounds__(2 * D) cache4_join_kernel(const __grid_constant__ AttnParams p) {
-  __shared__ float s_o[2][D], s_l[2];
-  constexpr int kPart = part_floats<D, THR>();
-  const int head = blockIdx.x, b = blockIdx.y, mp = threadIdx.x / D, d = threadIdx.x % D;
+// Joins a request's chunks: a block a head, G groups of 2 D threads (a map and a
+// dim each) over every G-th chunk, then the groups in order.
+// The chunks' weights 2^(M_c - M) are formed once, in shared memory, so that the
+// sums are independent loads: a request of 74 chunks waits for memory a few times,
+// not 74.
+constexpr int kMaxChunks = 1024;
+
+template <int D, bool THR, bool F16, int G>
+__global__ void __launch_bounds__(2 * D * G) cache4_join_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int kThreads = 2 * D * G, kPart = part_floats<D, THR>();
+  __shared__ float s_f[2][kMaxChunks];
+  __shared__ float s_o[G][2][D];
+  __shared__ float s_w[kThreads / 32][2];
+  __shared__ float s_top[2], s_l[2];
+  const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int grp = threadIdx.x / (2 * D), mp = threadIdx.x / D % 2, d = threadIdx.x % D;
   const int n = (length_of(p, b) + p.chunk - 1) / p.chunk;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float* part = p.part + (static_cast<long long>(b) * p.heads + head) * p.n_chunks * kPart;
-  float o = 0.f, l = 0.f;
-  if constexpr (THR) {
-#pragma unroll 4
-    for (int c = mp; c < n; c += 2) o += part[static_cast<long long>(c) * kPart + d];
-  } else {
-    float top = -kInf;
-#pragma unroll 4
-    for (int c = 0; c < n; ++c) top = fmaxf(top, part[static_cast<long long>(c) * kPart + 2 * mp]);
-#pragma unroll 4
-    for (int c = 0; c < n; ++c) {
-      const float* q = part + static_cast<long long>(c) * kPart;
-      const float mc = q[2 * mp], f = mc == -kInf ? 0.f : fast_ex2(mc - top);
-      l = fmaf(q[2 * mp + 1], f, l);
-      o = fmaf(q[8 + mp * D + d], f, o);
+  auto block_reduce = [&](float x, float y, bool max) {  // of a pair, into every thread by way of s_w
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float u = __shfl_xor_sync(0xffffffffu, x, o), v = __shfl_xor_sync(0xffffffffu, y, o);
+      x = max ? fmaxf(x, u) : x + u;
+      y = max ? fmaxf(y, v) : y + v;
     }
+    __syncthreads();
+    if (lane == 0) {
+      s_w[warp][0] = x;
+      s_w[warp][1] = y;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      float r = s_w[0][threadIdx.x];
+      for (int w = 1; w < kThreads / 32; ++w) r = max ? fmaxf(r, s_w[w][threadIdx.x]) : r + s_w[w][threadIdx.x];
+      (max ? s_top : s_l)[threadIdx.x] = r;
+    }
+    __syncthreads();
+  };
+  if constexpr (!THR) {
+    float m[2] = {-kInf, -kInf}, l[2] = {0.f, 0.f};
+    for (int c = threadIdx.x; c < n; c += kThreads) {
+      const float4 x = *reinterpret_cast<const float4*>(part + static_cast<long long>(c) * kPart);
+      m[0] = fmaxf(m[0], x.x);
+      m[1] = fmaxf(m[1], x.z);
+    }
+    block_reduce(m[0], m[1], true);
+    for (int c = threadIdx.x; c < n; c += kThreads) {
+      const float4 x = *reinterpret_cast<const float4*>(part + static_cast<long long>(c) * kPart);
+      const float f0 = x.x == -kInf ? 0.f : fast_ex2(x.x - s_top[0]), f1 = x.z == -kInf ? 0.f : fast_ex2(x.z - s_top[1]);
+      s_f[0][c] = f0;
+      s_f[1][c] = f1;
+      l[0] = fmaf(x.y, f0, l[0]);
+      l[1] = fmaf(x.w, f1, l[1]);
+    }
+    block_reduce(l[0], l[1], false);
   }
-  s_o[mp][d] = o;
-  if (d == 0) s_l[mp] = l;
+  float o = 0.f;
+  if constexpr (THR) {
+    const float* at = part + d;
+#pragma unroll 8
+    for (int c = 2 * grp + mp; c < n; c += 2 * G) o += at[static_cast<long long>(c) * kPart];
+  } else {
+    const float* at = part + 8 + mp * D + d;
+#pragma unroll 8
+    for (int c = grp; c < n; c += G) o = fmaf(at[static_cast<long long>(c) * kPart], s_f[mp][c], o);
+  }
+  s_o[grp][mp][d] = o;
   __syncthreads();
-  if (mp == 0)
-    write_out<F16>(p, b, head, D, d,
-                   THR ? s_o[0][d] + s_o[1][d] : share(s_o[0][d], s_l[0]) - lambda_at(p.lam, b, head) * share(s_o[1][d], s_l[1]));
+  if (threadIdx.x < D) {
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      x += s_o[g][0][d];
+      y += s_o[g][1][d];
+    }
+    write_out<F16>(p, b, head, D, d, THR ? x + y : share(x, s_l[0]) - lambda_at(p.lam, b, head) * share(y, s_l[1]));
+  }
 }
 
 template <int D, bool THR, bool F16, int PM>
@@ -569,14 +618,15 @@ cudaError_t launch(const AttnParams& p, cudaStream_t s) {
   // the join's blocks start while the last chunks run and wait for the grid in front of them
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.heads, p.B);
-  cfg.blockDim = dim3(2 * D);
+  const bool many = p.n_chunks > 24;  // four groups: one request of 74 chunks 53 -> 33 us; 128 requests of 8 pay 40 us for them
+  cfg.blockDim = dim3(2 * D * (many ? 4 : 1));
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, cache4_join_kernel<D, THR, F16>, p);
+  return many ? cudaLaunchKernelEx(&cfg, cache4_join_kernel<D, THR, F16, 4>, p) : cudaLaunchKernelEx(&cfg, cache4_join_kernel<D, THR, F16, 1>, p);
 }
 
 template <int D, bool F16>
@@ -590,15 +640,20 @@ cudaError_t dispatch(const AttnParams& p, bool thr, cudaStream_t s) {
   }
 }
 
-// Tokens a block takes: one wave of resident blocks (4 an SM) where the table's
-// width allows it, at least two slabs a warp, at most 2048 (uneven lengths then
-// still spread over the device).
+// Tokens a block takes: one wave of resident blocks (3 an SM) where the table's
+// width allows it, at least two slabs a warp, at most 1024, or 2048 where that
+// still makes eight waves (uneven lengths then spread over the device: 32 requests
+// of up to 8192 tokens and 16 heads take 158 us with 1024 and 164 with 2048, 128
+// of up to 16384 and 8 heads 428 and 410), more only where the join could not hold
+// the chunks of one request.
 int64_t chunk_tokens(int64_t B, int64_t head_groups, int64_t max_len) {
-  const int64_t want = 148 * 4 / (B * head_groups) + 1;  // chunks of one request
+  const int64_t want = 148 * 3 / (B * head_groups) + 1;  // chunks of one request
   int64_t chunk = ceil_div(ceil_div(max_len, want), 64) * 64;
   if (chunk < 128) chunk = 128;
-  if (chunk > 2048) chunk = 2048;
-  return chunk;
+  const int64_t cap = B * head_groups * ceil_div(max_len, 2048) >= 148 * 3 * 8 ? 2048 : 1024;
+  if (chunk > cap) chunk = cap;
+  const int64_t least = ceil_div(ceil_div(max_len, kMaxChunks), 64) * 64;
+  return chunk < least ? least : chunk;
 }
 
 }  // namespace

@@ -9,6 +9,7 @@
 #include "tda_ptx.cuh"
 #include "tda_sdiff.h"
 #include "tda_transform.cuh"
+#include "tda_wait.cuh"
 
 namespace tda {
 namespace sd {
@@ -147,29 +148,6 @@ __device__ __forceinline__ float2 poly_ex2(float2 x) {
   }
   return make_float2(__uint_as_float((__float_as_uint(r.x) << 23) + __float_as_uint(p.x)),
                      __uint_as_float((__float_as_uint(r.y) << 23) + __float_as_uint(p.y)));
-}
-
-// The bounded wait of tda_ptx.cuh without its call: a warp whose register count
-// changes (setmaxnreg) may not call a function.
-__device__ __forceinline__ bool wait_inline(uint64_t* bar, uint32_t parity, const WaitCtl& ctl, int code) {
-  const uint32_t a = smem_u32(bar);
-  if (mbar_try_wait(a, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
-  while (!mbar_try_wait(a, parity)) {
-    if (*ctl.abort_flag) return false;
-    const uint64_t waited = global_timer_ns() - t0;
-    const bool other = waited > 1000000ull && *reinterpret_cast<volatile int*>(ctl.status) != ctl.status0;
-    if (other || waited > ctl.timeout_ns) {
-      *ctl.abort_flag = 1;
-      if (!other) atomicCAS(ctl.status, 0, code);
-      return false;
-    }
-  }
-  return true;
-}
-__device__ __forceinline__ bool wait_inline_warp(uint64_t* bar, uint32_t parity, const WaitCtl& ctl, int code) {
-  const bool ok = wait_inline(bar, parity, ctl, code);
-  return __all_sync(0xffffffffu, ok);
 }
 
 template <int kRegs>
