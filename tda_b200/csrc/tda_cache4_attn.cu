@@ -18,8 +18,10 @@
 // are what bounds the kernel next to DRAM).  The factor 16 is divided out of
 // those dims of q, and of those rows of O at the end.  For K the product starts
 // from minus the offset's share, which removes it without an instruction (exact
-// products summed in fp32: an error near 1e-4 of |q| times a code unit); V
-// subtracts it (exact).  K's scale multiplies a group's fp32 product.
+// products summed in fp32: an error near 1e-4 of |q| times a code unit).  V
+// subtracts it (exact), and so does the threshold form with fp16 queries for the
+// nibbles of the larger offset: its weights are powers of s - tau, where the error
+// would show (4e-4 of the output; a bf16 output's own rounding is 2e-3).  K's scale multiplies a group's fp32 product.
 // q enters as fp16 after division by a power of two that brings its largest
 // element to [1, 2): exact but for elements 2^-21 below it.
 // V's scale goes into the weight, w = p s, rounded to fp16 (2^-12) relative to a
@@ -195,6 +197,7 @@ template <int D, bool THR, bool F16, int PM>
 __global__ void __launch_bounds__(32 * kWarps, DC<D>::kResident) cache4_attn_kernel(const __grid_constant__ AttnParams p) {
   using C = DC<D>;
   constexpr int W = D / 32;  // groups
+  constexpr bool kExactLow = THR && F16;
   constexpr int S = C::kStages;
   extern __shared__ __align__(128) uint8_t ring_all[];
   __shared__ uint64_t full[kWarps][S];
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(32 * kWarps, DC<D>::kResident) cache4_attn_ker
       q2[s][0] = m ? a : 0u;
       q2[s][1] = m ? c : 0u;
       const float2 ra = unpack_f16x2(a), rc = unpack_f16x2(c);
-      const float add = -1032.0f * (ra.x + ra.y) - 1152.0f * (rc.x + rc.y);
+      const float add = (kExactLow ? 0.f : -1032.0f) * (ra.x + ra.y) - 1152.0f * (rc.x + rc.y);
       sum[s >> 1] = (s & 1) ? sum[s >> 1] + add : add;
     }
 #pragma unroll
@@ -320,6 +323,7 @@ __global__ void __launch_bounds__(32 * kWarps, DC<D>::kResident) cache4_attn_ker
   float limit[2] = {THR ? 0.f : -kInf, THR ? 0.f : -kInf}, down[2] = {1.f, 1.f};
 
   const Magic mg;
+  auto low = [&](uint32_t w) { return kExactLow ? low_codes(mg, w) : mg.low(w); };  // K's low nibbles
   bool ok = true;
   int i = 0;
   for (; i < n; ++i) {
@@ -352,10 +356,10 @@ __global__ void __launch_bounds__(32 * kWarps, DC<D>::kResident) cache4_attn_ker
           const uint32_t x = k[mp][0][w], y = k[mp][1][w], x8 = x >> 8, y8 = y >> 8;
           const uint32_t(&q)[2 * W][2] = mp ? q2 : q1;
           if (mp == 0)
-            mma16816_from(acc, mg.low(x), mg.low(y), mg.high(x), mg.high(y), q[2 * w][0], q[2 * w][1], off[w][0], off[w][1]);
+            mma16816_from(acc, low(x), low(y), mg.high(x), mg.high(y), q[2 * w][0], q[2 * w][1], off[w][0], off[w][1]);
           else
-            mma16816(acc, mg.low(x), mg.low(y), mg.high(x), mg.high(y), q[2 * w][0], q[2 * w][1]);
-          mma16816(acc, mg.low(x8), mg.low(y8), mg.high(x8), mg.high(y8), q[2 * w + 1][0], q[2 * w + 1][1]);
+            mma16816(acc, low(x), low(y), mg.high(x), mg.high(y), q[2 * w][0], q[2 * w][1]);
+          mma16816(acc, low(x8), low(y8), mg.high(x8), mg.high(y8), q[2 * w + 1][0], q[2 * w + 1][1]);
         }
         const float s0 = scale_of(ks[0], w), s1 = scale_of(ks[1], w);
         s[0] = fmaf(acc[0], s0, s[0]);
