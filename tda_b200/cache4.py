@@ -69,6 +69,8 @@ class PagePlan(NamedTuple):
 
 
 def _ints(what, name, t, shape, device):
+    if type(t) is torch.Tensor and t.dtype is torch.int32 and t.device == device and (shape is None or t.shape == shape):
+        return
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
         raise TypeError(f"{what}: {name} must be an int32 tensor")
     if t.device != device:
@@ -78,6 +80,8 @@ def _ints(what, name, t, shape, device):
 
 
 def _cuda(what, t):
+    if type(t) is torch.Tensor and t.is_cuda:
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected torch.Tensor inputs")
     if not t.is_cuda:
@@ -119,7 +123,8 @@ def plan_pages(lengths, new_tokens, block_table, free_pages, free_head, page_siz
         raise ValueError(f"{what}: page_size must be >= 1, got {page_size}")
     if rows < 0:
         raise ValueError(f"{what}: rows must be >= 0, got {rows}")
-    lengths, new_tokens, free_pages = lengths.contiguous(), new_tokens.contiguous(), free_pages.contiguous()
+    if not (lengths.is_contiguous() and new_tokens.is_contiguous() and free_pages.is_contiguous()):
+        lengths, new_tokens, free_pages = lengths.contiguous(), new_tokens.contiguous(), free_pages.contiguous()
     # one allocation: its parts are views
     buf = torch.empty(3 * rows + 2 * B + 3, dtype=torch.int32, device=dev)
     at = buf.data_ptr()
@@ -127,7 +132,7 @@ def plan_pages(lengths, new_tokens, block_table, free_pages, free_head, page_siz
            stride, block_table.shape[1], free_pages.data_ptr(), free_pages.shape[0], free_head.data_ptr(), page_size,
            rows, at, at + 4 * rows, at + 8 * rows, at + 12 * rows, at + 4 * (3 * rows + B + 1),
            at + 4 * (3 * rows + 2 * B + 1), at + 4 * (3 * rows + 2 * B + 2))
-    return PagePlan(*buf.split((rows, rows, rows, B + 1, B, 1, 1)))
+    return PagePlan(*buf.split_with_sizes((rows, rows, rows, B + 1, B, 1, 1)))
 
 
 def _rows(what, cache, slots):

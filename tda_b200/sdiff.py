@@ -82,9 +82,8 @@ def lambda_ref(lam, B: int, H: int, device: torch.device, what: str):
 
 def _check(q1, q2, k1, k2, v, key_lengths, what="differential_softmax_attention"):
     ts = (q1, q2, k1, k2, v)
-    for t in ts:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{what}: expected torch.Tensor inputs")
+    if not all(isinstance(t, torch.Tensor) for t in ts):
+        raise TypeError(f"{what}: expected torch.Tensor inputs")
     if q1.dim() != 4 or k1.dim() != 4:
         raise ValueError(f"{what}: expected (batch, heads, seq_len, head_dim) tensors, got {tuple(q1.shape)} and "
                          f"{tuple(k1.shape)}")
@@ -102,10 +101,11 @@ def _check(q1, q2, k1, k2, v, key_lengths, what="differential_softmax_attention"
     if not q1.is_cuda:
         raise RuntimeError(f"{what}: tda_b200 runs on CUDA tensors only (got device {q1.device}); "
                            "there is no CPU fallback")
+    dev, dt = q1.device, q1.dtype
     for t in ts:
-        if t.device != q1.device:
+        if t.device != dev:
             raise RuntimeError(f"{what}: all inputs must be on one device")
-        if not t.dtype.is_floating_point:
+        if not (t.dtype is dt and dt in _CODE) and not t.dtype.is_floating_point:
             raise TypeError(f"{what}: floating point inputs required, got {t.dtype}")
     if key_lengths is not None:
         if not isinstance(key_lengths, torch.Tensor) or key_lengths.dtype not in (torch.int32, torch.int64):
@@ -119,7 +119,7 @@ def _check(q1, q2, k1, k2, v, key_lengths, what="differential_softmax_attention"
 def _compute_dtype(ts) -> torch.dtype:
     common = ts[0].dtype
     for t in ts[1:]:
-        if t.dtype != common:
+        if t.dtype is not common:
             common = torch.promote_types(common, t.dtype)
     return common if common in _CODE else torch.float32
 
