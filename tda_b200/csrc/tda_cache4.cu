@@ -260,26 +260,25 @@ struct Elem<__half> {
   }
 };
 
-// round-half-even of 7 x / amax without a division.  c, the nearest whole number
-// to an approximate quotient, is right or one off; the remainder 14 |x| - 2 c amax
-// is exact in fp32 for bf16 and fp16 inputs and says which: past amax the
-// neighbour is nearer, and at amax (a tie) it is taken when c is odd.
-__device__ __forceinline__ uint32_t code_of(float x, float amax, float inv7) {
-  const float ax = fabsf(x);
-  const float shifted = fmaf(ax, inv7, 12582912.0f);  // 1.5 2^23: the sum's last bits are c
-  const uint32_t c = __float_as_uint(shifted) & 7u;
-  const float rem = fmaf(-2.0f * (shifted - 12582912.0f), amax, 14.0f * ax);
-  const float edge = __uint_as_float(__float_as_uint(amax) - (c & 1u));
-  const uint32_t up = fabsf(rem) > edge ? (rem > 0.0f ? 1u : 0xffffffffu) : 0u;
-  const uint32_t m = c + up;
-  return x < 0.0f ? 8u - m : 8u + m;
+// The nibble 8 + round-half-even(7 x / amax) without a division.  Adding 1.5 2^23 +
+// 8 to an approximate quotient leaves 8 + c in the sum's last bits, c the nearest
+// whole number or one beside it; the remainder 7 x - c amax is exact in fp32 for
+// bf16 and fp16 inputs and says which: past amax / 2 the neighbour is nearer, and
+// at amax / 2 (a tie) it is taken when c is odd.  Returned with other bits above.
+__device__ __forceinline__ uint32_t nibble(float x, float amax, float half, float inv7) {
+  const float shifted = fmaf(x, inv7, 12582920.0f);
+  const uint32_t n = __float_as_uint(shifted);
+  const float rem = fmaf(-(shifted - 12582920.0f), amax, 7.0f * x);
+  const float edge = __uint_as_float(__float_as_uint(half) - (n & 1u));
+  const int step = (static_cast<int>(__float_as_uint(rem)) >> 31) | 1;
+  return n + (fabsf(rem) > edge ? step : 0);
 }
 
 __device__ __forceinline__ uint32_t max_bits(uint32_t a, float x) { return max(a, __float_as_uint(x) & 0x7fffffffu); }
 
 // one word of codes and the scales of its runs' groups from 8 elements
 template <int D, bool V>
-__device__ __forceinline__ uint32_t quantise(const float (&x)[8], bool normalize, float (&sc)[2]) {
+__device__ __forceinline__ uint32_t quantise(float (&x)[8], bool normalize, float (&sc)[2]) {
   // largest magnitude of each run's group, as bits so that a NaN wins
   uint32_t m[2] = {0, 0};
 #pragma unroll
@@ -300,21 +299,36 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[8], bool normalize
     for (int o = 1; o < RC<D>::kPer; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     inv_norm = 1.0f / fmaxf(sqrtf(ss), 1e-12f);
   }
+  // A largest magnitude near an end of the exponent's range (rare) is moved away from
+  // it, with its group, so that neither 7 / amax nor 7 x leaves the range.
+  float lift[2] = {1.0f, 1.0f};
+  if (__any_sync(0xffffffffu, min(m[0], m[1]) < 0x22000000u || max(m[0], m[1]) > 0x5e000000u)) {  // 2^-59, 2^61
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      lift[r] = m[r] < 0x22000000u ? 0x1p80f : (m[r] > 0x5e000000u ? 0x1p-64f : 1.0f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * r + j] *= lift[r];
+    }
+  }
   uint32_t word = 0;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    float amax = __uint_as_float(m[r]);
-    const bool finite = m[r] < 0x7f800000u;
-    sc[r] = finite ? amax / 7.0f * inv_norm : __uint_as_float(0x7fc00000u);
-    // far from the ends of the exponent's range, so that neither 7 / amax nor 14 x leaves it
-    const float lift = amax < 1e-18f ? 0x1p80f : (amax > 1e18f ? 0x1p-80f : 1.0f);
-    amax *= lift;
-    const bool any = finite && amax > 0.0f;
-    const float inv7 = __fdividef(7.0f, amax);
+    const float amax = __uint_as_float(m[r]) * lift[r], half = 0.5f * amax, inv7 = __fdividef(7.0f, amax);
+    uint32_t part = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      word |= (any ? code_of(x[4 * r + j] * lift, amax, inv7) : 8u) << (4 * nibble_of<V>(r, j));
+    for (int j = 0; j < 4; ++j) {
+      const int at = 4 * nibble_of<V>(r, j);
+      part |= (nibble(x[4 * r + j], amax, half, inv7) << at) & (15u << at);
+    }
+    // a group of zeros, or one that holds an infinity or a NaN (whose scale is NaN): codes of zero
+    uint32_t zeros = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) zeros |= 8u << (4 * nibble_of<V>(r, j));
+    word |= m[r] - 1u < 0x7f7fffffu ? part : zeros;
   }
+#pragma unroll
+  for (int r = 0; r < (V ? 2 : 1); ++r)
+    sc[r] = m[r] < 0x7f800000u ? __uint_as_float(m[r]) / 7.0f * inv_norm : __uint_as_float(0x7fc00000u);
   return word;
 }
 
