@@ -59,19 +59,30 @@ struct KvWork {
   int b, kvh, kt, i0, per_map;  // first query tile, steps of one map
 };
 
+// K1 and V, issued by the thread that set the barriers up while the others still
+// allocate and synchronise
+template <int D, bool F16>
+__device__ void kv_prime(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const KvWork& w) {
+  using C = KvC<D, F16>;
+  mbar_arrive_expect_tx(&bars->k_full, C::kTileBytes);
+  load_tile<D, F16>(smem, &tp.m.k[0], &bars->k_full, w.kt * kTile, w.kvh, w.b);
+  mbar_arrive_expect_tx(&bars->v_full, C::kTileBytes);
+  load_tile<D, F16>(smem + C::kTileBytes, &tp.m.v, &bars->v_full, w.kt * kTile, w.kvh, w.b);
+}
+
 template <int D, bool F16>
 __device__ void kv_produce(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const WaitCtl& ctl, const KvWork& w) {
   using C = KvC<D, F16>;
   const SdParams& p = tp.p;
-  mbar_arrive_expect_tx(&bars->v_full, C::kTileBytes);
-  load_tile<D, F16>(smem + C::kTileBytes, &tp.m.v, &bars->v_full, w.kt * kTile, w.kvh, w.b);
   bool ok = true;
   int t = 0, idx = 0, n_k = 0;
   for (int m = 0; m < 2 && ok; ++m) {
-    if (m == 1) ok = wait_inline(&bars->k_free, 0, ctl, ST_KP);
-    if (!ok) break;
-    mbar_arrive_expect_tx(&bars->k_full, C::kTileBytes);
-    load_tile<D, F16>(smem, &tp.m.k[m], &bars->k_full, w.kt * kTile, w.kvh, w.b);
+    if (m == 1) {
+      ok = wait_inline(&bars->k_free, 0, ctl, ST_KP);
+      if (!ok) break;
+      mbar_arrive_expect_tx(&bars->k_full, C::kTileBytes);
+      load_tile<D, F16>(smem, &tp.m.k[1], &bars->k_full, w.kt * kTile, w.kvh, w.b);
+    }
     ++n_k;
     for (int h = w.kvh * p.group; h < (w.kvh + 1) * p.group && ok; ++h) {
       for (int i = w.i0; i < tp.n_qt; ++i, ++t) {
@@ -307,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
   const int len = keys_of(p, w.b);
   w.i0 = p.causal ? max(0, w.kt * kTile - (p.Sk - p.Sq)) / kTile : 0;
   w.per_map = w.kt * kTile < len ? p.group * max(0, tp.n_qt - w.i0) : 0;
-  if (threadIdx.x == 0) {
+  if (warp == kProd && lane == 0) {
     uint64_t* one[] = {&bars->k_full, &bars->v_full, &bars->k_free, &bars->s_full, &bars->dp_full, &bars->map_done, &bars->drain};
     for (uint64_t* x : one) mbar_init(x, 1);
     mbar_init(&bars->p_full, 16);
@@ -322,6 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
     }
     bars->abort_flag = 0;
     fence_mbar_init();
+    if (w.per_map > 0) kv_prime<D, F16>(tp, smem, bars, w);
   }
   if (threadIdx.x >= 128 && threadIdx.x < 256) {  // the unit in three columns of every row
     const int r = threadIdx.x - 128;
@@ -378,23 +390,38 @@ struct QBars {
   int abort_flag;
 };
 
-// ring order: K1(t) V(t) K2(t)
+// tile idx of the ring: K1, V, K2 of key tile idx / 3
 template <int D, bool F16>
-__device__ void q_produce(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, int b, int h, int kvh, int qt, int n) {
+__device__ __forceinline__ void q_fetch(const SdTcParams& tp, uint8_t* smem, QBars* bars, int b, int kvh, int idx) {
+  using C = QC<D, F16>;
+  const int slot = idx % C::kSlots, x = idx % 3;
+  mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
+  load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, x == 1 ? &tp.m.v : &tp.m.k[x >> 1], &bars->slot_full[slot], idx / 3 * kTile,
+                    kvh, b);
+}
+
+// the loads that wait for nothing, as in the forward
+template <int D, bool F16>
+__device__ int q_prime(const SdTcParams& tp, uint8_t* smem, QBars* bars, int b, int h, int kvh, int qt, int n) {
   using C = QC<D, F16>;
   mbar_arrive_expect_tx(&bars->q_full, 3 * C::kTileBytes);
   load_tile<D, F16>(smem, &tp.m.q[0], &bars->q_full, qt * kTile, h, b);
+  q_fetch<D, F16>(tp, smem, bars, b, kvh, 0);
   load_tile<D, F16>(smem + 2 * C::kTileBytes, &tp.m.dout, &bars->q_full, qt * kTile, h, b);
   load_tile<D, F16>(smem + C::kTileBytes, &tp.m.q[1], &bars->q_full, qt * kTile, h, b);
+  const int primed = min(3 * n, C::kSlots);
+  for (int idx = 1; idx < primed; ++idx) q_fetch<D, F16>(tp, smem, bars, b, kvh, idx);
+  return primed;
+}
+
+template <int D, bool F16>
+__device__ void q_produce(const SdTcParams& tp, uint8_t* smem, QBars* bars, const WaitCtl& ctl, int b, int kvh, int n, int idx) {
+  using C = QC<D, F16>;
   bool ok = true;
-  int idx = 0;
   for (; idx < 3 * n; ++idx) {
-    const int slot = idx % C::kSlots, x = idx % 3;
-    ok = wait_inline(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_QP);
+    ok = wait_inline(&bars->slot_empty[idx % C::kSlots], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_QP);
     if (!ok) break;
-    mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
-    load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, x == 1 ? &tp.m.v : &tp.m.k[x >> 1], &bars->slot_full[slot], idx / 3 * kTile,
-                      kvh, b);
+    q_fetch<D, F16>(tp, smem, bars, b, kvh, idx);
   }
   if (!ok) {
     drain_wait(&bars->q_full, 0, ctl);
@@ -570,7 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
   int n_keys = len <= 1 ? 0 : len;  // a lone key's weight is 1 whatever its score: no gradient
   if (p.causal) n_keys = max(0, min(n_keys, min((qt + 1) * kTile, p.Sq) + p.Sk - p.Sq));
   const int n = (n_keys + kTile - 1) / kTile;
-  if (threadIdx.x == 0) {
+  int primed = 0;
+  if (warp == kProd && lane == 0) {
     mbar_init(&bars->q_full, 1);
     mbar_init(&bars->o_full, 1);
     mbar_init(&bars->drain, 1);
@@ -586,6 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
     }
     bars->abort_flag = 0;
     fence_mbar_init();
+    if (n > 0) primed = q_prime<D, F16>(tp, smem, bars, b, h, kvh, qt, n);
   }
   if (warp == kIssue) {
     tmem_alloc(&bars->tmem_base, 512);
@@ -601,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
     q_work<D, F16>(tp, smem, bars, ctl, tmem, b, h, qt, n, len, warp, lane);
   } else {
     fewer_registers<kFewRegs>();
-    if (n > 0 && warp == kProd && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, b, h, kvh, qt, n);
+    if (n > 0 && warp == kProd && lane == 0) q_produce<D, F16>(tp, smem, bars, ctl, b, kvh, n, primed);
     if (n > 0 && warp == kIssue) q_issue<D, F16>(smem, bars, ctl, uniform(tmem), n);
     __syncwarp();
   }

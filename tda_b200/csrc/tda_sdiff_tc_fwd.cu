@@ -57,22 +57,38 @@ struct FBars {
 };
 static_assert(sizeof(FBars) <= 1024, "barriers");
 
+// tile idx of the ring: K1, K2, V of key tile idx / 3
 template <int D, bool F16>
-__device__ void produce(const SdTcParams& tp, uint8_t* smem, FBars* bars, const WaitCtl& ctl, int b, int h, int kvh, int qt, int n) {
+__device__ __forceinline__ void fetch(const SdTcParams& tp, uint8_t* smem, FBars* bars, int b, int kvh, int idx) {
+  using C = FC<D, F16>;
+  const int slot = idx % C::kSlots, x = idx % 3;
+  mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
+  load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, x == 2 ? &tp.m.v : &tp.m.k[x], &bars->slot_full[slot], idx / 3 * kTile,
+                    kvh, b);
+}
+
+// The loads that wait for nothing, issued by the thread that set the barriers up
+// while the others still allocate and synchronise (1500 cycles of a CTA's start).
+template <int D, bool F16>
+__device__ int prime(const SdTcParams& tp, uint8_t* smem, FBars* bars, int b, int h, int kvh, int qt, int n) {
   using C = FC<D, F16>;
   mbar_arrive_expect_tx(&bars->q_full, 2 * C::kTileBytes);
   load_tile<D, F16>(smem, &tp.m.q[0], &bars->q_full, qt * kTile, h, b);
+  fetch<D, F16>(tp, smem, bars, b, kvh, 0);
   load_tile<D, F16>(smem + C::kTileBytes, &tp.m.q[1], &bars->q_full, qt * kTile, h, b);
+  const int primed = min(3 * n, C::kSlots);
+  for (int idx = 1; idx < primed; ++idx) fetch<D, F16>(tp, smem, bars, b, kvh, idx);
+  return primed;
+}
+
+template <int D, bool F16>
+__device__ void produce(const SdTcParams& tp, uint8_t* smem, FBars* bars, const WaitCtl& ctl, int b, int kvh, int n, int idx) {
+  using C = FC<D, F16>;
   bool ok = true;
-  int idx = 0;
   for (; idx < 3 * n; ++idx) {
-    const int slot = idx % C::kSlots;
-    ok = wait_inline(&bars->slot_empty[slot], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_PROD);
+    ok = wait_inline(&bars->slot_empty[idx % C::kSlots], ((idx / C::kSlots) & 1) ^ 1, ctl, ST_PROD);
     if (!ok) break;
-    mbar_arrive_expect_tx(&bars->slot_full[slot], C::kTileBytes);
-    const int x = idx % 3;
-    load_tile<D, F16>(smem + C::kOffRing + slot * C::kTileBytes, x == 2 ? &tp.m.v : &tp.m.k[x], &bars->slot_full[slot],
-                      idx / 3 * kTile, kvh, b);
+    fetch<D, F16>(tp, smem, bars, b, kvh, idx);
   }
   if (!ok) {
     drain_wait(&bars->q_full, 0, ctl);
@@ -241,9 +257,11 @@ __device__ void softmax(const SdTcParams& tp, uint8_t* smem, FBars* bars, const 
   uint8_t* stage = smem + C::kOffRing;
   uint8_t* stage1 = stage + C::kTileBytes;
   uint8_t* stage2 = stage1 + kTile * D * 4;
-  if (ok) {
+  // 32 columns at a time; a warpgroup's boxes leave as soon as they are staged
+  const bool leader = (warp & 3) == 0 && lane == 0;
 #pragma unroll
-    for (int x = m * (D / 2); x < (m + 1) * (D / 2); x += 32) {
+  for (int x = m * (D / 2); x < (m + 1) * (D / 2); x += 32) {
+    if (ok) {
       float a[32], d[32];
       if (n > 0) {
         uint32_t u[32], v[32];
@@ -266,17 +284,21 @@ __device__ void softmax(const SdTcParams& tp, uint8_t* smem, FBars* bars, const 
 #pragma unroll
       for (int i = 0; i < 32; ++i) a[i] -= lam * d[i];
       stage_16<F16>(stage, row, x, a);
+      fence_proxy_async_smem();
     }
-    fence_proxy_async_smem();
-  }
-  ok = named_barrier_and(2, kSoftmaxThreads, ok);
-  if (ok && warp == 0 && lane == 0) {
-    for (int x = 0; x < D / 64; ++x) tma_store_3d(&tp.m.out, stage + x * C::kBoxBytes, 64 * x, qt * kTile, static_cast<int>(bh));
-    if (p.o12)
-      for (int x = 0; x < D / 32; ++x) {
-        tma_store_3d(&tp.m.o12, stage1 + x * C::kBoxBytes, 32 * x, qt * kTile, static_cast<int>(bh));
-        tma_store_3d(&tp.m.o12, stage2 + x * C::kBoxBytes, 32 * x, qt * kTile, static_cast<int>(n_bh + bh));
+    if (p.o12) {
+      ok = named_barrier_and(2 + m, 128, ok);
+      if (ok && leader) {
+        const int box = x / 32;
+        tma_store_3d(&tp.m.o12, stage1 + box * C::kBoxBytes, x, qt * kTile, static_cast<int>(bh));
+        tma_store_3d(&tp.m.o12, stage2 + box * C::kBoxBytes, x, qt * kTile, static_cast<int>(n_bh + bh));
       }
+    }
+  }
+  ok = named_barrier_and(1, kSoftmaxThreads, ok);
+  if (ok && warp == 0 && lane == 0)
+    for (int x = 0; x < D / 64; ++x) tma_store_3d(&tp.m.out, stage + x * C::kBoxBytes, 64 * x, qt * kTile, static_cast<int>(bh));
+  if (leader) {
     bulk_commit_group();
     bulk_wait_group_read0();
   }
@@ -298,7 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_fwd_kernel(const __grid_
   int n_keys = len;
   if (p.causal) n_keys = max(0, min(len, min((qt + 1) * kTile, p.Sq) + p.Sk - p.Sq));
   const int n = (n_keys + kTile - 1) / kTile;
-  if (threadIdx.x == 0) {
+  int primed = 0;
+  if (warp == 8 && lane == 0) {
     mbar_init(&bars->q_full, 1);
     mbar_init(&bars->o_full, 1);
     mbar_init(&bars->drain, 1);
@@ -313,6 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_fwd_kernel(const __grid_
     }
     bars->abort_flag = 0;
     fence_mbar_init();
+    if (n > 0) primed = prime<D, F16>(tp, smem, bars, b, h, kvh, qt, n);
   }
   if (warp == 9) {
     tmem_alloc(&bars->tmem_base, 512);
@@ -328,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_fwd_kernel(const __grid_
     softmax<D, F16>(tp, smem, bars, ctl, tmem, b, h, qt, n, len, warp, lane);
   } else {
     fewer_registers<kFewRegs>();
-    if (n > 0 && warp == 8 && lane == 0) produce<D, F16>(tp, smem, bars, ctl, b, h, kvh, qt, n);
+    if (n > 0 && warp == 8 && lane == 0) produce<D, F16>(tp, smem, bars, ctl, b, kvh, n, primed);
     if (n > 0 && warp == 9) issue<D, F16>(smem, bars, ctl, uniform(tmem), n);
     __syncwarp();
   }
