@@ -239,6 +239,7 @@ class DifferentialSoftmaxFunction(torch.autograd.Function):
         return out if out.dtype == q1.dtype else out.to(q1.dtype)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q1, q2, k1, k2, v, lam_t, kl, o12, lse = ctx.saved_tensors
         lam = ctx.lam if lam_t is None else lam_t
