@@ -14,7 +14,8 @@
 // Sixteen warps (a row's 128 columns over four) hold the weights between the two halves of a step: while they
 // exponentiate S, the tensor cores run dK (dQ) of the last step and dP; while
 // they form dS, dV and the next S.  P and dS enter the products as one 16-bit
-// value each (2^-9 / 2^-12 of an element, averaged over a row); sums, the
+// value each (2^-9 / 2^-12 of an element, averaged over a row; P in dV with its
+// rest where rows see few keys, see few_tiles); sums, the
 // difference dP - D and the exponent stay in fp32.  O_1, O_2 come in fp32 for D.
 // Measured on B200, bf16, 8 heads of (8192, 128), causal: dkv 531 us, tensor pipe
 // 71% active (a step's four products take 2048 cycles of its 2800: weights of the
@@ -77,9 +78,11 @@ __device__ void kv_prime(const SdTcParams& tp, uint8_t* smem, KvBars* bars, cons
 
 // Query tiles (the first ones) whose rows see so few keys, 512 at most, that their
 // weights, large and few, make most of dV's norm in a causal sequence: there dV
-// takes the weights with what rounding left of them, a second product.  That
-// brings dV from 2.6e-3 to 2.4e-3 of its 64-bit value at (4, 32 on 8, 4096, 128)
-// for 10 of 528 steps (dkv 1890 -> 1990 us); for all of them it takes 2450 us.
+// takes the weights with what rounding left of them, a second product.  Measured
+// on B200: dV 2.6e-3 -> 2.0e-3 of its 64-bit value (bf16, causal, 4 heads on 1,
+// 4096 of 128; its own rounding is 1.7e-3), dkv 1900 -> 1990 us at (4, 32 on 8,
+// 4096, 128) for 10 of its 528 tile pairs a map and head, where all of them take
+// 2450 us.  Longer uncausal calls keep 2.6e-3.
 __device__ __forceinline__ int few_tiles(const SdParams& p, int len, int n_qt) {
   if (len <= 512) return n_qt;
   return p.causal ? max(0, 512 - (p.Sk - p.Sq)) / kTile : 0;
