@@ -18,6 +18,10 @@ cudaError_t launch_sdiff_tc_bwd(const SdTcParams& tp, int dtype, int D, cudaStre
 
 namespace {
 
+// bf16 and fp16 at these head dims fit the tensor-core kernels' tiles; fp32 needs
+// its own arithmetic and other head dims do not fill a 128-byte box
+bool on_tensor_cores(int dtype, int64_t D) { return dtype != TDA_F32 && (D == 64 || D == 128); }
+
 int fill(SdParams& p, const void* q1, const void* q2, const void* k1, const void* k2, const void* v,
          const int64_t* strides, int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Sk, int64_t D,
          float scale, int causal, const int32_t* key_lengths, const void* lambda, int lambda_dtype, int64_t lsb,
@@ -51,6 +55,9 @@ int fill(SdParams& p, const void* q1, const void* q2, const void* k1, const void
   p.H = static_cast<int>(H);
   p.Hkv = static_cast<int>(Hkv);
   p.group = static_cast<int>(H / Hkv);
+  const int rows = on_tensor_cores(dtype, D) ? 128 : simt_tile_rows(static_cast<int>(D));
+  p.q_together = heads_together(causal != 0, static_cast<int>(B * H), ceil_div(Sq, rows), p.group);
+  p.k_together = heads_together(causal != 0, static_cast<int>(B * Hkv), ceil_div(Sk, rows), 1);
   p.Sq = static_cast<int>(Sq);
   p.Sk = static_cast<int>(Sk);
   p.causal = causal != 0;
@@ -58,10 +65,6 @@ int fill(SdParams& p, const void* q1, const void* q2, const void* k1, const void
   p.c = scale * 1.4426950408889634f;
   return TDA_OK;
 }
-
-// bf16 and fp16 at these head dims fit the tensor-core kernels' tiles; fp32 needs
-// its own arithmetic and other head dims do not fill a 128-byte box
-bool on_tensor_cores(int dtype, int64_t D) { return dtype != TDA_F32 && (D == 64 || D == 128); }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;

@@ -24,7 +24,7 @@ constexpr float kInf = __builtin_huge_valf();
 
 template <int D>
 struct SC {
-  static constexpr int BT = D <= 128 ? 64 : 32;
+  static constexpr int BT = simt_tile_rows(D);
   static constexpr int R = BT / 16;
   static constexpr int LD = D + 4;       // row stride of a tile, floats
   static constexpr int LP = BT + 4;      // row stride of a weight tile
@@ -157,7 +157,9 @@ __global__ void __launch_bounds__(256) sdiff_simt_fwd_kernel(const SdParams p) {
   float *qs = sm, *ks = qs + C::kTile, *vs = ks + C::kTile, *ps = vs + C::kTile;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int n_t = (p.Sq + C::BT - 1) / C::BT;
-  const int bh = blockIdx.x / n_t, qt = n_t - 1 - static_cast<int>(blockIdx.x % n_t);  // longest rows first
+  int bh, qt;
+  tile_of_block(blockIdx.x, n_t, p.q_together, bh, qt);
+  qt = n_t - 1 - qt;  // longest rows first
   const int b = bh / p.H, h = bh % p.H, kvh = h / p.group, i0 = qt * C::BT;
   int n_keys = keys_of(p, b);
   const int len = n_keys;
@@ -316,7 +318,9 @@ __global__ void __launch_bounds__(256) sdiff_simt_dq_kernel(const SdParams p) {
   float *qs = sm, *gs = qs + C::kTile, *ks = gs + C::kTile, *vs = ks + C::kTile, *ps = vs + C::kTile;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, m = blockIdx.y;
   const int n_t = (p.Sq + C::BT - 1) / C::BT;
-  const int bh = blockIdx.x / n_t, qt = n_t - 1 - static_cast<int>(blockIdx.x % n_t);
+  int bh, qt;
+  tile_of_block(blockIdx.x, n_t, p.q_together, bh, qt);
+  qt = n_t - 1 - qt;
   const int b = bh / p.H, h = bh % p.H, kvh = h / p.group, i0 = qt * C::BT;
   const int len = keys_of(p, b);
   int n_keys = len <= 1 ? 0 : len;  // a lone key's weight is 1 whatever its score: no gradient
@@ -373,7 +377,9 @@ __global__ void __launch_bounds__(256) sdiff_simt_dkv_kernel(const SdParams p) {
         *ls = ds + C::kP, *es = ls + C::BT;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int n_t = (p.Sk + C::BT - 1) / C::BT;
-  const int bh = blockIdx.x / n_t, j0 = static_cast<int>(blockIdx.x % n_t) * C::BT;
+  int bh, j0;
+  tile_of_block(blockIdx.x, n_t, p.k_together, bh, j0);
+  j0 *= C::BT;
   const int b = bh / p.Hkv, kvh = bh % p.Hkv;
   const int len = keys_of(p, b);
   const int first = p.causal ? max(0, j0 - (p.Sk - p.Sq)) / C::BT * C::BT : 0;

@@ -318,10 +318,10 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_fwd_kernel(const __grid_
   FBars* bars = reinterpret_cast<FBars*>(smem + C::kOffBar);
   const SdParams& p = tp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the heads of one kv group run side by side, each group's longest rows first
-  const int per = p.group * tp.n_qt;
-  const int g = static_cast<int>(blockIdx.x) / per, r = static_cast<int>(blockIdx.x) % per;
-  const int b = g / p.Hkv, kvh = g % p.Hkv, h = kvh * p.group + r % p.group, qt = tp.n_qt - 1 - r / p.group;
+  int bh, qt;
+  tile_of_block(blockIdx.x, tp.n_qt, p.q_together, bh, qt);
+  qt = tp.n_qt - 1 - qt;  // longest rows first
+  const int b = bh / p.H, h = bh % p.H, kvh = h / p.group;
   const int len = keys_of(p, b);
   int n_keys = len;
   if (p.causal) n_keys = max(0, min(len, min((qt + 1) * kTile, p.Sq) + p.Sk - p.Sq));
