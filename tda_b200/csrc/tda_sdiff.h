@@ -68,10 +68,10 @@ constexpr int simt_tile_rows(int D) { return D <= 128 ? 64 : 32; }
 // head, the last head's longest one starts when the other SMs are nearly done.
 // Measured on B200 against that order: dkv at (4, 32 on 8, 4096, 128) 1990 -> 1820
 // us, a backward of (1, 8, 8192, 128) 960 -> 805, a fp32 step of (2, 16 on 8, 1024,
-// 64) 2010 -> 1670; the same bits.  So heads go together until they make 512 tiles, a few for each SM, and no
-// further, so that long sequences keep few heads' keys in L2; heads that share
-// keys (`side`) stay together.  Uncausal tiles are equal: side by side they only
-// lose L2 hits (a ragged fp16 backward of (6, 16, 1999, 64) 705 -> 728 us).
+// 64) 2010 -> 1670; the same bits.  So heads go together until they make 512 tiles,
+// a few for each SM, and no further, so that long sequences keep few heads' keys
+// in L2; heads that share keys (`side`) stay together.  Uncausal tiles are equal:
+// side by side they only lose L2 hits (a ragged fp16 backward of (6, 16, 1999, 64) 705 -> 728 us).
 inline int heads_together(bool causal, int heads, long long tiles, int side) {
   if (!causal) return side;
   for (int n = side; n < heads && n <= 2048; n += side)

@@ -17,9 +17,9 @@
 // value each (2^-9 / 2^-12 of an element, averaged over a row; P in dV with its
 // rest where rows see few keys, see few_tiles); sums, the
 // difference dP - D and the exponent stay in fp32.  O_1, O_2 come in fp32 for D.
-// Measured on B200, bf16, 8 heads of (8192, 128), causal: dkv 531 us, tensor pipe
-// 71% active (a step's four products take 2048 cycles of its 2800: weights of the
-// next step wait for S, S for the last weights' product); dq 391 us, 56% active
+// Measured on B200, bf16, 8 heads of (8192, 128), causal: dkv 475 us, tensor pipe
+// 67% active (a step's four products take 2048 cycles of its 3000: weights of the
+// next step wait for S, S for the last weights' product); dq 331 us, 57% active
 // (its warps' own work, 2 x 128 x 128 weights a tile, is longer than its products).
 #include <cstring>
 

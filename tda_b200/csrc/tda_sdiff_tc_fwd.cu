@@ -21,7 +21,7 @@
 // cycles to the row maximum, 1400 for the weights, 1300 until the products that
 // need them are done, for two maps in turn, 3200 a tile.  Measured on B200, bf16
 // (1,16,32768,128): 7.1 ms (7.9 under the power cap), 1240 TFLOP/s of executed
-// products; (8 heads, 8192): 303 us, tensor pipe 59% active, exponential unit 38%.
+// products; (8 heads, 8192): 256 us, tensor pipe 59% active, exponential unit 38%.
 // Polynomials for 0 to 4 of 8 pairs differ by 3%.
 #include <cstring>
 
