@@ -258,3 +258,26 @@ def test_cuda_graph_and_compile():
     g2 = torch.autograd.grad(tda_b200.differential_softmax_attention(*leaves, l), leaves + [l], dout)
     for x, y in zip(g1, g2):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("shape", [
+    # B, H, Hkv, S, D, dtype: heads that make several groups of tiles, of a prime number of heads, of one head
+    (3, 40, 8, 1025, 16, torch.float32),
+    (20, 6, 3, 1300, 64, torch.bfloat16),
+    (1, 37, 37, 1999, 64, torch.float16),
+    (2, 5, 5, 4300, 64, torch.bfloat16),
+])
+def test_causal_tiles_of_many_heads(shape):
+    """Every tile of every head is computed once whatever the number of heads that run side by side."""
+    B, H, Hkv, S, D, dtype = shape
+    xs, dout, lam = make(B, H, Hkv, S, S, D, dtype, seed=S)
+    check(xs, dout, lam, True, None)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Sq,Sk,causal", [(700, 700, True), (300, 700, True), (700, 300, True), (520, 640, False)])
+def test_weights_around_512_keys(Sq, Sk, causal, dtype):
+    """dv where some query tiles see 512 keys or fewer, and lengths on either side of that."""
+    lens = torch.tensor([n for n in (511, 512, 513, Sk) if n <= Sk], dtype=torch.int32, device="cuda")
+    xs, dout, lam = make(len(lens), 4, 2, Sq, Sk, 128, dtype, seed=Sq)
+    check(xs, dout, lam, causal, lens)
