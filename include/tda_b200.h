@@ -310,7 +310,9 @@ size_t tda_cache4_block_bytes(int64_t page_size, int64_t head_dim);
  * found no page (list or table exhausted), all three are -1 for rows past the
  * last token.  starts ((requests + 1) prefix sums of new_tokens), lengths_out
  * (tokens held afterwards), *free_head_out and *dropped (tokens that found no
- * page) describe the step; outputs must not overlap inputs. */
+ * page) describe the step; starts and *dropped stay at 2^31 - 1 where they
+ * would pass it.  Negative lengths and counts are taken as 0.  Outputs must not
+ * overlap inputs. */
 int tda_plan_pages(const int32_t* lengths, const int32_t* new_tokens, int64_t requests, int32_t* block_table,
                    int64_t table_stride, int64_t table_width, const int32_t* free_pages, int64_t num_free,
                    const int32_t* free_head, int64_t page_size, int64_t rows, int32_t* slots, int32_t* positions,

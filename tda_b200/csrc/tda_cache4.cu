@@ -38,19 +38,28 @@ constexpr int kPlanThreads = 512;
 constexpr int kPlanScan = 2048;   // requests scanned at a time
 constexpr int kPlanRows = 2048;   // token rows of one block
 
-// Exclusive prefix sums of (a, b) over the block and their totals.
+// Counts are added up to 2^31 - 1 and stay there: new_tokens may sum to more, and
+// a wrapped sum would place rows and pages in front of their arrays.  Capped
+// addition of non-negative numbers is associative, so a scan may use it.
+__device__ __forceinline__ int add_capped(int a, int b) {
+  return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b), 0x7fffffffu));
+}
+
+// Exclusive prefix sums of (a, b) over the block and their totals, capped.
 __device__ void block_scan2(int& a, int& b, int& ta, int& tb, int2* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int a0 = a, b0 = b;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
     if (lane >= o) {
-      a += x;
-      b += y;
+      a = add_capped(a, x);
+      b = add_capped(b, y);
     }
   }
   if (lane == 31) warp_sums[warp] = make_int2(a, b);
+  a = __shfl_up_sync(0xffffffffu, a, 1);
+  b = __shfl_up_sync(0xffffffffu, b, 1);
+  if (lane == 0) a = b = 0;
   __syncthreads();
   int pa = 0, pb = 0;
   ta = tb = 0;
@@ -58,15 +67,27 @@ __device__ void block_scan2(int& a, int& b, int& ta, int& tb, int2* warp_sums) {
   for (int w = 0; w < kPlanThreads / 32; ++w) {
     const int2 s = warp_sums[w];
     if (w < warp) {
-      pa += s.x;
-      pb += s.y;
+      pa = add_capped(pa, s.x);
+      pb = add_capped(pb, s.y);
     }
-    ta += s.x;
-    tb += s.y;
+    ta = add_capped(ta, s.x);
+    tb = add_capped(tb, s.y);
   }
-  a += pa - a0;
-  b += pb - b0;
+  a = add_capped(a, pa);
+  b = add_capped(b, pb);
   __syncthreads();
+}
+
+// Sum of x over the block, in thread 0.
+__device__ long long block_sum(long long x, long long* warp_sums) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = x;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int w = 1; w < kPlanThreads / 32; ++w) x += warp_sums[w];
+  __syncthreads();
+  return x;
 }
 
 // Every block scans all requests (a few KB from L2) and then writes its own
@@ -78,12 +99,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
   __shared__ int s_start[kPlanScan + 1], s_first[kPlanScan], s_len[kPlanScan], s_after[kPlanScan],
       s_got[kPlanScan];
   __shared__ int2 warp_sums[kPlanThreads / 32];
+  __shared__ long long warp_totals[kPlanThreads / 32];
   const int tid = threadIdx.x;
   const int head = max(0, *p.free_head);
   const int left = max(0, p.n_free - head);
   const long long row0 = static_cast<long long>(blockIdx.x) * kPlanRows;
   const int row_end = static_cast<int>(min(static_cast<long long>(p.rows), row0 + kPlanRows));
-  int base_tok = 0, base_page = 0, kept = 0, taken = 0;
+  int base_tok = 0, base_page = 0;
+  long long lost = 0, taken = 0;  // of this thread's requests: tokens without a place, pages handed out
   constexpr int kPer = kPlanScan / kPlanThreads;
   for (int r0 = 0; r0 < p.B; r0 += kPlanScan) {
     const int n = min(kPlanScan, p.B - r0);
@@ -100,12 +123,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
         want[i] = static_cast<int>(min(last, static_cast<long long>(p.width))) - held[i];
         s_len[r] = len;
       }
-      sa += add[i];
-      sw += want[i];
+      sa = add_capped(sa, add[i]);
+      sw = add_capped(sw, want[i]);
     }
     block_scan2(sa, sw, ta, tw, warp_sums);
-    sa += base_tok;
-    sw += base_page;
+    sa = add_capped(sa, base_tok);
+    sw = add_capped(sw, base_page);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int r = tid * kPer + i;
@@ -118,18 +141,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
         s_first[r] = sw;
         s_after[r] = after;
         s_got[r] = got;
-        kept += after - len;
+        lost += static_cast<long long>(add[i]) - (after - len);
         taken += got;
         if (blockIdx.x == 0) {
           p.starts[r0 + r] = sa;
           p.lengths_out[r0 + r] = after;
         }
       }
-      sa += add[i];
-      sw += want[i];
+      sa = add_capped(sa, add[i]);
+      sw = add_capped(sw, want[i]);
     }
-    base_tok += ta;
-    base_page += tw;
+    base_tok = add_capped(base_tok, ta);
+    base_page = add_capped(base_page, tw);
     if (tid == 0) s_start[n] = base_tok;
     __syncthreads();
     // fresh table entries: a warp a request
@@ -139,7 +162,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
         p.table[(r0 + r) * p.table_stride + held0 + c] = p.free_pages[head + s_first[r] + c];
     }
     // rows of these requests that belong to this block
-    const int lo = max(static_cast<int>(row0), s_start[0]), hi = min(row_end, s_start[n]);
+    const int lo = min(max(static_cast<int>(row0), s_start[0]), row_end), hi = min(row_end, s_start[n]);
     for (int i = lo + tid; i < hi; i += kPlanThreads) {
       int a = 0, b = n - 1;  // last request whose start is <= i
       while (a < b) {
@@ -162,15 +185,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
     }
     __syncthreads();
   }
-  for (int i = max(static_cast<int>(row0), base_tok) + tid; i < row_end; i += kPlanThreads)
+  for (int i = min(max(static_cast<int>(row0), base_tok), row_end) + tid; i < row_end; i += kPlanThreads)
     p.slots[i] = p.positions[i] = p.requests[i] = -1;
   if (blockIdx.x == 0) {
-    int tk, tt;
-    block_scan2(kept, taken, tk, tt, warp_sums);
+    lost = block_sum(lost, warp_totals);
+    taken = block_sum(taken, warp_totals);
     if (tid == 0) {
       p.starts[p.B] = base_tok;
-      *p.free_head_out = head + tt;
-      *p.dropped = base_tok - tk;
+      *p.free_head_out = head + static_cast<int>(taken);
+      *p.dropped = static_cast<int>(min(lost, 0x7fffffffll));
     }
   }
 }
