@@ -308,9 +308,10 @@ size_t tda_cache4_block_bytes(int64_t page_size, int64_t head_dim);
  * num_free) in request order and written into the table.  Row i of the packed
  * new tokens gets its slot, position and request; slots is -1 for a token that
  * found no page (list or table exhausted), all three are -1 for rows past the
- * last token.  starts ((requests + 1) prefix sums of new_tokens), lengths_out
+ * last token.  Tokens past the last of the `rows` rows are dropped too: they take
+ * no page.  starts ((requests + 1) prefix sums of new_tokens), lengths_out
  * (tokens held afterwards), *free_head_out and *dropped (tokens that found no
- * page) describe the step; starts and *dropped stay at 2^31 - 1 where they
+ * page or no row) describe the step; starts and *dropped stay at 2^31 - 1 where they
  * would pass it.  Negative lengths and counts are taken as 0.  Outputs must not
  * overlap inputs. */
 int tda_plan_pages(const int32_t* lengths, const int32_t* new_tokens, int64_t requests, int32_t* block_table,

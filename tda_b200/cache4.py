@@ -58,7 +58,7 @@ class PagePlan(NamedTuple):
     """One step's plan, all int32 on the device: per packed row its slot,
     position and request (-1 past the last token; slot -1 too where no page was
     left), prefix sums of the new tokens, tokens held afterwards, the free
-    list's new head and the number of tokens that found no page."""
+    list's new head and the number of tokens that found no page or no row."""
     slots: torch.Tensor
     positions: torch.Tensor
     requests: torch.Tensor
@@ -105,7 +105,8 @@ def plan_pages(lengths, new_tokens, block_table, free_pages, free_head, page_siz
     entries of its ``block_table`` row and gets ``new_tokens[r]`` more.  Fresh
     pages are taken from ``free_pages[free_head:]`` in request order and written
     into ``block_table`` in place; the new head is returned, not written back.
-    ``rows``: rows of the packed batch of new tokens (its capacity)."""
+    ``rows``: rows of the packed batch of new tokens (its capacity); tokens past
+    them take no page, are not in ``lengths`` and count as ``dropped``."""
     what = "plan_pages"
     _cuda(what, lengths)
     dev = lengths.device

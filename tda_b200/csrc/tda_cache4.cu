@@ -12,7 +12,9 @@ namespace {
 // ================================================================== page plan
 // Request r holds len[r] tokens in ceil(len / page) pages and gets new[r] more.
 // Pages wanted are handed out in request order from free[head..]; a request
-// that the list cannot serve keeps what it got and drops its last tokens.
+// that the list cannot serve keeps what it got and drops its last tokens, and so
+// does one whose tokens pass the last row: a token without a row is never written,
+// so it takes no page and no length counts it.
 struct PlanParams {
   const int* lengths;
   const int* added;
@@ -45,36 +47,26 @@ __device__ __forceinline__ int add_capped(int a, int b) {
   return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b), 0x7fffffffu));
 }
 
-// Exclusive prefix sums of (a, b) over the block and their totals, capped.
-__device__ void block_scan2(int& a, int& b, int& ta, int& tb, int2* warp_sums) {
+// Exclusive prefix sum of a over the block and its total, capped.
+__device__ void block_scan(int& a, int& total, int* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
-    if (lane >= o) {
-      a = add_capped(a, x);
-      b = add_capped(b, y);
-    }
+    const int x = __shfl_up_sync(0xffffffffu, a, o);
+    if (lane >= o) a = add_capped(a, x);
   }
-  if (lane == 31) warp_sums[warp] = make_int2(a, b);
+  if (lane == 31) warp_sums[warp] = a;
   a = __shfl_up_sync(0xffffffffu, a, 1);
-  b = __shfl_up_sync(0xffffffffu, b, 1);
-  if (lane == 0) a = b = 0;
+  if (lane == 0) a = 0;
   __syncthreads();
-  int pa = 0, pb = 0;
-  ta = tb = 0;
+  int front = 0;
+  total = 0;
 #pragma unroll
   for (int w = 0; w < kPlanThreads / 32; ++w) {
-    const int2 s = warp_sums[w];
-    if (w < warp) {
-      pa = add_capped(pa, s.x);
-      pb = add_capped(pb, s.y);
-    }
-    ta = add_capped(ta, s.x);
-    tb = add_capped(tb, s.y);
+    if (w < warp) front = add_capped(front, warp_sums[w]);
+    total = add_capped(total, warp_sums[w]);
   }
-  a = add_capped(a, pa);
-  b = add_capped(b, pb);
+  a = add_capped(a, front);
   __syncthreads();
 }
 
@@ -98,7 +90,7 @@ __device__ long long block_sum(long long x, long long* warp_sums) {
 __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanParams p) {
   __shared__ int s_start[kPlanScan + 1], s_first[kPlanScan], s_len[kPlanScan], s_after[kPlanScan],
       s_got[kPlanScan];
-  __shared__ int2 warp_sums[kPlanThreads / 32];
+  __shared__ int warp_sums[kPlanThreads / 32];
   __shared__ long long warp_totals[kPlanThreads / 32];
   const int tid = threadIdx.x;
   const int head = max(0, *p.free_head);
@@ -110,24 +102,32 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
   constexpr int kPer = kPlanScan / kPlanThreads;
   for (int r0 = 0; r0 < p.B; r0 += kPlanScan) {
     const int n = min(kPlanScan, p.B - r0);
-    int add[kPer], want[kPer], held[kPer], sa = 0, sw = 0, ta, tw;
+    int add[kPer], fits[kPer], want[kPer], held[kPer], sa = 0, sw = 0, ta, tw;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int r = tid * kPer + i;
-      add[i] = want[i] = held[i] = 0;
+      add[i] = r < n ? max(0, p.added[r0 + r]) : 0;
+      sa = add_capped(sa, add[i]);
+    }
+    block_scan(sa, ta, warp_sums);
+    sa = add_capped(sa, base_tok);
+    int start = sa;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = tid * kPer + i;
+      fits[i] = want[i] = held[i] = 0;
       if (r < n) {
         const int len = max(0, min(p.lengths[r0 + r], p.width * p.page));  // a table holds no more
-        add[i] = max(0, p.added[r0 + r]);
+        fits[i] = min(add[i], max(0, p.rows - start));  // tokens that have a row
         held[i] = (len + p.page - 1) / p.page;
-        const long long last = (static_cast<long long>(len) + add[i] + p.page - 1) / p.page;
+        const long long last = (static_cast<long long>(len) + fits[i] + p.page - 1) / p.page;
         want[i] = static_cast<int>(min(last, static_cast<long long>(p.width))) - held[i];
         s_len[r] = len;
       }
-      sa = add_capped(sa, add[i]);
+      start = add_capped(start, add[i]);
       sw = add_capped(sw, want[i]);
     }
-    block_scan2(sa, sw, ta, tw, warp_sums);
-    sa = add_capped(sa, base_tok);
+    block_scan(sw, tw, warp_sums);
     sw = add_capped(sw, base_page);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
       if (r < n) {
         const int got = min(want[i], max(0, left - sw));
         const int len = s_len[r];
-        const int after = static_cast<int>(min(static_cast<long long>(len) + add[i],
+        const int after = static_cast<int>(min(static_cast<long long>(len) + fits[i],
                                                static_cast<long long>(held[i] + got) * p.page));
         s_start[r] = sa;
         s_first[r] = sw;
