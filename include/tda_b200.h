@@ -336,7 +336,7 @@ int tda_cache4_read(const void* cache, int64_t num_pages, int64_t kv_heads, int6
 #define TDA_MAP_SOFTMAX 0
 #define TDA_MAP_THRESHOLD 1
 
-/* Device scratch of tda_cache4_attention (may be 0). */
+/* Bytes of device scratch tda_cache4_attention needs: may be 0, and is for sizes it refuses. */
 size_t tda_cache4_workspace_size(int map, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                  int64_t page_size, int64_t table_width);
 

@@ -673,7 +673,9 @@ extern "C" {
 
 size_t tda_cache4_workspace_size(int map, int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                  int64_t page_size, int64_t table_width) {
-  if (batch < 1 || kv_heads < 1 || heads % kv_heads != 0 || table_width < 1) return 0;
+  // sizes that tda_cache4_attention refuses need none (and would divide by zero or overflow below)
+  if (batch < 1 || batch > 65535 || kv_heads < 1 || heads < kv_heads || heads > 65535 || heads % kv_heads != 0) return 0;
+  if (tda_cache4_block_bytes(page_size, head_dim) == 0 || table_width < 1 || table_width > 0x7fffffffll / page_size - 8) return 0;
   const int64_t hb = ceil_div(heads / kv_heads, kHeadsPerBlock);
   const int64_t max_len = table_width * page_size;
   const int64_t n = ceil_div(max_len, chunk_tokens(batch, kv_heads * hb, max_len));
