@@ -116,6 +116,21 @@ def _check(q1, q2, k1, k2, v, key_lengths, what="differential_softmax_attention"
             raise RuntimeError(f"{what}: key_lengths must be on the inputs' device")
 
 
+def _check_saved(q1, dout, o12, lse, what="differential_softmax_attention backward"):
+    """What the backward kernels read besides the inputs: by pointer, so a wrong
+    shape, type or device would be read out of bounds."""
+    B, H, Sq, D = q1.shape
+    for name, t, shape in (("dout", dout, (B, H, Sq, D)), ("o12", o12, (2, B, H, Sq, D)), ("lse", lse, (2, B, H, Sq))):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: {name} must be a tensor, got {type(t).__name__}")
+        if t.shape != shape:
+            raise ValueError(f"{what}: {name} must have shape {shape}, got {tuple(t.shape)}")
+        if t.device != q1.device:
+            raise RuntimeError(f"{what}: {name} must be on the inputs' device, got {t.device}")
+        if not (t.dtype.is_floating_point if t is dout else t.dtype == torch.float32 and t.is_contiguous()):
+            raise TypeError(f"{what}: {name} must be {'floating point' if t is dout else 'contiguous fp32'}, got {t.dtype}")
+
+
 def _compute_dtype(ts) -> torch.dtype:
     common = ts[0].dtype
     for t in ts[1:]:
@@ -189,9 +204,7 @@ def sdiff_backward(q1, q2, k1, k2, v, dout, o12, lse, lambda_param, scale=None, 
     the forward's (o12, lse); gradients in the compute type, ``dlam`` fp32 (B,
     H), None when not asked for."""
     _check(q1, q2, k1, k2, v, key_lengths)
-    if dout.shape != q1.shape:
-        raise ValueError(f"differential_softmax_attention: dout must have shape {tuple(q1.shape)}, got "
-                         f"{tuple(dout.shape)}")
+    _check_saved(q1, dout, o12, lse)
     B, H, Sq, D = q1.shape
     Hkv, Sk = k1.shape[1], k1.shape[2]
     dt = _compute_dtype((q1, q2, k1, k2, v))
