@@ -219,6 +219,8 @@ __global__ void __launch_bounds__(256) sdiff_simt_fwd_kernel(const SdParams p) {
 #pragma unroll
       for (int x = 1; x < 16; x <<= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], x);
       const int i = i0 + ty * C::R + r;
+      // keys, but -infinity for every score: no softmax, where a row without keys is zeros
+      if (sum[r] == 0.f && sees(p, i, 0, len)) sum[r] = __uint_as_float(0x7fffffffu);
       const float inv = sum[r] == 0.f ? 0.f : 1.f / sum[r];
       if (tx == 0 && i < p.Sq && p.lse) p.lse[row_at(p, m, b, h, i)] = sum[r] == 0.f ? kInf : top[r] + log2f(sum[r]);
       const long long at = row_at(p, 0, b, h, i) * D;

@@ -125,13 +125,21 @@ __device__ __forceinline__ void zero_row(uint8_t* tile, int r) {
     for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + x * (kTile * 128) + r * 128 + 16 * c) = make_uint4(0, 0, 0, 0);
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where an operand is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // 2^x of a pair for -125 <= x <= 126 on the FMA pipe (below: 2^-125): 2^n by the
 // exponent field, 2^f, |f| <= 1/2, by the polynomial of least relative error,
-// 7.5e-5 (degree 3, bf16 weights) or 2.6e-6 (degree 4, fp16 weights).
+// 7.5e-5 (degree 3, bf16 weights) or 2.6e-6 (degree 4, fp16 weights).  Of a NaN it
+// gives the largest finite number: r and p are then the NaN 0x7fffffff, the only
+// one that fp32 arithmetic makes, and their bits add up to 0x7f7fffff.
 template <bool F16>
 __device__ __forceinline__ float2 poly_ex2(float2 x) {
-  x.x = fmaxf(x.x, -125.0f);
-  x.y = fmaxf(x.y, -125.0f);
+  x.x = max_nan(x.x, -125.0f);
+  x.y = max_nan(x.y, -125.0f);
   const float2 r = __fadd2_rn(x, make_float2(12582912.0f, 12582912.0f));  // 1.5 2^23: the last bits are n
   const float2 n = __fadd2_rn(r, make_float2(-12582912.0f, -12582912.0f));
   const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);

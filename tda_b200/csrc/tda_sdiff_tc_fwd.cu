@@ -163,6 +163,16 @@ __device__ __forceinline__ void exponentials(const uint32_t (&s)[32], float c, f
   tmem_st16(col, w);
 }
 
+// The polynomial exponential is finite whatever the score, so that rows which have no
+// softmax are found by their sum and their maximum, off the common path: a sum
+// of weights (2^30 of 2^8 at most) is larger than 2^100 if a score was NaN
+// (poly_ex2), and after a score of +infinity the maximum is.  Both rows become NaN, as the
+// definition has it, and so does a row whose scores are all -infinity: its maximum is,
+// and the polynomial's 2^-125 are no weights.
+__device__ __forceinline__ float checked(float sum, float top) {
+  return sum < 0x1p100f && top < __builtin_huge_valf() ? sum : __uint_as_float(0x7fffffffu);
+}
+
 template <int D, bool F16>
 __device__ void softmax(const SdTcParams& tp, uint8_t* smem, FBars* bars, const WaitCtl& ctl, uint32_t tmem, int b, int h, int qt,
                         int n, int len, int warp, int lane) {
@@ -207,7 +217,7 @@ __device__ void softmax(const SdTcParams& tp, uint8_t* smem, FBars* bars, const 
       const float f = grow_m ? fast_ex2(top - now) : 1.0f;  // 0 for a row's first keys
       if (grow_m) top = now;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sum[i] = __fmul2_rn(sum[i], make_float2(f, f));
+      for (int i = 0; i < 2; ++i) sum[i] = __fmul2_rn(make_float2(checked(sum[i].x, top), checked(sum[i].y, top)), make_float2(f, f));
       if (j > 0) {
 #pragma unroll
         for (int x = 0; x < D; x += 16) {
@@ -252,7 +262,9 @@ __device__ void softmax(const SdTcParams& tp, uint8_t* smem, FBars* bars, const 
   }
   // epilogue: out = O1 / l1 - lambda O2 / l2, a warpgroup half of the columns
   float* inv = reinterpret_cast<float*>(smem + C::kOffBar + 1024);
-  const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+  const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+  float l = checked(all, top);
+  if (top == -__builtin_huge_valf() && all < 1.0f) l = last >= 0 ? __uint_as_float(0x7fffffffu) : 0.f;
   inv[m * kTile + row] = l == 0.f ? 0.f : 1.0f / l;
   const long long bh = static_cast<long long>(b) * p.H + h, n_bh = static_cast<long long>(p.B) * p.H;
   if (p.lse && grow < p.Sq) p.lse[(m * n_bh + bh) * p.Sq + grow] = l == 0.f ? __builtin_huge_valf() : top + log2f(l);
