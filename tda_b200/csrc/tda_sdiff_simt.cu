@@ -246,7 +246,8 @@ __global__ void __launch_bounds__(256) sdiff_simt_fwd_kernel(const SdParams p) {
 template <typename T>
 __device__ __forceinline__ void put_aux(uint8_t* table, int r, float x) {
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
-  float rest = fmaxf(x / aux_unit(kF16), kF16 ? -65504.0f : -1e30f);  // a row without keys: what no score reaches
+  float rest = x / aux_unit(kF16);
+  if (rest < (kF16 ? -65504.0f : -1e30f)) rest = kF16 ? -65504.0f : -1e30f;  // a row without keys: what no score reaches.  A NaN stays
   T part[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {

@@ -135,8 +135,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN where an op
 // exponent field, 2^f, |f| <= 1/2, by the polynomial of least relative error,
 // 7.5e-5 (degree 3, bf16 weights) or 2.6e-6 (degree 4, fp16 weights).  Of a NaN it
 // gives the largest finite number: r and p are then the NaN 0x7fffffff, the only
-// one that fp32 arithmetic makes, and their bits add up to 0x7f7fffff.
-template <bool F16>
+// one that fp32 arithmetic makes, and their bits add up to 0x7f7fffff.  With
+// KEEP_NAN a multiplication by 2^n takes the addition's place, the same bits for
+// numbers, and a NaN stays one.
+template <bool F16, bool KEEP_NAN = false>
 __device__ __forceinline__ float2 poly_ex2(float2 x) {
   x.x = max_nan(x.x, -125.0f);
   x.y = max_nan(x.y, -125.0f);
@@ -154,6 +156,9 @@ __device__ __forceinline__ float2 poly_ex2(float2 x) {
     p = __ffma2_rn(p, f, make_float2(0.6932609677314758f, 0.6932609677314758f));
     p = __ffma2_rn(p, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
   }
+  if constexpr (KEEP_NAN)
+    return __fmul2_rn(p, make_float2(__uint_as_float((__float_as_uint(r.x) << 23) + 0x3f800000u),
+                                     __uint_as_float((__float_as_uint(r.y) << 23) + 0x3f800000u)));
   return make_float2(__uint_as_float((__float_as_uint(r.x) << 23) + __float_as_uint(p.x)),
                      __uint_as_float((__float_as_uint(r.y) << 23) + __float_as_uint(p.y)));
 }

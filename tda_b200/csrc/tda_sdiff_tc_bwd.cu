@@ -267,7 +267,8 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
 #pragma unroll
           for (int y = 0; y < 32; y += 2) {
             const float2 z = __fmul2_rn(f2u(s[y], s[y + 1]), make_float2(c, c));  // s - L / c
-            const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
+            // a row without a softmax has a NaN for L, and its weights go into dV by themselves
+            const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16, true>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
             const float2 r = __fmul2_rn(ez, make_float2(wt, wt));
             pr[y] = r.x;
             pr[y + 1] = r.y;
@@ -556,6 +557,7 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
 #pragma unroll
         for (int y = 0; y < 32; y += 2) {
           const float2 z = __ffma2_rn(f2u(s[y], s[y + 1]), make_float2(c, c), make_float2(minus_l[m], minus_l[m]));
+          // where L is NaN so is D, which the weight is multiplied by below
           const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
           pr[y] = ez.x;
           pr[y + 1] = ez.y;
