@@ -19,8 +19,12 @@
 namespace tda {
 
 constexpr int kAuxTileBytes = 128 * 16 * 2;
-// fp16 holds -L / c up to 2^24 as a multiple of this
-constexpr float aux_unit(bool f16) { return f16 ? 256.0f : 1.0f; }
+// The units of the product tables' columns, three columns a unit.  bf16 has the
+// exponents of fp32 and needs one.  fp16 holds numbers from 1 to 65504 to 33 bits in three
+// values, and D is as small as the gradient that comes in: a number takes the columns
+// of the largest unit that it is not below (the last one below 2^-14 too, to 2^-38).
+constexpr int aux_units(bool f16) { return f16 ? 3 : 1; }
+constexpr float aux_unit(bool f16, int g) { return !f16 || g == 1 ? 1.0f : g == 0 ? 0x1p15f : 0x1p-14f; }
 
 struct SdView {  // (batch, head, seq, dim) view: element strides, dim contiguous
   const void* p;
@@ -46,7 +50,7 @@ struct SdParams {
   float* table;    // [2][B][H][pad / 128][2][128]: -L_m, then -D_m of each row; -inf, 0 past Sq
   // The same numbers as products read them (16-bit types): per tile of 128 rows
   // [128][16] for -L / c, then for -D, three values a row that add up to it over
-  // aux_unit, in core-matrix order.
+  // their columns' aux_unit and zeros, in core-matrix order.
   void* aux;
   int pad;         // Sq rounded up to a tile of 128
   void* dq[2];     // contiguous, of the inputs' type

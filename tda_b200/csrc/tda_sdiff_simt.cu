@@ -246,17 +246,26 @@ __global__ void __launch_bounds__(256) sdiff_simt_fwd_kernel(const SdParams p) {
 template <typename T>
 __device__ __forceinline__ void put_aux(uint8_t* table, int r, float x) {
   constexpr bool kF16 = !std::is_same<T, __nv_bfloat16>::value;
-  float rest = x / aux_unit(kF16);
-  if (rest < (kF16 ? -65504.0f : -1e30f)) rest = kF16 ? -65504.0f : -1e30f;  // a row without keys: what no score reaches.  A NaN stays
-  T part[8];
+  int g = 0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    store1(part + k, k < 3 ? rest : 0.f);
-    if (k < 3) rest -= static_cast<float>(part[k]);
+  for (int u = 0; u + 1 < aux_units(kF16); ++u) g += !(fabsf(x) >= aux_unit(kF16, u));
+  float rest = x / aux_unit(kF16, g);
+  if (kF16 && fabsf(rest) > 65504.0f) rest = __uint_as_float(0x7fffffffu);  // no fp16 values add up to it: not a wrong gradient in silence
+  if (x == -kInf) rest = kF16 ? -65504.0f : -1e30f;  // a row without keys: what no score reaches
+  float part[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    T v;
+    store1(&v, rest);
+    part[k] = static_cast<float>(v);
+    rest -= part[k];
   }
+  alignas(16) T column[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) store1(column + k, k / 3 == g && k / 3 < aux_units(kF16) ? part[k % 3] : 0.f);
   uint4* at = reinterpret_cast<uint4*>(table + (r >> 3) * 256 + (r & 7) * 16);
-  at[0] = *reinterpret_cast<uint4*>(part);
-  at[8] = make_uint4(0, 0, 0, 0);
+  at[0] = reinterpret_cast<uint4*>(column)[0];
+  at[8] = reinterpret_cast<uint4*>(column)[1];
 }
 
 // D_1 = dout . O_1 and D_2 = dout . O_2, a warp a row.

@@ -96,8 +96,8 @@ __device__ __forceinline__ void mma_weights(uint32_t dcol, uint32_t wcol, uint32
 
 // One more step of 16 along the contracted dimension: D[dcol] += ones aux^T, with
 // `aux` a [128][16] table in shared memory (unswizzled: 8 x 16-byte core matrices,
-// 128 bytes apart along the columns, 256 along the rows) whose first three columns
-// add up to a number a row, and `ones` of the same form.  It subtracts L or D of
+// 128 bytes apart along the columns, 256 along the rows) whose columns times their
+// units add up to a number a row, and `ones` the units, of the same form.  It subtracts L or D of
 // the query from a column of scores without a load in the threads that use them:
 // 16 shared-memory loads a thread and step cost more than the product.
 template <bool F16>

@@ -371,12 +371,17 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
     fence_mbar_init();
     if (w.per_map > 0) kv_prime<D, F16>(tp, smem, bars, w);
   }
-  if (threadIdx.x >= 128 && threadIdx.x < 256) {  // the unit in three columns of every row
+  if (threadIdx.x >= 128 && threadIdx.x < 256) {  // the columns' units in every row
     const int r = threadIdx.x - 128;
-    const uint32_t u = pack2<F16>(aux_unit(F16), aux_unit(F16));
+    uint32_t u[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const auto unit = [](int x) { return x / 3 < aux_units(F16) ? aux_unit(F16, x / 3) : 0.f; };
+      u[k] = pack2<F16>(unit(2 * k), unit(2 * k + 1));
+    }
     uint4* at = reinterpret_cast<uint4*>(smem + C::kOffOnes + (r >> 3) * 256 + (r & 7) * 16);
-    at[0] = make_uint4(u, u & 0xffffu, 0, 0);
-    at[8] = make_uint4(0, 0, 0, 0);
+    at[0] = make_uint4(u[0], u[1], u[2], u[3]);
+    at[8] = make_uint4(u[4], u[5], u[6], u[7]);
     fence_proxy_async_smem();
   }
   if (warp == kIssue) {
