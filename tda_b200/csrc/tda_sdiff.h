@@ -59,6 +59,31 @@ struct SdParams {
   float* dlam;     // [B][H], or null
 };
 
+#ifdef __CUDACC__
+// fp16: the largest finite |dout| of a kv head's query heads and the largest finite
+// |v| of its keys, two words that hold an fp16 number each.  They lie in the last
+// four columns of the first row of the head's D tables, whose unit is zero.
+__device__ __forceinline__ uint32_t* sizes_of(const SdParams& p, int b, int kvh) {
+  const long long tile = (static_cast<long long>(b) * p.H + kvh * p.group) * (p.pad / kTile);
+  return reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(p.aux) + (tile * 2 + 1) * kAuxTileBytes + 128 + 8);
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+// The e with x <= 2^e for 0 <= x, within +-60
+__device__ __forceinline__ int exponent_above(float x) {
+  return min(max(static_cast<int>(__float_as_uint(x) >> 23) - 126, -60), 60);
+}
+// fp16: dS enters its products times 2^e.  |dP - D| <= 2 |dout| |v| <= 2 head_dim max|dout|
+// max|v|, so with this e no dS passes 2^15, and one 2^29 below the largest possible is
+// still a normal number: gradients of any size keep their bits.
+__device__ __forceinline__ int ds_exponent(const SdParams& p, int b, int kvh, int D, float largest_weight) {
+  const uint32_t* s = sizes_of(p, b, kvh);
+  float g, v;
+  asm("cvt.f32.f16 %0, %1;" : "=f"(g) : "h"(static_cast<unsigned short>(s[0])));
+  asm("cvt.f32.f16 %0, %1;" : "=f"(v) : "h"(static_cast<unsigned short>(s[1])));
+  return min(15 - exponent_above(2.0f * D * g * v * largest_weight), 60);
+}
+#endif
+
 cudaError_t launch_sdiff_simt_fwd(const SdParams& p, int dtype, int D, cudaStream_t s);
 cudaError_t launch_sdiff_simt_bwd(const SdParams& p, int dtype, int D, cudaStream_t s);
 // D_1, D_2 from dout and o12, and dlambda where asked for

@@ -309,6 +309,40 @@ __global__ void __launch_bounds__(256) sdiff_delta_kernel(const SdParams p) {
   }
 }
 
+// The numbers of sizes_of, after the tables are written: a block a tile of 128 rows
+// of dout or v.  A maximum is the same in any order.  Infinities and NaN, which
+// spoil what they enter anyway, do not take the others' bits.
+template <int D>
+__global__ void __launch_bounds__(256) sdiff_sizes_kernel(const SdParams p) {
+  const int n_q = (p.Sq + kTile - 1) / kTile, n_k = (p.Sk + kTile - 1) / kTile;
+  long long block = blockIdx.x;
+  const bool values = block >= static_cast<long long>(p.B) * p.H * n_q;
+  if (values) block -= static_cast<long long>(p.B) * p.H * n_q;
+  const SdView& x = values ? p.v : p.dout;
+  const int heads = values ? p.Hkv : p.H, tiles = values ? n_k : n_q;
+  const int h = static_cast<int>(block / tiles % heads), b = static_cast<int>(block / tiles / heads);
+  const int r0 = static_cast<int>(block % tiles) * kTile, end = min(r0 + kTile, values ? keys_of(p, b) : p.Sq);
+  const __half* base = static_cast<const __half*>(x.p) + b * x.sb + h * x.sh + threadIdx.x % (D / 8) * 8;
+  uint32_t top = 0;
+#pragma unroll 4
+  for (int r = r0 + threadIdx.x / (D / 8); r < end; r += 256 / (D / 8)) {
+    const uint4 u = *reinterpret_cast<const uint4*>(base + r * x.ss);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = (i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w) & 0x7fff7fffu;
+      top = __vmaxu2(top, m & ~__vcmpgeu2(m, 0x7c007c00u));
+    }
+  }
+  __shared__ uint32_t part[8];
+  top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) top = max(top, part[w]);
+    if (top) atomicMax(sizes_of(p, b, values ? h : h / p.group) + values, top);
+  }
+}
+
 // dlambda of one (batch, head): a fixed tree over its rows, the same sum every time
 __global__ void __launch_bounds__(256) sdiff_dlam_kernel(const SdParams p) {
   __shared__ float part[256];
@@ -475,6 +509,13 @@ cudaError_t delta(const SdParams& p, cudaStream_t s) {
   constexpr int kPerBlock = 8 * (32 / (D / 4 < 32 ? D / 4 : 32));
   sdiff_delta_kernel<T, D><<<static_cast<unsigned>(ceil_div(rows, kPerBlock)), 256, 0, s>>>(p);
   cudaError_t e = cudaGetLastError();
+  if constexpr (std::is_same<T, __half>::value && (D == 64 || D == 128)) {
+    if (e == cudaSuccess && p.aux) {
+      const long long blocks = static_cast<long long>(p.B) * p.H * ceil_div(p.Sq, kTile) + static_cast<long long>(p.B) * p.Hkv * ceil_div(p.Sk, kTile);
+      sdiff_sizes_kernel<D><<<static_cast<unsigned>(blocks), 256, 0, s>>>(p);
+      e = cudaGetLastError();
+    }
+  }
   if (e != cudaSuccess || !p.dlam) return e;
   sdiff_dlam_kernel<<<static_cast<unsigned>(p.B * p.H), 256, 0, s>>>(p);
   return cudaGetLastError();

@@ -246,6 +246,16 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
   const bool dead = key >= len;          // past the sequence's length: no weight, whatever K and V hold there
   const bool lone = len <= 1;            // weight 1 whatever the score: no dS
   const float c = p.c;
+  // fp16 keeps its bits between 2^-14 and 2^16 alone: the weights enter times 2^k, at
+  // most 2^14 with lambda, dS times 2^e, and the accumulators are scaled back.
+  int k = 0, e = 0;
+  if constexpr (F16) {
+    float largest = 1.0f;
+    for (int h = w.kvh * p.group; h < (w.kvh + 1) * p.group; ++h) largest = fmaxf(largest, fabsf(lambda_at(p.lam, w.b, h)));
+    k = 14 - exponent_above(largest);
+    e = ds_exponent(p, w.b, w.kvh, D, largest);
+  }
+  const float kf = static_cast<float>(k), more = exp2i(e - k);
   bool ok = true;
   int t = 0;
   if (w.per_map > 0) ok = wait_inline_warp(&bars->v_full, 0, ctl, ST_KW);
@@ -266,7 +276,8 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
           tmem_wait_ld();
 #pragma unroll
           for (int y = 0; y < 32; y += 2) {
-            const float2 z = __fmul2_rn(f2u(s[y], s[y + 1]), make_float2(c, c));  // s - L / c
+            const float2 x = f2u(s[y], s[y + 1]);  // s - L / c
+            const float2 z = F16 ? __ffma2_rn(x, make_float2(c, c), make_float2(kf, kf)) : __fmul2_rn(x, make_float2(c, c));
             // a row without a softmax has a NaN for L, and its weights go into dV by themselves
             const float2 ez = (y / 2 * kPolyPairs) % 8 < kPolyPairs ? poly_ex2<F16, true>(z) : make_float2(fast_ex2(z.x), fast_ex2(z.y));
             const float2 r = __fmul2_rn(ez, make_float2(wt, wt));
@@ -296,7 +307,9 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
           tmem_wait_ld();
 #pragma unroll
           for (int y = 0; y < 32; y += 2) {
-            const float2 r = __fmul2_rn(make_float2(pr[y], pr[y + 1]), f2u(s[y], s[y + 1]));  // P (dP - D)
+            float2 r = make_float2(pr[y], pr[y + 1]);
+            if constexpr (F16) r = __fmul2_rn(r, make_float2(more, more));
+            r = __fmul2_rn(r, f2u(s[y], s[y + 1]));  // P (dP - D)
             pr[y] = r.x;
             pr[y + 1] = r.y;
           }
@@ -316,8 +329,8 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
     if (ok && w.per_map > 0) ok = wait_inline_warp(&bars->map_done, m, ctl, ST_KW);
     tc_fence_after();
     if (ok) {
-      stage_accumulator<D, F16>(smem, tmem + lane_off + C::kDK, row, wg, p.scale, w.per_map == 0);
-      if (m == 1) stage_accumulator<D, F16>(smem + C::kTileBytes, tmem + lane_off + C::kDV, row, wg, 1.0f, w.per_map == 0);
+      stage_accumulator<D, F16>(smem, tmem + lane_off + C::kDK, row, wg, p.scale * exp2i(-e), w.per_map == 0);
+      if (m == 1) stage_accumulator<D, F16>(smem + C::kTileBytes, tmem + lane_off + C::kDV, row, wg, exp2i(-k), w.per_map == 0);
       fence_proxy_async_smem();
     }
     tc_fence_before();
@@ -542,6 +555,13 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
     minus_d[m] = t[kTile];
   }
   const float c = p.c;
+  int e = 0;  // dS enters the products times 2^e, by the exponent of the weights
+  if constexpr (F16) {
+    e = ds_exponent(p, b, h / p.group, D, 1.0f);
+    minus_l[0] += static_cast<float>(e);
+    minus_l[1] += static_cast<float>(e);
+  }
+  const float back = p.scale * exp2i(-e);
   const int last = p.causal ? min(len - 1, grow + off) : len - 1;
   bool ok = true;
   for (int t = 0; t < n && ok; ++t) {
@@ -608,8 +628,8 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
   tc_fence_after();
   uint8_t* stage = smem + C::kOffRing;
   if (ok) {
-    const float w2 = -lambda_at(p.lam, b, h) * p.scale;
-    stage_accumulator<D, F16>(stage, tmem + lane_off + C::dq_col(0), row, wg, p.scale, n == 0);
+    const float w2 = -lambda_at(p.lam, b, h) * back;
+    stage_accumulator<D, F16>(stage, tmem + lane_off + C::dq_col(0), row, wg, back, n == 0);
     stage_accumulator<D, F16>(stage + C::kTileBytes, tmem + lane_off + C::dq_col(1), row, wg, w2, n == 0);
     fence_proxy_async_smem();
   }
