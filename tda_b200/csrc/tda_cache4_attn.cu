@@ -30,7 +30,10 @@
 // element to [1, 2): exact but for elements 2^-21 below it.
 // V's scale goes into the weight, w = p s, rounded to fp16 (2^-12) relative to a
 // running bound M >= log2 of the largest w so far (minus 8): weights lie below
-// 2^8 and small scales do not underflow.  The threshold form forms its whole
+// 2^8 and small scales do not underflow.  As long as all scales are zero, M bounds p
+// alone (no weight is added yet, and a bound on w would be -infinity), and the first
+// scale that is not zero joins it; M stays above -120, below which 2^-M
+// has no float and w adds nothing to a 16-bit output.  The threshold form forms its whole
 // weight (p1 - lambda p2) s at once, which takes the columns of one map, so the
 // other four carry what rounding left: nothing is lost where the maps cancel.
 #include <cuda_bf16.h>
@@ -406,8 +409,9 @@ __global__ void __launch_bounds__(32 * kWarps, DC<D>::kResident) cache4_attn_ker
       for (int y = 1; y < 32; y <<= 1) big = max_bf16x2(big, __shfl_xor_sync(0xffffffffu, big, y));
       const float2 halves = unpack_bf16x2(big);
       const float largest = fmaxf(halves.x, halves.y);
+      const float lb = largest > 0.f ? fast_lg2(fmaxf(largest, 0x1p-100f)) : 0.f;
+      const float first = bound == 0u ? lb : 0.f;  // M bounds p alone so far
       bound = pack_bf16x2(largest, largest);
-      const float lb = fast_lg2(fmaxf(largest, 0x1p-100f));
       float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -418,7 +422,8 @@ __global__ void __launch_bounds__(32 * kWarps, DC<D>::kResident) cache4_attn_ker
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));  // a head's two columns hold one weight
           x = x > 0.f ? fast_lg2(x) : -kInf;
         }
-        x = fmaxf(x + lb, m[c]);
+        x = fmaxf(x + lb, m[c] + first);
+        if constexpr (THR) x = x == -kInf ? x : fmaxf(x, -120.f);
         f[c] = m[c] == x ? 1.f : fast_ex2(m[c] - x);
         m[c] = x;
         l[c] *= f[c];
