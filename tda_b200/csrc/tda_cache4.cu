@@ -290,19 +290,27 @@ struct Elem<__half> {
 // whole number or one beside it; the remainder 7 x - c amax is exact in fp32 for
 // bf16 and fp16 inputs and says which: past amax / 2 the neighbour is nearer, and
 // at amax / 2 (a tie) it is taken when c is odd.  Returned with other bits above.
+// Of an fp32 input (WIDE) 7 x has up to 27 bits: its rounding rest is kept beside it,
+// c amax is subtracted from the rounded part exactly (they agree to amax / 2), and the
+// distance from amax / 2, exact as well, is corrected by the rest.
+template <bool WIDE>
 __device__ __forceinline__ uint32_t nibble(float x, float amax, float half, float inv7) {
   const float shifted = fmaf(x, inv7, 12582920.0f);
   const uint32_t n = __float_as_uint(shifted);
-  const float rem = fmaf(-(shifted - 12582920.0f), amax, 7.0f * x);
-  const float edge = __uint_as_float(__float_as_uint(half) - (n & 1u));
+  const float seven = 7.0f * x, rem = fmaf(-(shifted - 12582920.0f), amax, seven);
   const int step = (static_cast<int>(__float_as_uint(rem)) >> 31) | 1;
+  if constexpr (WIDE) {
+    const float past = (fabsf(rem) - half) + static_cast<float>(step) * fmaf(7.0f, x, -seven);
+    return n + (past > 0.f || (past == 0.f && (n & 1u)) ? step : 0);
+  }
+  const float edge = __uint_as_float(__float_as_uint(half) - (n & 1u));
   return n + (fabsf(rem) > edge ? step : 0);
 }
 
 __device__ __forceinline__ uint32_t max_bits(uint32_t a, float x) { return max(a, __float_as_uint(x) & 0x7fffffffu); }
 
 // one word of codes and the scales of its runs' groups from 8 elements
-template <int D, bool V>
+template <int D, bool V, bool WIDE>
 __device__ __forceinline__ uint32_t quantise(float (&x)[8], bool normalize, float (&sc)[2]) {
   // largest magnitude of each run's group, as bits so that a NaN wins
   uint32_t m[2] = {0, 0};
@@ -343,7 +351,7 @@ __device__ __forceinline__ uint32_t quantise(float (&x)[8], bool normalize, floa
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int at = 4 * nibble_of<V>(r, j);
-      part |= (nibble(x[4 * r + j], amax, half, inv7) << at) & (15u << at);
+      part |= (nibble<WIDE>(x[4 * r + j], amax, half, inv7) << at) & (15u << at);
     }
     // a group of zeros, or one that holds an infinity or a NaN (whose scale is NaN): codes of zero
     uint32_t zeros = 0;
@@ -381,7 +389,7 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, const T* x, l
 #pragma unroll
   for (int u = 0; u < C::kUnroll; ++u) {
     float sc[2];
-    const uint32_t word = quantise<D, V>(v[u], p.normalize != 0, sc);
+    const uint32_t word = quantise<D, V, sizeof(T) == 4>(v[u], p.normalize != 0, sc);
     if (static_cast<unsigned>(slot[u]) >= static_cast<unsigned>(p.num_slots)) continue;
     uint8_t* slab = p.cache + slab_of<D>(slot[u], h, p.heads, p.page_log2);
     const int r = slot[u] % kSlab4;
