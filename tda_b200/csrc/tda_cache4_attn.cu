@@ -27,7 +27,9 @@
 // nibbles of the larger offset: its weights are powers of s - tau, where the error
 // would show (4e-4 of the output; a bf16 output's own rounding is 2e-3).  K's scale multiplies a group's fp32 product.
 // q enters as fp16 after division by a power of two that brings its largest
-// element to [1, 2): exact but for elements 2^-21 below it.
+// element to [2^14, 2^15), next to the end of fp16's range, half of its dims a
+// sixteenth of that: an element is rounded there by 2^-25 at most, so a bf16
+// element is exact down to 2^-27 of the largest, an fp16 one to 2^-24.
 // V's scale goes into the weight, w = p s, rounded to fp16 (2^-12) relative to a
 // running bound M >= log2 of the largest w so far (minus 8): weights lie below
 // 2^8 and small scales do not underflow.  As long as all scales are zero, M bounds p
@@ -287,9 +289,10 @@ __global__ void __launch_bounds__(32 * kWarps, DC<D>::kResident) cache4_attn_ker
       ss += __shfl_xor_sync(0xffffffffu, ss, o);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
-    // 2^e <= top < 2^(e + 1); both powers are normal numbers for any top but 0
-    const uint32_t e = min(max(__float_as_uint(top) >> 23, 2u), 252u);
-    const float up = __uint_as_float(e << 23), down = __uint_as_float((254u - e) << 23);
+    // 2^e <= top < 2^(e + 1): down = 2^(14 - e), up its inverse, both normal numbers for
+    // any top; a query of zeros keeps its size
+    const uint32_t e = top > 0.f ? min(max(__float_as_uint(top) >> 23, 15u), 252u) : 127u + 14u;
+    const float up = __uint_as_float((e - 14u) << 23), down = __uint_as_float((268u - e) << 23);
     float sum[W];
 #pragma unroll
     for (int s = 0; s < 2 * W; ++s) {
