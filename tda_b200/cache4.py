@@ -9,7 +9,8 @@ it, and attention of one new token a request over it.
 Everything stays on the device and runs on the current stream, nothing is read
 back, so a step can be captured in a CUDA graph.  K1, K2 and V are held as
 4-bit codes in groups of 32 along the head dimension with a bf16 scale (4.5
-bits an element).  There is no CPU fallback.
+bits an element).  There is no CPU fallback, and no gradient: the cache holds
+values alone, and a backward through the attention raises.
 """
 from __future__ import annotations
 
@@ -187,6 +188,21 @@ def _workspace_size(*sizes) -> int:
     return _lib.load().tda_cache4_workspace_size(*sizes)
 
 
+class _NoBackward(torch.autograd.Function):
+    """``out`` as a result of inputs that want a gradient: asking for it raises
+    where an output without a graph would leave it out in silence."""
+
+    @staticmethod
+    def forward(ctx, what, out, *inputs):
+        ctx.what = what
+        return out.detach()
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise RuntimeError(f"{ctx.what} has no backward: it serves from a 4-bit cache (train with "
+                           "differential_softmax_attention or differential_threshold_rela_triton)")
+
+
 def _attend(what, kind, q1, q2, cache, block_table, lengths, lambda_param, scale, beta, relu_power):
     for t in (q1, q2):
         _cuda(what, t)
@@ -217,6 +233,9 @@ def _attend(what, kind, q1, q2, cache, block_table, lengths, lambda_param, scale
            cache.page_size, block_table.data_ptr(), stride, width, lengths.data_ptr(), lp, lc, lsb, lsh, lv, scale,
            beta, relu_power, int(cache.normalize_keys), None if ws is None else ws.data_ptr(), ws_n,
            _ops._status_word(dev).data_ptr())
+    if torch.is_grad_enabled() and (q1.requires_grad or q2.requires_grad or
+                                    isinstance(lambda_param, torch.Tensor) and lambda_param.requires_grad):
+        return _NoBackward.apply(what, out, q1, q2, lambda_param)
     return out
 
 
@@ -224,7 +243,8 @@ def cache4_softmax_attention(q1, q2, cache: Cache4, block_table, lengths, lambda
     """One new token a request: (softmax(scale q1 K1^T) - lambda softmax(scale
     q2 K2^T)) V over the request's ``lengths`` cached tokens, the new one among
     them.  q1, q2: (batch, heads, head_dim) bf16 / fp16; lambda as in
-    ``differential_softmax_attention``; a request of length 0 gives zeros."""
+    ``differential_softmax_attention``; a request of length 0 gives zeros.  Not
+    differentiable: a backward through it raises."""
     sc = 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale)
     if cache.normalize_keys:
         raise ValueError("cache4_softmax_attention: the cache holds normalized keys (made for the threshold form)")
@@ -238,7 +258,8 @@ def cache4_threshold_attention(q1, q2, cache: Cache4, block_table, lengths, beta
     clamp(lambda, 0, 1) P2) V with P = ReLU(q K^T - tau)^p and tau = beta
     sqrt(2 log(lengths) / head_dim); q is L2-normalized when the cache
     normalizes its keys.  ``beta`` and ``relu_power`` are floats (or one-element
-    tensors, read on the host)."""
+    tensors, read on the host).  Not differentiable: a backward through it
+    raises."""
     b = float(beta.item()) if isinstance(beta, torch.Tensor) else float(beta)
     p = float(relu_power.item()) if isinstance(relu_power, torch.Tensor) else float(relu_power)
     return _attend("cache4_threshold_attention", _lib.TDA_MAP_THRESHOLD, q1, q2, cache, block_table, lengths,
