@@ -262,12 +262,21 @@ class DifferentialSoftmaxFunction(torch.autograd.Function):
         return (*cast, dlam_like(g[5], lam_t) if need else None, None, None, None)
 
 
+def _traced(q1) -> bool:
+    """Whether the call is recorded or run without data (torch.compile, make_fx,
+    fake and meta tensors, dispatch modes): then it is the registered operator.
+    A plain call goes past it: small calls are bound by the host."""
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or isinstance(q1, torch.Tensor) and (type(q1) not in (torch.Tensor, torch.nn.Parameter) or q1.is_meta))
+
+
 def differential_softmax_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=True, key_lengths=None):
     """out = (softmax(scale q1 k1^T) - lambda softmax(scale q2 k2^T)) v, q1's
     shape and dtype; differentiable in q1, q2, k1, k2, v and lambda.  ``scale``
-    defaults to head_dim ** -0.5.  See the module's docstring.  Under
-    torch.compile it runs as the operator ``tda::sdiff_fwd``."""
-    if torch.compiler.is_compiling():
+    defaults to head_dim ** -0.5.  See the module's docstring.  Where it is
+    traced (torch.compile, make_fx, fake tensors) it is the operator
+    ``tda::sdiff_fwd``."""
+    if _traced(q1):
         lam = lambda_param if isinstance(lambda_param, torch.Tensor) else torch.tensor(float(lambda_param))
         sc = 1.0 / math.sqrt(q1.shape[-1]) if scale is None else float(scale)
         return torch.ops.tda.sdiff_fwd(q1, q2, k1, k2, v, lam, sc, bool(causal), key_lengths)[0]
