@@ -262,6 +262,10 @@ class DifferentialSoftmaxFunction(torch.autograd.Function):
         return (*cast, dlam_like(g[5], lam_t) if need else None, None, None, None)
 
 
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
+
+
 def _traced(q1) -> bool:
     """Whether the call is recorded or run without data (torch.compile, make_fx,
     fake and meta tensors, dispatch modes): then it is the registered operator.
@@ -279,9 +283,9 @@ def differential_softmax_attention(q1, q2, k1, k2, v, lambda_param, scale=None, 
     if _traced(q1):
         lam = lambda_param if isinstance(lambda_param, torch.Tensor) else torch.tensor(float(lambda_param))
         sc = 1.0 / math.sqrt(q1.shape[-1]) if scale is None else float(scale)
-        return torch.ops.tda.sdiff_fwd(q1, q2, k1, k2, v, lam, sc, bool(causal), key_lengths)[0]
-    if not (torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                            for t in (q1, q2, k1, k2, v, lambda_param))):
+        return torch.ops.tda.sdiff_fwd(q1, q2, k1, k2, v, lam, sc, bool(causal), key_lengths,
+                                       _wants_grad(q1, q2, k1, k2, v, lambda_param))[0]
+    if not _wants_grad(q1, q2, k1, k2, v, lambda_param):
         out = sdiff_forward(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths, save=False)[0]
         return out if out.dtype == q1.dtype else out.to(q1.dtype)
     return DifferentialSoftmaxFunction.apply(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths)

@@ -5,7 +5,8 @@
     torch.ops.tda.rect_bwd(q, k, v, dout, beta, relu_power, normalize) -> (dq, dk, dv)
     torch.ops.tda.diff_bwd(q1, q2, k1, k2, v, dout, beta, lambda_param, relu_power, normalize,
                            need_dlam) -> (dq1, dq2, dk1, dk2, dv, dlambda)
-    torch.ops.tda.sdiff_fwd(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths) -> (out, o12, lse)
+    torch.ops.tda.sdiff_fwd(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths, save=True)
+                            -> (out, o12, lse)
     torch.ops.tda.sdiff_bwd(q1, q2, k1, k2, v, dout, o12, lse, lambda_param, scale, causal, key_lengths,
                             need_dlam) -> (dq1, dq2, dk1, dk2, dv, dlambda)
 
@@ -128,15 +129,20 @@ diff_fwd.register_autograd(_diff_backward, setup_context=_diff_setup)
 # ------------------------------------------------- softmax differential attention
 @torch.library.custom_op("tda::sdiff_fwd", mutates_args=())
 def sdiff_fwd(q1: Tensor, q2: Tensor, k1: Tensor, k2: Tensor, v: Tensor, lambda_param: Tensor, scale: float,
-              causal: bool, key_lengths: Tensor | None) -> tuple[Tensor, Tensor, Tensor]:
-    """Softmax differential attention: (out, o12, lse), the last two for the backward."""
-    out, o12, lse = sdiff.sdiff_forward(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths)
+              causal: bool, key_lengths: Tensor | None, save: bool = True) -> tuple[Tensor, Tensor, Tensor]:
+    """Softmax differential attention: (out, o12, lse), the last two for the
+    backward; they are empty, and there is none, when ``save`` is False."""
+    out, o12, lse = sdiff.sdiff_forward(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths, save)
+    if not save:
+        o12, lse = (q1.new_empty((0,), dtype=torch.float32) for _ in range(2))
     return out.to(q1.dtype), o12, lse
 
 
 @sdiff_fwd.register_fake
-def _sdiff_fwd_fake(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths):
+def _sdiff_fwd_fake(q1, q2, k1, k2, v, lambda_param, scale, causal, key_lengths, save=True):
     shape = q1.shape
+    if not save:
+        return q1.new_empty(shape), *(q1.new_empty((0,), dtype=torch.float32) for _ in range(2))
     return (q1.new_empty(shape), q1.new_empty((2, *shape), dtype=torch.float32),
             q1.new_empty((2, shape[0], shape[1], shape[2]), dtype=torch.float32))
 
@@ -160,7 +166,7 @@ def _sdiff_bwd_fake(q1, q2, k1, k2, v, dout, o12, lse, lambda_param, scale, caus
 
 
 def _sdiff_setup(ctx, inputs, output):
-    q1, q2, k1, k2, v, lam, scale, causal, key_lengths = inputs
+    q1, q2, k1, k2, v, lam, scale, causal, key_lengths, _save = inputs
     _out, o12, lse = output
     ctx.save_for_backward(q1, q2, k1, k2, v, lam, key_lengths, o12, lse)
     ctx.args = (scale, causal)
@@ -170,11 +176,11 @@ def _sdiff_setup(ctx, inputs, output):
 def _sdiff_backward(ctx, dout, _do12, _dlse):
     q1, q2, k1, k2, v, lam, key_lengths, o12, lse = ctx.saved_tensors
     if dout is None:
-        return (None,) * 9
+        return (None,) * 10
     scale, causal = ctx.args
     need = bool(ctx.needs_input_grad[5])
     g = torch.ops.tda.sdiff_bwd(q1, q2, k1, k2, v, dout, o12, lse, lam, scale, causal, key_lengths, need)
-    return g[0], g[1], g[2], g[3], g[4], (g[5] if need else None), None, None, None
+    return g[0], g[1], g[2], g[3], g[4], (g[5] if need else None), None, None, None, None
 
 
 sdiff_fwd.register_autograd(_sdiff_backward, setup_context=_sdiff_setup)

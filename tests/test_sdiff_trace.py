@@ -45,3 +45,27 @@ def test_compile_fullgraph(grad):
     if grad:
         out.float().sum().backward()
         assert all(x.grad.shape == x.shape for x in xs)
+
+
+def saved_shapes(fn, xs):
+    """Shapes of the operator's outputs in the graph that torch.compile makes of fn."""
+    seen = []
+
+    def backend(gm, _example):
+        seen.extend(tuple(t.shape for t in n.meta["example_value"]) for n in gm.graph.nodes if "sdiff_fwd" in str(n.target))
+        return gm.forward
+
+    torch._dynamo.reset()
+    torch.compile(fn, fullgraph=True, backend=backend)(*xs)
+    return seen
+
+
+def test_compiled_inference_keeps_nothing_for_a_backward():
+    """o12 and lse are four times the output's bytes."""
+    fn = lambda *a: tda_b200.differential_softmax_attention(*a, 0.5)
+    xs = on_meta()
+    assert saved_shapes(fn, xs) == [(SHAPES[0], (0,), (0,))]
+    wants = [x.requires_grad_(True) for x in on_meta()]
+    assert saved_shapes(fn, wants) == [(SHAPES[0], (2, *SHAPES[0]), (2, *SHAPES[0][:3]))]
+    with torch.no_grad():
+        assert saved_shapes(fn, wants) == [(SHAPES[0], (0,), (0,))]
