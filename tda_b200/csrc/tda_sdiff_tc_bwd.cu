@@ -58,6 +58,7 @@ struct KvBars {
   uint64_t slot_full[4], slot_empty[4], tab_full[kTab], tab_empty[kTab];
   uint32_t tmem_base;
   int abort_flag;
+  int weight_exp, ds_exp;  // fp16: see kv_exponents
 };
 
 struct KvWork {
@@ -196,6 +197,19 @@ __device__ void kv_issue(uint8_t* smem, KvBars* bars, const WaitCtl& ctl, uint32
   }
 }
 
+// fp16 keeps its bits between 2^-14 and 2^16 alone: weights enter the products times
+// 2^weight_exp, at most 2^14 with lambda, dS times 2^ds_exp, and the accumulators are
+// scaled back.  One thread finds both while the others set up; they are read
+// again at the end, since registers kept for them cost dq 5%.
+template <int D>
+__device__ void kv_exponents(const SdParams& p, KvBars* bars, const KvWork& w) {
+  float largest = 1.0f;
+  for (int h = w.kvh * p.group; h < (w.kvh + 1) * p.group; ++h) largest = fmaxf(largest, fabsf(lambda_at(p.lam, w.b, h)));
+  bars->weight_exp = 14 - exponent_above(largest);
+  bars->ds_exp = ds_exponent(p, w.b, w.kvh, D, largest);
+}
+__device__ __forceinline__ int again(const int& x) { return *const_cast<const volatile int*>(&x); }
+
 // 32 accumulator columns of this thread's row, scaled, into the staged 16-bit tile
 template <int D, bool F16>
 __device__ __forceinline__ void stage_accumulator(uint8_t* boxes, uint32_t col, int row, int wg, float scale, bool zero) {
@@ -246,16 +260,8 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
   const bool dead = key >= len;          // past the sequence's length: no weight, whatever K and V hold there
   const bool lone = len <= 1;            // weight 1 whatever the score: no dS
   const float c = p.c;
-  // fp16 keeps its bits between 2^-14 and 2^16 alone: the weights enter times 2^k, at
-  // most 2^14 with lambda, dS times 2^e, and the accumulators are scaled back.
-  int k = 0, e = 0;
-  if constexpr (F16) {
-    float largest = 1.0f;
-    for (int h = w.kvh * p.group; h < (w.kvh + 1) * p.group; ++h) largest = fmaxf(largest, fabsf(lambda_at(p.lam, w.b, h)));
-    k = 14 - exponent_above(largest);
-    e = ds_exponent(p, w.b, w.kvh, D, largest);
-  }
-  const float kf = static_cast<float>(k), more = exp2i(e - k);
+  const float kf = F16 ? static_cast<float>(bars->weight_exp) : 0.f;
+  const float more = F16 ? exp2i(bars->ds_exp - bars->weight_exp) : 1.0f;
   bool ok = true;
   int t = 0;
   if (w.per_map > 0) ok = wait_inline_warp(&bars->v_full, 0, ctl, ST_KW);
@@ -329,8 +335,8 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
     if (ok && w.per_map > 0) ok = wait_inline_warp(&bars->map_done, m, ctl, ST_KW);
     tc_fence_after();
     if (ok) {
-      stage_accumulator<D, F16>(smem, tmem + lane_off + C::kDK, row, wg, p.scale * exp2i(-e), w.per_map == 0);
-      if (m == 1) stage_accumulator<D, F16>(smem + C::kTileBytes, tmem + lane_off + C::kDV, row, wg, exp2i(-k), w.per_map == 0);
+      stage_accumulator<D, F16>(smem, tmem + lane_off + C::kDK, row, wg, F16 ? p.scale * exp2i(-again(bars->ds_exp)) : p.scale, w.per_map == 0);
+      if (m == 1) stage_accumulator<D, F16>(smem + C::kTileBytes, tmem + lane_off + C::kDV, row, wg, F16 ? exp2i(-again(bars->weight_exp)) : 1.0f, w.per_map == 0);
       fence_proxy_async_smem();
     }
     tc_fence_before();
@@ -397,6 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dkv_kernel(const __grid_
     at[8] = make_uint4(u[4], u[5], u[6], u[7]);
     fence_proxy_async_smem();
   }
+  if constexpr (F16)
+    if (threadIdx.x == 0) kv_exponents<D>(p, bars, w);
   if (warp == kIssue) {
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
@@ -442,6 +450,7 @@ struct QBars {
   uint64_t slot_full[8], slot_empty[8];
   uint32_t tmem_base;
   int abort_flag;
+  int ds_exp;  // fp16: dS enters the products times 2^ds_exp, by the exponent of the weights
 };
 
 // tile idx of the ring: K1, V, K2 of key tile idx / 3
@@ -555,13 +564,10 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
     minus_d[m] = t[kTile];
   }
   const float c = p.c;
-  int e = 0;  // dS enters the products times 2^e, by the exponent of the weights
   if constexpr (F16) {
-    e = ds_exponent(p, b, h / p.group, D, 1.0f);
-    minus_l[0] += static_cast<float>(e);
-    minus_l[1] += static_cast<float>(e);
+    minus_l[0] += static_cast<float>(bars->ds_exp);
+    minus_l[1] += static_cast<float>(bars->ds_exp);
   }
-  const float back = p.scale * exp2i(-e);
   const int last = p.causal ? min(len - 1, grow + off) : len - 1;
   bool ok = true;
   for (int t = 0; t < n && ok; ++t) {
@@ -628,6 +634,7 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
   tc_fence_after();
   uint8_t* stage = smem + C::kOffRing;
   if (ok) {
+    const float back = F16 ? p.scale * exp2i(-again(bars->ds_exp)) : p.scale;
     const float w2 = -lambda_at(p.lam, b, h) * back;
     stage_accumulator<D, F16>(stage, tmem + lane_off + C::dq_col(0), row, wg, back, n == 0);
     stage_accumulator<D, F16>(stage + C::kTileBytes, tmem + lane_off + C::dq_col(1), row, wg, w2, n == 0);
@@ -678,6 +685,8 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
     fence_mbar_init();
     if (n > 0) primed = q_prime<D, F16>(tp, smem, bars, b, h, kvh, qt, n);
   }
+  if constexpr (F16)
+    if (threadIdx.x == 0) bars->ds_exp = ds_exponent(p, b, kvh, D, 1.0f);
   if (warp == kIssue) {
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
