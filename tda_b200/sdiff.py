@@ -31,6 +31,7 @@ _CODE = {torch.float32: _lib.TDA_F32, torch.bfloat16: _lib.TDA_BF16, torch.float
 
 # Small calls are bound by the host: a stream object costs 2 us to make, its handle alone 0.1.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_dispatch_modes = torch._C._len_torch_dispatch_stack
 
 
 def launch(entry, device: torch.device, *args) -> None:
@@ -263,15 +264,21 @@ class DifferentialSoftmaxFunction(torch.autograd.Function):
 
 
 def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                return True
+    return False
 
 
 def _traced(q1) -> bool:
     """Whether the call is recorded or run without data (torch.compile, make_fx,
     fake and meta tensors, dispatch modes): then it is the registered operator.
     A plain call goes past it: small calls are bound by the host."""
-    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or isinstance(q1, torch.Tensor) and (type(q1) not in (torch.Tensor, torch.nn.Parameter) or q1.is_meta))
+    if torch.compiler.is_compiling() or _dispatch_modes():
+        return True
+    kind = type(q1)
+    return q1.is_meta if kind is torch.Tensor or kind is torch.nn.Parameter else isinstance(q1, torch.Tensor)
 
 
 def differential_softmax_attention(q1, q2, k1, k2, v, lambda_param, scale=None, causal=True, key_lengths=None):
