@@ -249,7 +249,8 @@ int tda_debug_stats(void* counters);
  * Softmax differential attention: out = (P1 - lambda P2) v with
  * P_m = softmax(scale q_m k_m^T) over the keys a query row sees: j <
  * key_lengths[b] (all when NULL) and, when causal, j <= i + k_len - q_len.  A
- * row that sees no key gives zeros (and no gradient).
+ * row that sees no key gives zeros (and no gradient); one whose scores hold a NaN
+ * or +infinity, or -infinity alone, is NaN.
  *
  * q1, q2: (batch, heads, q_len, head_dim); k1, k2, v: (batch, kv_heads, k_len,
  * head_dim), query head h reads kv head h / (heads / kv_heads).  strides:

@@ -7,8 +7,9 @@
 // Bound by the cache bytes, 3 (D/2 + D/16) a token and kv head (216 at D = 128),
 // and next to them by issuing: about 500 instructions a slab and warp.  Measured
 // on B200, D = 128, 32 query heads on 8: 64 requests of 8192 tokens 208 us (906 MB,
-// 4.4 TB/s, 67% of a copy's rate; issue slots 59%, logic pipe 53% busy), 128
-// uneven ones of up to 16384 383 us; the threshold form 149 us for 555 MB.
+// 4.4 TB/s, 67% of a copy's rate; issue slots 60%, logic pipe 53% busy), 128
+// uneven ones of up to 16384 380-435 us by their lengths; the threshold form 147 us
+// for 555 MB.
 // Each warp walks slabs of 16 tokens by itself: one bulk copy a slab into its
 // own ring in shared memory, several slabs ahead, no barrier with other warps.
 // The products are m16n8k16 with the cache as the A operand, stored in fragment

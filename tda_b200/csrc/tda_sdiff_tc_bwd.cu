@@ -17,9 +17,9 @@
 // value each (2^-9 / 2^-12 of an element, averaged over a row; P in dV with its
 // rest where rows see few keys, see few_tiles); sums, the
 // difference dP - D and the exponent stay in fp32.  O_1, O_2 come in fp32 for D.
-// Measured on B200, bf16, 8 heads of (8192, 128), causal: dkv 475 us, tensor pipe
-// 67% active (a step's four products take 2048 cycles of its 3000: weights of the
-// next step wait for S, S for the last weights' product); dq 331 us, 57% active
+// Measured on B200, bf16, 8 heads of (8192, 128), causal: dkv 473 us, tensor pipe
+// 66% active (a step's four products take 2048 cycles of its 3000: weights of the
+// next step wait for S, S for the last weights' product); dq 334 us, 55% active
 // (its warps' own work, 2 x 128 x 128 weights a tile, is longer than its products).
 #include <cstring>
 
@@ -83,7 +83,8 @@ __device__ void kv_prime(const SdTcParams& tp, uint8_t* smem, KvBars* bars, cons
 // on B200: dV 2.6e-3 -> 2.0e-3 of its 64-bit value (bf16, causal, 4 heads on 1,
 // 4096 of 128; its own rounding is 1.7e-3), dkv 1900 -> 1990 us at (4, 32 on 8,
 // 4096, 128) for 10 of its 528 tile pairs a map and head, where all of them take
-// 2450 us.  Longer uncausal calls keep 2.6e-3.
+// 2450 us.  Longer uncausal calls keep 2.6e-3: with it for all of their tiles the
+// backward takes 10-12% longer ((6, 16, 1999, 64) fp16 1142 -> 1250 us).
 __device__ __forceinline__ int few_tiles(const SdParams& p, int len, int n_qt) {
   if (len <= 512) return n_qt;
   return p.causal ? max(0, 512 - (p.Sk - p.Sq)) / kTile : 0;

@@ -20,9 +20,15 @@
 // pipe as a polynomial).  What bounds it is the hand-over: scores ready, 500
 // cycles to the row maximum, 1400 for the weights, 1300 until the products that
 // need them are done, for two maps in turn, 3200 a tile.  Measured on B200, bf16
-// (1,16,32768,128): 7.1 ms (7.9 under the power cap), 1240 TFLOP/s of executed
-// products; (8 heads, 8192): 256 us, tensor pipe 59% active, exponential unit 38%.
+// (1,16,32768,128): 7.7 to 8.2 ms by the card, 1080-1140 TFLOP/s of executed
+// products; (8 heads, 8192): 254 us, tensor pipe 59% active, exponential unit 38%.
 // Polynomials for 0 to 4 of 8 pairs differ by 3%.
+//
+// P_m enters its product as one 16-bit value, which leaves out with 1.4 to 1.6 times
+// the error of a single rounding (the most where rows see many keys and the maps'
+// common mean cancels).  A second product with the rounding rest brings that to 1.0 and
+// costs more than it is worth: 7.95 -> 12.6 ms at (1,16,32768,128), 374 -> 506 us at
+// (6,16,1999,64) fp16.
 #include <cstring>
 
 #include "tda_sdiff_tc.cuh"
