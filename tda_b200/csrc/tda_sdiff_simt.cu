@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(256) sdiff_simt_dq_kernel(const SdParams p) {
   qt = n_t - 1 - qt;
   const int b = bh / p.H, h = bh % p.H, kvh = h / p.group, i0 = qt * C::BT;
   const int len = keys_of(p, b);
-  int n_keys = len <= 1 ? 0 : len;  // a lone key's weight is 1 whatever its score: no gradient
+  int n_keys = len;
   if (p.causal) n_keys = max(0, min(n_keys, min(i0 + C::BT, p.Sq) + p.Sk - p.Sq));
   const float w = (m ? -lambda_at(p.lam, b, h) : 1.f) * p.scale;
   load_tile<T, D>(qs, p.q[m], b, h, i0, p.Sq);
@@ -399,8 +399,9 @@ __global__ void __launch_bounds__(256) sdiff_simt_dq_kernel(const SdParams p) {
 #pragma unroll
       for (int c = 0; c < C::R; ++c) {
         const float pr = exp2f(fmaf(s[r][c], p.c, -lse[r]));
+        const float dsx = pr * (dp[r][c] - del[r]);  // a lone key's is 0: its weight is 1 whatever its score, but for a NaN
         ps[(ty * C::R + r) * C::LP + tx + 16 * c] =
-            sees(p, i0 + ty * C::R + r, j0 + tx + 16 * c, len) ? pr * (dp[r][c] - del[r]) : 0.f;
+            sees(p, i0 + ty * C::R + r, j0 + tx + 16 * c, len) && !(len <= 1 && dsx == dsx) ? dsx : 0.f;
       }
     __syncwarp();
     accumulate<D>(o, ps, ks, ty, tx);
@@ -468,7 +469,8 @@ __global__ void __launch_bounds__(256) sdiff_simt_dkv_kernel(const SdParams p) {
             const bool on = i0 + x < p.Sq && sees(p, i0 + x, j0 + ty * C::R + r, len);
             const float pr = on ? w * exp2f(fmaf(s[r][c], p.c, -ls[x])) : 0.f;
             ps[(ty * C::R + r) * C::LP + x] = pr;
-            ds[(ty * C::R + r) * C::LP + x] = on && len > 1 ? pr * (dp[r][c] - es[x]) : 0.f;
+            const float dsx = pr * (dp[r][c] - es[x]);
+            ds[(ty * C::R + r) * C::LP + x] = on && !(len <= 1 && dsx == dsx) ? dsx : 0.f;  // a lone key's is 0, or NaN
           }
         __syncwarp();
         accumulate<D>(dv, ps, gs, ty, tx);

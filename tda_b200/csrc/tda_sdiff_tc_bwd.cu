@@ -259,7 +259,7 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
   const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
   const uint32_t s_col = tmem + lane_off + C::kS + 32 * wg, p_col = tmem + lane_off + C::kP + 32 * wg;
   const bool dead = key >= len;          // past the sequence's length: no weight, whatever K and V hold there
-  const bool lone = len <= 1;            // weight 1 whatever the score: no dS
+  const bool lone = len <= 1;            // weight 1 whatever the score: no dS, but of a NaN
   const float c = p.c;
   const float kf = F16 ? static_cast<float>(bars->weight_exp) : 0.f;
   const float more = F16 ? exp2i(bars->ds_exp - bars->weight_exp) : 1.0f;
@@ -323,7 +323,7 @@ __device__ void kv_work(const SdTcParams& tp, uint8_t* smem, KvBars* bars, const
         }
         if (masked) {
 #pragma unroll
-          for (int y = 0; y < 32; ++y) pr[y] = 32 * wg + y >= lo && !lone ? pr[y] : 0.f;
+          for (int y = 0; y < 32; ++y) pr[y] = 32 * wg + y >= lo && !(lone && pr[y] == pr[y]) ? pr[y] : 0.f;
         }
         store_weights<F16>(p_col, pr);
         tmem_wait_st();
@@ -570,6 +570,7 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
     minus_l[1] += static_cast<float>(bars->ds_exp);
   }
   const int last = p.causal ? min(len - 1, grow + off) : len - 1;
+  const bool lone = len <= 1;  // weight 1 whatever the score: no dS, but of a NaN
   bool ok = true;
   for (int t = 0; t < n && ok; ++t) {
     const bool masked = (t + 1) * kTile > len || (p.causal && (t + 1) * kTile - 1 > qt * kTile + off);
@@ -617,7 +618,7 @@ __device__ void q_work(const SdTcParams& tp, uint8_t* smem, QBars* bars, const W
       }
       if (masked) {
 #pragma unroll
-        for (int y = 0; y < 32; ++y) pr[y] = y <= lim ? pr[y] : 0.f;
+        for (int y = 0; y < 32; ++y) pr[y] = y <= lim && !(lone && pr[y] == pr[y]) ? pr[y] : 0.f;
       }
       // K rows past the length: zeroed (S is done with them) before the product with dS reads them
       if (tail) {
@@ -664,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) sdiff_tc_dq_kernel(const __grid_c
   qt = tp.n_qt - 1 - qt;  // longest rows first
   const int b = bh / p.H, h = bh % p.H, kvh = h / p.group;
   const int len = keys_of(p, b);
-  int n_keys = len <= 1 ? 0 : len;  // a lone key's weight is 1 whatever its score: no gradient
+  int n_keys = len;
   if (p.causal) n_keys = max(0, min(n_keys, min((qt + 1) * kTile, p.Sq) + p.Sk - p.Sq));
   const int n = (n_keys + kTile - 1) / kTile;
   int primed = 0;
