@@ -4,13 +4,14 @@
 //         and, when causal, j <= i + Sk - Sq;  a row that sees none gives zeros
 //   out = P_1 v - lambda P_2 v
 //   L_m(i) = log2 of the row's sum of 2^(scale log2(e) s_ij): P_ij = 2^(c s_ij - L_m(i));
-//            +infinity where the row sees no key
+//            +infinity where the row sees no key; NaN where its keys have no softmax
+//            (a NaN or +infinity among the scores, or -infinity alone)
 // Backward, with O_m = P_m v, dP = dout v^T, D_m = rowsum(dout O_m):
 //   dS_1 = P_1 (dP - D_1), dS_2 = -lambda P_2 (dP - D_2)
 //   dq_m = scale dS_m k_m, dk_m = scale dS_m^T q_m, dv = (P_1 - lambda P_2)^T dout
 //   dlambda = -sum_i D_2(i)
 // With a single key the weight is 1 whatever its score: dS is exactly zero, and
-// set so, since dP and D are sums in different orders.
+// set so where it is a number, since dP and D are sums in different orders.
 // Shared heads: query head h reads kv head h / (H / Hkv); dk and dv sum over the group.
 #pragma once
 
